@@ -262,6 +262,101 @@ int mlvc_b200_test_wait_expiry(mlvc_b200_backend* backend, size_t step_index, ui
 int mlvc_b200_set_debug_tensors(mlvc_b200_backend* backend, int enable);
 int mlvc_b200_read_tensor(mlvc_b200_backend* backend, const char* name, void* dst, size_t bytes, int* found);
 
+/* ------------------------------------------------------------------------
+ * Microscaled matrices, products and caches (no reference counterpart; no
+ * loaded graph needed).  Rows are held in blocks that share a scale,
+ * value = code * scale * tensor_scale:
+ *   0 mxfp4  codes E2M1, blocks of 32, scales powers of two (E8M0)
+ *   1 nvfp4  codes E2M1, blocks of 16, scales E4M3, one float per tensor
+ *   2 mxfp8  codes E4M3, blocks of 32, scales powers of two (E8M0)
+ * tensor_scale is 1 except for nvfp4.  A block that holds an infinity or a NaN
+ * reads back as NaN, and so does every product with it.
+ *
+ * All pointers are device addresses on the backend's device and all work is
+ * enqueued on `stream` (a CUstream handle; 0 is the legacy default stream)
+ * without a wait, a copy or an allocation; the caller keeps the memory alive
+ * and orders calls on several streams.  The first call loads the kernels'
+ * module, so it is made outside a stream capture.  Waits that ran out and
+ * cache rows with no place are reported by mlvc_b200_synchronize, after the
+ * stream has been waited for. */
+typedef struct mlvc_b200_matrix {  /* dense */
+    uint64_t data;
+    int32_t dtype;                 /* 0 = FP16, 2 = BF16, 3 = FP32 */
+    int32_t reserved;
+    int64_t rows, cols;
+    int64_t row_stride, col_stride; /* elements; inputs may repeat (stride 0) */
+} mlvc_b200_matrix;
+
+typedef struct mlvc_b200_mx_matrix {
+    int32_t format;
+    float tensor_scale;
+    int64_t rows, cols;
+    uint64_t data, scales;         /* 16-byte boundaries, sizes by mlvc_b200_mx_layout */
+} mlvc_b200_mx_matrix;
+
+typedef struct mlvc_b200_mx_cache {
+    int32_t format;
+    float tensor_scale;
+    int64_t pages, page_rows, cols; /* row `r` of page `p` is row p * page_rows + r */
+    uint64_t data, scales;         /* 16-byte boundaries, sizes by mlvc_b200_mx_cache_layout */
+} mlvc_b200_mx_cache;
+
+/* Where the packed rows of several sequences lie in a cache: packed row t with
+ * offsets[s] <= t < offsets[s + 1] is position starts[s] + t - offsets[s] of
+ * sequence s, in row position % page_rows of page
+ * pages[s][position / page_rows].  Rows outside the offsets and pages < 0 have
+ * no place: not written, read as zeros.  Positions outside the page table and
+ * pages outside the cache are treated so too, and reported. */
+typedef struct mlvc_b200_mx_rows {
+    uint64_t pages;                /* int32 [sequences, pages_per_sequence] */
+    int64_t pages_per_sequence;
+    uint64_t offsets;              /* int32 [sequences + 1], ascending */
+    uint64_t starts;               /* int32 [sequences], 0: all zero */
+    int64_t sequences;
+} mlvc_b200_mx_rows;
+
+/* Bytes of a quantised row, of all codes and of all scales.  Codes: row after
+ * row, columns padded to a multiple of 32 with zeros; two E2M1 codes a byte,
+ * the lower first.  Scales of a matrix: tiles of 128 rows x 4 scales, 512
+ * bytes, tile (row / 128) * ceil(scales of a row / 4) + column / 4, byte
+ * (row % 32) * 16 + (row / 32 % 4) * 4 + column % 4; scales of a cache: row
+ * after row. */
+int mlvc_b200_mx_layout(int format, int64_t rows, int64_t cols, size_t* pitch, size_t* data_bytes, size_t* scale_bytes);
+int mlvc_b200_mx_cache_layout(int format, int64_t pages, int64_t page_rows, int64_t cols, size_t* pitch,
+                              size_t* data_bytes, size_t* scale_bytes);
+
+int mlvc_b200_mx_quantise(mlvc_b200_backend* backend, const mlvc_b200_matrix* x, const mlvc_b200_mx_matrix* out,
+                          uint64_t stream);
+int mlvc_b200_mx_dequantise(mlvc_b200_backend* backend, const mlvc_b200_mx_matrix* m, const mlvc_b200_matrix* y,
+                            uint64_t stream);
+
+/* y = leaky(x . w^T + bias) + residual: x [rows, cols] dense (quantised to w's
+ * format with `tensor_scale` on the way) or, with x.data = 0, already
+ * quantised in `a`; w [outputs, cols]; y and residual of one type,
+ * [rows, outputs], columns contiguous (residual may be y itself); bias FP32
+ * [outputs] or 0; slope of negative results (1: none).  Sums are held in 32
+ * bits, y is rounded once.  Dense x needs a workspace on a 256-byte boundary
+ * that no other call uses meanwhile. */
+typedef struct mlvc_b200_mx_linear_args {
+    mlvc_b200_matrix x;
+    mlvc_b200_mx_matrix a, w;
+    mlvc_b200_matrix y, residual;  /* residual.data = 0: none */
+    uint64_t bias;
+    float slope, tensor_scale;
+    uint64_t workspace;
+    size_t workspace_bytes;
+} mlvc_b200_mx_linear_args;
+
+int mlvc_b200_mx_linear_workspace(int64_t rows, const mlvc_b200_mx_matrix* w, size_t* bytes);
+int mlvc_b200_mx_linear(mlvc_b200_backend* backend, const mlvc_b200_mx_linear_args* args, uint64_t stream);
+
+/* Quantises packed rows into their places / reads packed rows back.  Two rows
+ * of one call with the same place leave it undefined which one stays. */
+int mlvc_b200_mx_cache_write(mlvc_b200_backend* backend, const mlvc_b200_mx_cache* cache, const mlvc_b200_matrix* x,
+                             const mlvc_b200_mx_rows* rows, uint64_t stream);
+int mlvc_b200_mx_cache_read(mlvc_b200_backend* backend, const mlvc_b200_mx_cache* cache, const mlvc_b200_matrix* y,
+                            const mlvc_b200_mx_rows* rows, uint64_t stream);
+
 #ifdef __cplusplus
 }
 #endif

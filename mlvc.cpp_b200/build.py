@@ -1,8 +1,9 @@
 """Build libmlvc_b200.so in-tree.
 
-1. nvcc compiles csrc/kernels/module.cu (every kernel, one translation unit)
-   to an sm_100a cubin with -lineinfo.
-2. The cubin is embedded into the shared library with an assembler .incbin
+1. nvcc compiles csrc/kernels/module.cu (the codec's kernels, one translation
+   unit) and mx_module.cu (the microscaled kernels) to sm_100a cubins with
+   -lineinfo.
+2. The cubins are embedded into the shared library with an assembler .incbin
    (the reference embeds its fatbin the same way, cmake/EmbedBinary.cmake) and
    loaded at run time with cuModuleLoadData.
 3. g++ compiles the C++ host runtime (Driver API) and the C ABI and links
@@ -21,6 +22,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -58,14 +60,23 @@ def build(force=False, verbose=False):
     nvcc = shutil.which("nvcc") or str(CUDA / "bin" / "nvcc")
     BUILD.mkdir(exist_ok=True)
     LIB.parent.mkdir(exist_ok=True)
-    cubin = BUILD / "mlvc_b200_sm100a.cubin"
-    out = _run([nvcc, *ARCH, "-lineinfo", "-O3", "-std=c++17", "-cubin", "-Xptxas", "-v",
-                "-o", str(cubin), str(HERE / "csrc" / "kernels" / "module.cu")])
+    modules = {"": "module.cu", "_mx": "mx_module.cu"}
+
+    def compile_module(suffix):
+        cubin = BUILD / f"mlvc_b200{suffix}_sm100a.cubin"
+        return cubin, _run([nvcc, *ARCH, "-lineinfo", "-O3", "-std=c++17", "-cubin", "-Xptxas", "-v",
+                            "-o", str(cubin), str(HERE / "csrc" / "kernels" / modules[suffix])])
+
+    with ThreadPoolExecutor(len(modules)) as pool:
+        compiled = list(pool.map(compile_module, modules))
+    out = "".join(log for _, log in compiled)
     (BUILD / "ptxas.txt").write_text(out)
     blob = BUILD / "cubin_blob.S"
     blob.write_text(
-        ".section .rodata\n.balign 128\n.global mlvc_b200_cubin_start\n.global mlvc_b200_cubin_end\n"
-        f"mlvc_b200_cubin_start:\n.incbin \"{cubin}\"\nmlvc_b200_cubin_end:\n.byte 0\n"
+        ".section .rodata\n" + "".join(
+            f".balign 128\n.global mlvc_b200{s}_cubin_start\n.global mlvc_b200{s}_cubin_end\n"
+            f"mlvc_b200{s}_cubin_start:\n.incbin \"{cubin}\"\nmlvc_b200{s}_cubin_end:\n.byte 0\n"
+            for s, (cubin, _) in zip(modules, compiled)) +
         ".section .note.GNU-stack,\"\",@progbits\n")
     # The system g++ links libstdc++ dynamically; a statically linked copy
     # inside a library that is dlopen'ed next to the process's own libstdc++

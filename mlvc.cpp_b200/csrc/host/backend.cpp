@@ -267,6 +267,7 @@ Backend::~Backend()
     input_stage_dev_.clear();
     output_stage_dev_.clear();
     state_dev_.clear();
+    mx_.reset();
     if (module_)
         cuModuleUnload(module_);
     for (CUstream s : {copy_in_, copy_out_})
@@ -277,6 +278,19 @@ Backend::~Backend()
     if (stream_)
         cuStreamDestroy(stream_);
     cuDevicePrimaryCtxRelease(dev_);
+}
+
+Mx& Backend::mx()
+{
+    if (!mx_) {
+        if (offline_) {
+            mx_ = std::make_unique<Mx>(nullptr, sm_count_);
+        } else {
+            ContextGuard guard(ctx_);
+            mx_ = std::make_unique<Mx>(ctx_, sm_count_);
+        }
+    }
+    return *mx_;
 }
 
 CUfunction Backend::fn(const char* name)
@@ -2754,15 +2768,21 @@ void Backend::check_status()
 {
     unsigned int status = 0;
     check(cuMemcpyDtoH(&status, status_ptr_, sizeof(status)), "cuMemcpyDtoH(status)");
+    const unsigned int own = status;
+    if (mx_)
+        status |= mx_->take_status();
     if (status) {
         const unsigned int zero = 0;
-        cuMemcpyHtoD(status_ptr_, &zero, sizeof(zero));
+        if (own)
+            cuMemcpyHtoD(status_ptr_, &zero, sizeof(zero));
         std::ostringstream os;
         os << "mlvc-b200:";
         if (status & 0xffu)  // wait-timeout / alignment bits of the tensor-core kernels
             os << " a device-side wait timed out or a TMA destination was misaligned;";
         if (status & 0x100u)  // mlvc_gather_rows_f16 (reference: "cpu: GATHER index out of range")
             os << " GATHER index out of range;";
+        if (status & 0x200u)  // mlvc_mx_cache_*
+            os << " cache row outside the page table or page outside the cache;";
         os << " status 0x" << std::hex << status;
         throw std::runtime_error(os.str());
     }

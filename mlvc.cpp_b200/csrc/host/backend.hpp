@@ -13,6 +13,7 @@
 
 #include "driver.hpp"
 #include "graph.hpp"
+#include "mx.hpp"
 
 #include <cuda.h>
 
@@ -95,6 +96,10 @@ public:
     void extract_scales_device(CUdeviceptr z, const ScaleConfig& cfg, CUdeviceptr scales_0, CUdeviceptr scales_1);
     void integer_values_device(CUdeviceptr values, size_t count, CUdeviceptr symbols, CUdeviceptr out_of_range);
 
+    // Microscaled matrices, products and caches (no loaded graph needed); the
+    // module of their kernels is loaded by the first call.
+    Mx& mx();
+
     // Slot path: pinned host staging per slot, asynchronous submit, wait.
     void configure_slots(size_t count);
     size_t slot_count() const;
@@ -173,6 +178,7 @@ private:
     CUstream copy_in_ = nullptr, copy_out_ = nullptr;       // slot pipeline copies
     CUmodule module_ = nullptr;
     CUdeviceptr status_ptr_ = 0;
+    std::unique_ptr<Mx> mx_;
     int sm_count_ = 148;
     int max_smem_optin_ = 227 * 1024;
 

@@ -63,6 +63,45 @@ mlvc_b200::Backend& require(const mlvc_b200_backend* b)
     return *b->impl;
 }
 
+mlvc_b200::MxDense mx_dense(const mlvc_b200_matrix& m)
+{
+    return {m.data, m.dtype, m.rows, m.cols, m.row_stride, m.col_stride};
+}
+
+mlvc_b200::MxMatrix mx_matrix(const mlvc_b200_mx_matrix& m)
+{
+    return {m.format, m.tensor_scale, m.rows, m.cols, m.data, m.scales};
+}
+
+mlvc_b200::MxCache mx_cache(const mlvc_b200_mx_cache& c)
+{
+    return {c.format, c.tensor_scale, c.pages, c.page_rows, c.cols, c.data, c.scales};
+}
+
+mlvc_b200::MxRows mx_rows(const mlvc_b200_mx_rows& r)
+{
+    return {r.pages, r.pages_per_sequence, r.offsets, r.starts, r.sequences};
+}
+
+template <typename... P>
+void require_args(const P*... args)
+{
+    if ((!args || ...))
+        throw std::runtime_error("mlvc-b200: null argument");
+}
+
+void give_layout(const mlvc_b200::MxLayout& l, size_t* pitch, size_t* data_bytes, size_t* scale_bytes)
+{
+    if (pitch)
+        *pitch = l.pitch;
+    if (data_bytes)
+        *data_bytes = l.data_bytes;
+    if (scale_bytes)
+        *scale_bytes = l.scale_bytes;
+}
+
+CUstream to_stream(uint64_t stream) { return reinterpret_cast<CUstream>(stream); }
+
 }  // namespace
 
 extern "C" {
@@ -253,6 +292,74 @@ int mlvc_b200_integer_values(mlvc_b200_backend* backend, const uint16_t* values,
 int mlvc_b200_integer_values_noalloc(const uint16_t* values, size_t count, int32_t* symbols)
 {
     return guarded([&] { mlvc_b200::integer_values_noalloc(values, count, symbols); });
+}
+
+int mlvc_b200_mx_layout(int format, int64_t rows, int64_t cols, size_t* pitch, size_t* data_bytes, size_t* scale_bytes)
+{
+    return guarded([&] { give_layout(mlvc_b200::mx_layout(format, rows, cols), pitch, data_bytes, scale_bytes); });
+}
+
+int mlvc_b200_mx_cache_layout(int format, int64_t pages, int64_t page_rows, int64_t cols, size_t* pitch,
+                              size_t* data_bytes, size_t* scale_bytes)
+{
+    return guarded(
+        [&] { give_layout(mlvc_b200::mx_cache_layout(format, pages, page_rows, cols), pitch, data_bytes, scale_bytes); });
+}
+
+int mlvc_b200_mx_quantise(mlvc_b200_backend* backend, const mlvc_b200_matrix* x, const mlvc_b200_mx_matrix* out,
+                          uint64_t stream)
+{
+    return guarded([&] {
+        require_args(x, out);
+        require(backend).mx().quantise(mx_dense(*x), mx_matrix(*out), to_stream(stream));
+    });
+}
+
+int mlvc_b200_mx_dequantise(mlvc_b200_backend* backend, const mlvc_b200_mx_matrix* m, const mlvc_b200_matrix* y,
+                            uint64_t stream)
+{
+    return guarded([&] {
+        require_args(m, y);
+        require(backend).mx().dequantise(mx_matrix(*m), mx_dense(*y), to_stream(stream));
+    });
+}
+
+int mlvc_b200_mx_linear_workspace(int64_t rows, const mlvc_b200_mx_matrix* w, size_t* bytes)
+{
+    return guarded([&] {
+        require_args(w, bytes);
+        *bytes = mlvc_b200::mx_linear_workspace(rows, mx_matrix(*w));
+    });
+}
+
+int mlvc_b200_mx_linear(mlvc_b200_backend* backend, const mlvc_b200_mx_linear_args* args, uint64_t stream)
+{
+    return guarded([&] {
+        require_args(args);
+        const mlvc_b200::MxLinear l{mx_dense(args->x),        mx_matrix(args->a), mx_matrix(args->w),
+                                    mx_dense(args->y),        mx_dense(args->residual),
+                                    args->bias,               args->slope,        args->tensor_scale,
+                                    args->workspace,          args->workspace_bytes};
+        require(backend).mx().linear(l, to_stream(stream));
+    });
+}
+
+int mlvc_b200_mx_cache_write(mlvc_b200_backend* backend, const mlvc_b200_mx_cache* cache, const mlvc_b200_matrix* x,
+                             const mlvc_b200_mx_rows* rows, uint64_t stream)
+{
+    return guarded([&] {
+        require_args(cache, x, rows);
+        require(backend).mx().cache_write(mx_cache(*cache), mx_dense(*x), mx_rows(*rows), to_stream(stream));
+    });
+}
+
+int mlvc_b200_mx_cache_read(mlvc_b200_backend* backend, const mlvc_b200_mx_cache* cache, const mlvc_b200_matrix* y,
+                            const mlvc_b200_mx_rows* rows, uint64_t stream)
+{
+    return guarded([&] {
+        require_args(cache, y, rows);
+        require(backend).mx().cache_read(mx_cache(*cache), mx_dense(*y), mx_rows(*rows), to_stream(stream));
+    });
 }
 
 int mlvc_b200_configure_slots(mlvc_b200_backend* backend, size_t slot_count)

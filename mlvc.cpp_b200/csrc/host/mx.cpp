@@ -1,0 +1,405 @@
+#include "mx.hpp"
+
+#include "../kernels/mx_params.h"
+
+#include <algorithm>
+#include <cmath>
+#include <stdexcept>
+#include <string>
+
+extern "C" const unsigned char mlvc_b200_mx_cubin_start[];
+
+namespace mlvc_b200 {
+
+namespace {
+
+[[noreturn]] void refuse(const std::string& why) { throw std::runtime_error("mlvc-b200: " + why); }
+
+const char* const kFormatNames[3] = {"mxfp4", "nvfp4", "mxfp8"};
+const char* const kTypeNames[4] = {"f16", nullptr, "bf16", "f32"};
+
+void check_format(int format, float tensor_scale)
+{
+    if (format < 0 || format > 2)
+        refuse("unknown microscaled format " + std::to_string(format));
+    if (format == kNvFp4 ? !(std::isfinite(tensor_scale) && tensor_scale > 0.0f) : tensor_scale != 1.0f)
+        refuse(format == kNvFp4 ? "the tensor scale must be finite and positive"
+                                : "only nvfp4 has a tensor scale: it must be 1");
+    // 6 g and s g stay finite and normal
+    if (format == kNvFp4 && (tensor_scale > 0x1p100f || tensor_scale < 0x1p-100f))
+        refuse("the tensor scale must lie in [2^-100, 2^100]");
+}
+
+constexpr int64_t kMaxCols = int64_t{1} << 24, kMaxRows = int64_t{1} << 36;
+
+void check_size(int64_t rows, int64_t cols)
+{
+    if (cols < 1 || cols > kMaxCols)
+        refuse("a microscaled matrix has 1 to 2^24 columns");
+    if (rows < 0 || rows > kMaxRows)
+        refuse("a microscaled matrix has 0 to 2^36 rows");
+}
+
+size_t elem_size(int dtype) { return dtype == kMxF32 ? 4 : 2; }
+
+void check_dense(const MxDense& d, const char* what, bool output)
+{
+    if (d.dtype != kMxF16 && d.dtype != kMxBf16 && d.dtype != kMxF32)
+        refuse(std::string(what) + " must be FP16, BF16 or FP32");
+    check_size(d.rows, d.cols);
+    if (d.rows == 0)
+        return;
+    if (!d.data || d.data % elem_size(d.dtype))
+        refuse(std::string(what) + ": null or misaligned device pointer");
+    if (d.row_stride < 0 || d.col_stride < 0)
+        refuse(std::string(what) + ": negative stride");
+    if (output && ((d.rows > 1 && d.row_stride < 1) || (d.cols > 1 && d.col_stride < 1)))
+        refuse(std::string(what) + ": an output's elements must not overlap");
+    const int64_t limit = int64_t{1} << 60;
+    if (d.row_stride > limit / std::max<int64_t>(d.rows, 1) || d.col_stride > limit / d.cols)
+        refuse(std::string(what) + ": stride out of range");
+}
+
+void check_held(uint64_t data, uint64_t scales, const char* what)
+{
+    if (!data || !scales || data % 16 || scales % 16)
+        refuse(std::string(what) + ": data and scales must be device pointers on 16-byte boundaries");
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+int block_of(int format) { return format == kNvFp4 ? 16 : 32; }
+
+int chunks_of(int64_t cols) { return static_cast<int>(ceil_div(cols, 32) * 2); }
+
+size_t pitch_of(int format, int64_t cols) { return static_cast<size_t>(chunks_of(cols)) * (format == kMxFp8 ? 16 : 8); }
+
+int64_t k_tiles_of(int format, int64_t cols) { return ceil_div(ceil_div(cols, block_of(format)), 4); }
+
+// Rows are contiguous and every chunk of 16 values begins on a 32-byte
+// boundary, so that a lane moves its chunk with one (FP32: two) accesses.
+int wide(const MxDense& d)
+{
+    const uint64_t stride = static_cast<uint64_t>(d.row_stride) * elem_size(d.dtype);
+    return d.data % 32 == 0 && (d.rows <= 1 || stride % 32 == 0) && (d.col_stride == 1 || d.cols == 1);
+}
+
+// Order of functions_: the four conversions by type and format, then products.
+enum { kQuantise = 0, kDequantise = 9, kCacheWrite = 18, kCacheRead = 27, kGemm64 = 36, kGemm128 = 39, kFunctions = 42 };
+
+int convert_index(int base, int dtype, int format) { return base + (dtype == kMxF16 ? 0 : dtype == kMxBf16 ? 3 : 6) + format; }
+
+std::string function_name(int i)
+{
+    static const char* const conversions[4] = {"quantise", "dequantise", "cache_write", "cache_read"};
+    static const int types[3] = {kMxF16, kMxBf16, kMxF32};
+    if (i < kGemm64)
+        return std::string("mlvc_mx_") + conversions[i / 9] + "_" + kTypeNames[types[i % 9 / 3]] + "_" + kFormatNames[i % 3];
+    return std::string(i < kGemm128 ? "mlvc_mx_gemm64_" : "mlvc_mx_gemm128_") + kFormatNames[i % 3];
+}
+
+constexpr unsigned kGemmSmem = 227 * 1024;
+
+}  // namespace
+
+MxLayout mx_layout(int format, int64_t rows, int64_t cols)
+{
+    check_format(format, 1.0f);
+    check_size(rows, cols);
+    const size_t pitch = pitch_of(format, cols);
+    return {pitch, pitch * static_cast<size_t>(rows),
+            static_cast<size_t>(ceil_div(rows, 128) * k_tiles_of(format, cols)) * 512};
+}
+
+MxLayout mx_cache_layout(int format, int64_t pages, int64_t page_rows, int64_t cols)
+{
+    check_format(format, 1.0f);
+    if (pages < 1 || pages > 0x7FFFFFFF || page_rows < 1 || page_rows > 0x7FFFFFFF)
+        refuse("a cache has at least one page of at least one row, and below 2^31 of each");
+    if (pages > kMaxRows / page_rows)
+        refuse("a cache has at most 2^36 rows");
+    check_size(pages * page_rows, cols);
+    const size_t pitch = pitch_of(format, cols), rows = static_cast<size_t>(pages * page_rows);
+    return {pitch, pitch * rows, rows * (format == kNvFp4 ? chunks_of(cols) : chunks_of(cols) / 2)};
+}
+
+size_t mx_linear_workspace(int64_t rows, const MxMatrix& w)
+{
+    check_format(w.format, w.tensor_scale);
+    const MxLayout l = mx_layout(w.format, rows, w.cols);
+    return (l.data_bytes + 255) / 256 * 256 + l.scale_bytes;
+}
+
+Mx::Mx(CUcontext ctx, int sm_count) : ctx_(ctx), sm_count_(sm_count)
+{
+    if (!ctx_)
+        return;
+    check(cuModuleLoadData(&module_, mlvc_b200_mx_cubin_start), "cuModuleLoadData(mx)");
+    size_t bytes = 0;
+    check(cuModuleGetGlobal(&status_, &bytes, module_, "mlvc_b200_status"), "cuModuleGetGlobal(mx status)");
+}
+
+Mx::~Mx()
+{
+    if (module_)
+        cuModuleUnload(module_);
+}
+
+void Mx::require_device() const
+{
+    if (!ctx_)
+        refuse("planning-only backend cannot execute");
+}
+
+CUfunction Mx::fn(int index)
+{
+    static_assert(kFunctions <= sizeof(functions_) / sizeof(functions_[0]), "function table");
+    CUfunction& f = functions_[index];
+    if (!f) {
+        const std::string name = function_name(index);
+        CUfunction got = nullptr;
+        check(cuModuleGetFunction(&got, module_, name.c_str()), name.c_str());
+        if (index >= kGemm64)
+            check(cuFuncSetAttribute(got, CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES, kGemmSmem), name.c_str());
+        f = got;
+    }
+    return f;
+}
+
+unsigned int Mx::take_status()
+{
+    unsigned int status = 0;
+    if (!status_)
+        return 0;
+    check(cuMemcpyDtoH(&status, status_, sizeof(status)), "cuMemcpyDtoH(mx status)");
+    if (status) {
+        const unsigned int zero = 0;
+        check(cuMemcpyHtoD(status_, &zero, sizeof(zero)), "cuMemcpyHtoD(mx status)");
+    }
+    return status;
+}
+
+// A CTA of 256 threads takes up to 1024 chunks: up to 256 of a row, as many
+// rows as that leaves.  Small calls get fewer rows a CTA, down to one chunk a
+// thread, so that they reach more SMs.
+void Mx::convert(const MxDense& d, int format, float tensor_scale, uint64_t data, uint64_t scales, const MxCache* cache,
+                 const MxRows* rows, bool read, CUstream stream)
+{
+    require_device();
+    if (d.rows == 0)
+        return;
+    ContextGuard guard(ctx_);
+    MxConvertParams p{};
+    p.dense = reinterpret_cast<void*>(d.data);
+    p.row_stride = d.row_stride;
+    p.col_stride = d.col_stride;
+    p.rows = d.rows;
+    p.cols = static_cast<int>(d.cols);
+    p.chunks = chunks_of(d.cols);
+    p.cta_chunks = std::min(p.chunks, 256);
+    const int64_t columns = ceil_div(p.chunks, p.cta_chunks);
+    int64_t cta_rows = std::max(1, 1024 / p.cta_chunks);
+    const int64_t least = std::max(1, 256 / p.cta_chunks);
+    while (cta_rows > least && ceil_div(d.rows, cta_rows) * columns < 4 * sm_count_)
+        cta_rows = std::max(least, cta_rows / 2);
+    p.cta_rows = static_cast<int>(std::min<int64_t>(cta_rows, kMxCacheRowsMax));
+    p.vec = wide(d);
+    p.data = reinterpret_cast<uint8_t*>(data);
+    p.scales = reinterpret_cast<uint8_t*>(scales);
+    p.pitch = static_cast<long long>(pitch_of(format, d.cols));
+    p.k_tiles = static_cast<int>(k_tiles_of(format, d.cols));
+    p.scale_pitch = format == kNvFp4 ? p.chunks : p.chunks / 2;
+    p.tensor_scale = tensor_scale;
+    p.six_tensor_scale = 6.0f * tensor_scale;
+    if (cache) {
+        p.pages = reinterpret_cast<const int*>(rows->pages);
+        p.offsets = reinterpret_cast<const int*>(rows->offsets);
+        p.starts = reinterpret_cast<const int*>(rows->starts);
+        p.sequences = static_cast<int>(rows->sequences);
+        p.pages_per_sequence = static_cast<int>(rows->pages_per_sequence);
+        p.page_rows = static_cast<int>(cache->page_rows);
+        p.page_count = static_cast<int>(cache->pages);
+    }
+    const int base = cache ? (read ? kCacheRead : kCacheWrite) : (read ? kDequantise : kQuantise);
+    const int index = convert_index(base, d.dtype, format);
+    const int64_t grid = ceil_div(d.rows, p.cta_rows);
+    if (grid > 0x7FFFFFFF)
+        refuse("too many rows for one call");
+    void* args[] = {&p};
+    check(cuLaunchKernel(fn(index), static_cast<unsigned>(grid), static_cast<unsigned>(columns), 1, 256, 1, 1, 0, stream, args,
+                         nullptr),
+          "cuLaunchKernel(mx convert)");
+}
+
+void Mx::quantise(const MxDense& x, const MxMatrix& out, CUstream stream)
+{
+    check_format(out.format, out.tensor_scale);
+    check_dense(x, "x", false);
+    if (x.rows != out.rows || x.cols != out.cols)
+        refuse("x and the quantised matrix differ in shape");
+    if (out.rows)
+        check_held(out.data, out.scales, "quantised matrix");
+    convert(x, out.format, out.tensor_scale, out.data, out.scales, nullptr, nullptr, false, stream);
+}
+
+void Mx::dequantise(const MxMatrix& m, const MxDense& y, CUstream stream)
+{
+    check_format(m.format, m.tensor_scale);
+    check_dense(y, "y", true);
+    if (y.rows != m.rows || y.cols != m.cols)
+        refuse("y and the quantised matrix differ in shape");
+    if (m.rows)
+        check_held(m.data, m.scales, "quantised matrix");
+    convert(y, m.format, m.tensor_scale, m.data, m.scales, nullptr, nullptr, true, stream);
+}
+
+namespace {
+void check_cache(const MxCache& c, const MxDense& d, const MxRows& r, const char* what, bool output)
+{
+    check_format(c.format, c.tensor_scale);
+    mx_cache_layout(c.format, c.pages, c.page_rows, c.cols);
+    check_held(c.data, c.scales, "cache");
+    check_dense(d, what, output);
+    if (d.cols != c.cols)
+        refuse(std::string(what) + " and the cache differ in columns");
+    if (d.rows > 0x7FFFFFFF)
+        refuse("packed rows are counted in 32 bits");
+    if (r.sequences < 0 || r.sequences > 0x7FFFFFFE || r.pages_per_sequence < 0 || r.pages_per_sequence > 0x7FFFFFFF)
+        refuse("sequences and their pages are counted in 32 bits");
+    if (d.rows == 0)
+        return;
+    if (r.sequences < 1)
+        refuse("packed rows need at least one sequence");
+    if (!r.offsets || r.offsets % 4 || r.starts % 4 || r.pages % 4 || (r.pages_per_sequence && !r.pages))
+        refuse("page table, offsets or starts: null or misaligned device pointer");
+}
+}  // namespace
+
+void Mx::cache_write(const MxCache& c, const MxDense& x, const MxRows& r, CUstream stream)
+{
+    check_cache(c, x, r, "x", false);
+    convert(x, c.format, c.tensor_scale, c.data, c.scales, &c, &r, false, stream);
+}
+
+void Mx::cache_read(const MxCache& c, const MxDense& y, const MxRows& r, CUstream stream)
+{
+    check_cache(c, y, r, "y", true);
+    convert(y, c.format, c.tensor_scale, c.data, c.scales, &c, &r, true, stream);
+}
+
+void Mx::linear(const MxLinear& l, CUstream stream)
+{
+    const bool dense = l.x.data != 0 || l.a.data == 0;
+    const MxMatrix& w = l.w;
+    check_format(w.format, w.tensor_scale);
+    check_size(w.rows, w.cols);
+    const int64_t rows = dense ? l.x.rows : l.a.rows, cols = dense ? l.x.cols : l.a.cols;
+    if (dense) {
+        check_format(w.format, l.tensor_scale);
+        check_dense(l.x, "x", false);
+    } else {
+        check_format(l.a.format, l.a.tensor_scale);
+        check_size(rows, cols);
+        if (l.a.format != w.format)
+            refuse("x and the weights differ in format");
+    }
+    if (cols != w.cols)
+        refuse("x and the weights differ in columns");
+    if (w.rows < 1 || w.rows > kMaxCols)
+        refuse("weights have 1 to 2^24 rows");
+    if (rows > 0x7FFFFFFF - 127)
+        refuse("too many rows for one call");
+    check_dense(l.y, "y", true);
+    if (l.y.rows != rows || l.y.cols != w.rows)
+        refuse("y must have x's rows and one column for each row of the weights");
+    if (l.y.cols > 1 && l.y.col_stride != 1)
+        refuse("y's columns must be contiguous");
+    if (l.residual.data) {
+        check_dense(l.residual, "residual", false);
+        if (l.residual.dtype != l.y.dtype || l.residual.rows != rows || l.residual.cols != w.rows)
+            refuse("the residual must have y's type and shape");
+        if (l.residual.cols > 1 && l.residual.col_stride != 1)
+            refuse("the residual's columns must be contiguous");
+    }
+    if (l.bias % 4)
+        refuse("bias: misaligned device pointer");
+    if (!std::isfinite(l.slope))
+        refuse("the slope must be finite");
+    if (rows)
+        check_held(w.data, w.scales, "weights");
+    if (rows && !dense)
+        check_held(l.a.data, l.a.scales, "x");
+    if (dense && rows) {
+        if (l.workspace_bytes < mx_linear_workspace(rows, w) || !l.workspace || l.workspace % 256)
+            refuse("the workspace must hold " + std::to_string(mx_linear_workspace(rows, w)) +
+                   " bytes on a 256-byte boundary");
+    }
+    require_device();
+    if (rows == 0)
+        return;
+    if (!dense) {
+        product(l, l.a, stream);
+        return;
+    }
+    const MxLayout lay = mx_layout(w.format, rows, cols);
+    const MxMatrix a{w.format, l.tensor_scale, rows, cols, l.workspace, l.workspace + (lay.data_bytes + 255) / 256 * 256};
+    quantise(l.x, a, stream);
+    product(l, a, stream);
+}
+
+namespace {
+void encode_rows(CUtensorMap* map, uint64_t data, size_t pitch, int64_t rows, int box_rows)
+{
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(pitch), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
+    const cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)}, elem[2] = {1, 1};
+    check(cuTensorMapEncodeTiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, reinterpret_cast<void*>(data), dims, strides, box, elem,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
+          "cuTensorMapEncodeTiled(mx)");
+}
+}  // namespace
+
+void Mx::product(const MxLinear& l, const MxMatrix& a, CUstream stream)
+{
+    ContextGuard guard(ctx_);
+    const MxMatrix& w = l.w;
+    const int panel = w.format == kMxFp8 ? 128 : 256, step = panel / 4, words = panel / block_of(w.format) / 4;
+    MxGemmParams p{};
+    const size_t pitch = pitch_of(w.format, w.cols);
+    p.scales_a = reinterpret_cast<const uint8_t*>(a.scales);
+    p.scales_b = reinterpret_cast<const uint8_t*>(w.scales);
+    p.k_tiles = static_cast<int>(k_tiles_of(w.format, w.cols));
+    p.k_stages = static_cast<int>(ceil_div(w.cols, panel));
+    p.last_steps = static_cast<int>(ceil_div(w.cols - static_cast<int64_t>(p.k_stages - 1) * panel, step));
+    p.last_words = p.k_tiles - (p.k_stages - 1) * words;
+    p.M = static_cast<int>(a.rows);
+    p.N = static_cast<int>(w.rows);
+    p.bias = reinterpret_cast<const float*>(l.bias);
+    p.residual = reinterpret_cast<const void*>(l.residual.data);
+    p.residual_stride = l.residual.row_stride;
+    p.y = reinterpret_cast<void*>(l.y.data);
+    p.y_stride = l.y.row_stride;
+    p.y_dtype = l.y.dtype;
+    const size_t size = elem_size(l.y.dtype);
+    auto aligned = [&](const MxDense& d) {
+        return d.data % 16 == 0 && (d.rows <= 1 || static_cast<size_t>(d.row_stride) * size % 16 == 0);
+    };
+    p.vec = aligned(l.y) && (!l.residual.data || aligned(l.residual));
+    p.alpha = a.tensor_scale * w.tensor_scale;
+    p.slope = l.slope;
+    p.m_tiles = static_cast<int>(ceil_div(a.rows, 128));
+    const bool narrow = p.m_tiles * ceil_div(w.rows, 128) < sm_count_;
+    const int bn = narrow ? 64 : 128;
+    p.n_tiles = static_cast<int>(ceil_div(w.rows, bn));
+    if (static_cast<int64_t>(p.m_tiles) * p.n_tiles > 0x7FFFFFFF - 8 * p.n_tiles)
+        refuse("too many output tiles for one call");
+    encode_rows(&p.map_a, a.data, pitch, a.rows, 128);
+    encode_rows(&p.map_b, w.data, pitch, w.rows, bn);
+    void* args[] = {&p};
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(sm_count_, static_cast<int64_t>(p.m_tiles) * p.n_tiles));
+    check(cuLaunchKernel(fn((narrow ? kGemm64 : kGemm128) + w.format), grid, 1, 1, 320, 1, 1, kGemmSmem, stream, args, nullptr),
+          "cuLaunchKernel(mx product)");
+}
+
+}  // namespace mlvc_b200

@@ -1,0 +1,93 @@
+// Microscaled matrices, their products and the paged cache: argument checks,
+// layouts and launches.  The kernels live in a cubin of their own, which a
+// backend loads at its first call here.
+#pragma once
+
+#include "driver.hpp"
+
+#include <cuda.h>
+
+#include <cstddef>
+#include <cstdint>
+
+namespace mlvc_b200 {
+
+struct MxDense {  // a dense matrix in device memory; strides in elements
+    uint64_t data;
+    int dtype;  // 0 FP16, 2 BF16, 3 FP32
+    int64_t rows, cols, row_stride, col_stride;
+};
+
+struct MxMatrix {
+    int format;  // 0 mxfp4, 1 nvfp4, 2 mxfp8
+    float tensor_scale;
+    int64_t rows, cols;
+    uint64_t data, scales;
+};
+
+struct MxCache {
+    int format;
+    float tensor_scale;
+    int64_t pages, page_rows, cols;
+    uint64_t data, scales;
+};
+
+struct MxRows {  // where packed rows of sequences lie in a cache
+    uint64_t pages;
+    int64_t pages_per_sequence;
+    uint64_t offsets, starts;
+    int64_t sequences;
+};
+
+struct MxLinear {
+    MxDense x;   // data 0: `a` holds x already quantised
+    MxMatrix a, w;
+    MxDense y, residual;  // residual.data 0: none
+    uint64_t bias;        // FP32 [w.rows], 0: none
+    float slope;          // of negative results, 1: none
+    float tensor_scale;   // of x when it is quantised here
+    uint64_t workspace;
+    size_t workspace_bytes;
+};
+
+struct MxLayout {
+    size_t pitch, data_bytes, scale_bytes;
+};
+
+MxLayout mx_layout(int format, int64_t rows, int64_t cols);
+MxLayout mx_cache_layout(int format, int64_t pages, int64_t page_rows, int64_t cols);
+// Bytes that a linear call on `rows` rows of dense x needs as workspace.
+size_t mx_linear_workspace(int64_t rows, const MxMatrix& w);
+
+class Mx {
+public:
+    // ctx null: a planning-only backend; every call checks its arguments and
+    // then refuses to execute.
+    Mx(CUcontext ctx, int sm_count);
+    ~Mx();
+    Mx(const Mx&) = delete;
+    Mx& operator=(const Mx&) = delete;
+
+    void quantise(const MxDense& x, const MxMatrix& out, CUstream stream);
+    void dequantise(const MxMatrix& m, const MxDense& y, CUstream stream);
+    void linear(const MxLinear& l, CUstream stream);
+    void cache_write(const MxCache& c, const MxDense& x, const MxRows& r, CUstream stream);
+    void cache_read(const MxCache& c, const MxDense& y, const MxRows& r, CUstream stream);
+    // The module's status word, cleared by the read.
+    unsigned int take_status();
+
+private:
+    CUfunction fn(int index);
+    void convert(const MxDense& d, int format, float tensor_scale, uint64_t data, uint64_t scales, const MxCache* cache,
+                 const MxRows* rows, bool read, CUstream stream);
+    void product(const MxLinear& l, const MxMatrix& a, CUstream stream);
+    void require_device() const;
+
+    CUcontext ctx_ = nullptr;
+    CUmodule module_ = nullptr;
+    CUdeviceptr status_ = 0;
+    int sm_count_ = 0;
+    CUfunction functions_[64] = {};
+};
+
+}  // namespace mlvc_b200

@@ -1,0 +1,357 @@
+// Device primitives of the microscaled formats: block quantisation, reading
+// back, and the block-scaled tensor-core instructions.
+#pragma once
+
+#include "mx_params.h"
+#include "sm100.cuh"
+
+#include <cuda_bf16.h>
+
+namespace mlvc_b200 {
+
+// A cache row whose position has no place in the page table, or a page number
+// outside the cache.
+constexpr unsigned int kStatusCachePage = 0x200u;
+
+template <int F>
+struct Mx {
+    static constexpr bool kIsNv = F == kNvFp4;
+    static constexpr bool kIs8 = F == kMxFp8;
+    static constexpr int kBlock = kIsNv ? 16 : 32;
+    static constexpr int kChunkBytes = kIs8 ? 16 : 8;   // 16 values
+    static constexpr int kExponentMax = kIs8 ? 8 : 2;   // of the largest code
+    static constexpr int kPanelValues = kIs8 ? 128 : 256;           // values in 128 bytes
+    static constexpr int kWords = kPanelValues / kBlock / 4;        // scale tiles (4 scales a row) in a panel
+};
+
+// -------------------------------------------------------- dense elements
+template <int DT>
+struct Dense;
+template <>
+struct Dense<kMxF16> {
+    using T = __half;
+    static __device__ __forceinline__ float load(const T* p) { return __half2float(*p); }
+    static __device__ __forceinline__ T pack(float v) { return __float2half_rn(v); }
+    static __device__ __forceinline__ void unpack(uint32_t w, float& a, float& b) { unpack_h2(w, a, b); }
+    static __device__ __forceinline__ uint32_t pack2(float a, float b) { return pack_h2(a, b); }
+};
+template <>
+struct Dense<kMxBf16> {
+    using T = __nv_bfloat16;
+    static __device__ __forceinline__ float load(const T* p) { return __bfloat162float(*p); }
+    static __device__ __forceinline__ T pack(float v) { return __float2bfloat16_rn(v); }
+    static __device__ __forceinline__ void unpack(uint32_t w, float& a, float& b)
+    {
+        a = __uint_as_float(w << 16);
+        b = __uint_as_float(w & 0xFFFF0000u);
+    }
+    static __device__ __forceinline__ uint32_t pack2(float a, float b)
+    {
+        __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<uint32_t*>(&h);
+    }
+};
+template <>
+struct Dense<kMxF32> {
+    using T = float;
+    static __device__ __forceinline__ float load(const T* p) { return *p; }
+    static __device__ __forceinline__ T pack(float v) { return v; }
+};
+
+// 32-byte accesses: one per lane covers a chunk of 16-bit values, so a warp
+// touches whole sectors only.
+__device__ __forceinline__ void load32(const void* p, uint32_t (&w)[8])
+{
+    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(p));
+}
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8])
+{
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+
+// 16 values of a dense row from column `col`; columns from `cols` on read as 0.
+template <int DT>
+__device__ __forceinline__ void load_chunk(const void* dense, long long row_at, long long col_stride, int col, int cols,
+                                           int vec, float (&v)[16])
+{
+    using D = Dense<DT>;
+    const typename D::T* p = static_cast<const typename D::T*>(dense) + row_at;
+    if (vec && col + 16 <= cols) {
+        uint32_t w[8];
+        load32(p + col, w);
+        if constexpr (DT == kMxF32) {
+            uint32_t u[8];
+            load32(p + col + 8, u);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                v[i] = __uint_as_float(w[i]);
+                v[8 + i] = __uint_as_float(u[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                D::unpack(w[i], v[2 * i], v[2 * i + 1]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        v[i] = col + i < cols ? D::load(p + (col + i) * col_stride) : 0.0f;
+}
+
+template <int DT>
+__device__ __forceinline__ void store_chunk(void* dense, long long row_at, long long col_stride, int col, int cols,
+                                            int vec, const float (&v)[16])
+{
+    using D = Dense<DT>;
+    typename D::T* p = static_cast<typename D::T*>(dense) + row_at;
+    if (vec && col + 16 <= cols) {
+        uint32_t w[8];
+        if constexpr (DT == kMxF32) {
+            uint32_t u[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                w[i] = __float_as_uint(v[i]);
+                u[i] = __float_as_uint(v[8 + i]);
+            }
+            store32(p + col, w);
+            store32(p + col + 8, u);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                w[i] = D::pack2(v[2 * i], v[2 * i + 1]);
+            store32(p + col, w);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        if (col + i < cols)
+            p[(col + i) * col_stride] = D::pack(v[i]);
+}
+
+// ------------------------------------------------------ block arithmetic
+// Eight E2M1 codes of v[0..7], the first in the lowest four bits; nearest,
+// ties to even, larger magnitudes become 6.
+__device__ __forceinline__ uint32_t e2m1x8(const float* v)
+{
+    uint32_t r;
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+        "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+        : "=r"(r)
+        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+    return r;
+}
+
+// Four E4M3 codes of v[0..3], the first in the lowest byte; larger magnitudes
+// become 448.
+__device__ __forceinline__ uint32_t e4m3x4(const float* v)
+{
+    uint32_t r;
+    asm("{\n\t.reg .b16 l, h;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n\t"
+        "mov.b32 %0, {l, h};\n\t}"
+        : "=r"(r)
+        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]));
+    return r;
+}
+
+__device__ __forceinline__ void e4m3x2_to_floats(uint32_t two, float& a, float& b)
+{
+    uint32_t h;
+    asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(h) : "r"(two));
+    unpack_h2(h, a, b);
+}
+
+// The value a scale byte stands for.
+template <int F>
+__device__ __forceinline__ float scale_value(uint32_t s)
+{
+    if constexpr (Mx<F>::kIsNv) {
+        float a, b;
+        e4m3x2_to_floats(s & 0xFFu, a, b);
+        return a;
+    } else {
+        // 0 stands for 2^-127, a subnormal float; 255 for NaN
+        return s == 0 ? __uint_as_float(1u << 22) : s == 255 ? __uint_as_float(0x7FFFFFFFu) : __uint_as_float(s << 23);
+    }
+}
+
+// One chunk's codes and its block's scale byte.  In the 32-value formats two
+// neighbouring lanes hold a block's halves, so all lanes of a warp call this.
+//
+//   mx: e = max(floor(log2 max|v|) - emax, -127): the exponent field of the
+//       float is that floor; codes of v * 2^-e, an exact product.
+//   nv: s = e4m3(max|v| / (6 g)); codes of v / (s g).  The quotient is the
+//       correctly rounded one (reciprocal, product, one correction by the
+//       remainder), because values on the middle between two codes are common
+//       in 16-bit inputs and v * (1 / (s g)) alone would leave that middle.
+//
+// A block with an infinity or a NaN gets the NaN scale and zero codes: all of
+// it reads back as NaN and so does every product with it.
+template <int F>
+__device__ __forceinline__ void quantise_chunk(float (&v)[16], float tensor_scale, float six_tensor_scale,
+                                               uint32_t (&codes)[4], uint32_t& scale)
+{
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);  // orders NaN above infinity above the finite
+    if constexpr (!Mx<F>::kIsNv)
+        m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+    const bool finite = m < 0x7F800000u;
+    if constexpr (Mx<F>::kIsNv) {
+        const float want = __fdiv_rn(__uint_as_float(m), six_tensor_scale);
+        const float w4[4] = {want, 0.0f, 0.0f, 0.0f};
+        scale = finite ? e4m3x4(w4) & 0xFFu : 0x7Fu;
+        const float r = scale_value<F>(scale) * tensor_scale;
+        if (!finite || !(r > 0.0f)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                v[i] = finite ? v[i] * 0.0f : 0.0f;  // zeros keep their sign
+        } else if (scale != 0x7Eu && r > 0x1p-100f && r < 0x1p100f) {
+            // |v / r| stays below 8 here, so nothing overflows, and what
+            // underflows is far below the smallest code's half
+            const float inv = __frcp_rn(r);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float q = v[i] * inv;
+                v[i] = fmaf(-fmaf(q, r, -v[i]), inv, q);  // a zero keeps its sign this way round
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                v[i] = __fdiv_rn(v[i], r);
+        }
+    } else {
+        const int e = static_cast<int>(m >> 23) - Mx<F>::kExponentMax;
+        scale = finite ? static_cast<uint32_t>(max(e, 0)) : 255u;
+        const float inv = finite ? __uint_as_float((254u - scale) << 23) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            v[i] = finite ? v[i] * inv : 0.0f;
+    }
+    if constexpr (Mx<F>::kIs8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            codes[i] = e4m3x4(&v[4 * i]);
+    } else {
+        codes[0] = e2m1x8(&v[0]);
+        codes[1] = e2m1x8(&v[8]);
+        codes[2] = codes[3] = 0;
+    }
+}
+
+// The values that a chunk's codes stand for: code * scale is exact, the tensor
+// scale's product is rounded once.
+template <int F>
+__device__ __forceinline__ void read_chunk(const uint32_t (&codes)[4], uint32_t scale, float tensor_scale,
+                                           float (&v)[16])
+{
+    const float s = scale_value<F>(scale);
+    if constexpr (Mx<F>::kIs8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            e4m3x2_to_floats(codes[i] & 0xFFFFu, v[4 * i], v[4 * i + 1]);
+            e4m3x2_to_floats(codes[i] >> 16, v[4 * i + 2], v[4 * i + 3]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            uint32_t h0, h1, h2, h3;
+            asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+                "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+                "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+                "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+                "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+                "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+                : "=r"(h0), "=r"(h1), "=r"(h2), "=r"(h3)
+                : "r"(codes[i]));
+            unpack_h2(h0, v[8 * i], v[8 * i + 1]);
+            unpack_h2(h1, v[8 * i + 2], v[8 * i + 3]);
+            unpack_h2(h2, v[8 * i + 4], v[8 * i + 5]);
+            unpack_h2(h3, v[8 * i + 6], v[8 * i + 7]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        v[i] *= s;
+        if constexpr (Mx<F>::kIsNv)
+            v[i] *= tensor_scale;
+    }
+}
+
+// Byte of scale column `column` (of a row's blocks) in a matrix's scale tiles.
+__device__ __forceinline__ long long scale_at(long long row, int column, int k_tiles)
+{
+    return ((row >> 7) * k_tiles + (column >> 2)) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (column & 3);
+}
+
+// ------------------------------------------------- tensor core, block scaled
+// Instruction descriptor: operand formats, scale format, N / 8, M / 16; the
+// scale ids (which byte of the 4-scale word a step uses) are added per step.
+template <int F>
+__host__ __device__ constexpr uint32_t mx_idesc(uint32_t m, uint32_t n)
+{
+    const uint32_t type = F == kMxFp8 ? 0u : 1u;  // E4M3 / E2M1
+    return (type << 7) | (type << 10) | ((n >> 3) << 17) | ((F == kNvFp4 ? 0u : 1u) << 23) | ((m >> 4) << 24);
+}
+
+// D (+)= (A * SA) (B * SB)^T for one 32-byte step of both operands: 64 values
+// of 4 bits (4 or 2 scales a row) or 32 of 8 bits (1 scale a row).  `id` is the
+// first scale's byte in its word.
+template <int F>
+__device__ __forceinline__ void umma_mx(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t id,
+                                        uint32_t tmem_sa, uint32_t tmem_sb, uint32_t accumulate)
+{
+    idesc |= (id << 4) | (id << 29);
+    if constexpr (F == kNvFp4)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+                tmem_d),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
+            : "memory");
+    else if constexpr (F == kMxFp4)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+                tmem_d),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+                tmem_d),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
+            : "memory");
+}
+
+// A scale tile (512 bytes of shared memory) into four TMEM columns, repeated
+// for each warp's 32 lanes.
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t saddr)
+{
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(smem_desc(saddr, 16, 128, 0))
+                 : "memory");
+}
+
+// Untiled copy into shared memory (16-byte multiples), completing on `bar`.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_u32(dst)),
+                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+}  // namespace mlvc_b200

@@ -1,0 +1,290 @@
+// Products of microscaled matrices on the tensor cores:
+//     y[m, n] = leaky(alpha * sum_k a[m, k] b[n, k] + bias[n]) + residual[m, n]
+// with a and b quantised along k, alpha the product of their tensor scales,
+// sums in 32 bits in tensor memory and one rounding to y's type.
+#include "mx.cuh"
+
+namespace mlvc_b200 {
+
+constexpr unsigned int kErrMxProducer = 0x1u;
+constexpr unsigned int kErrMxMma = 0x2u;
+constexpr unsigned int kErrMxEpilogue = 0x4u;
+
+// 32 results of one row from column `col`.
+template <int DT>
+__device__ __forceinline__ void mx_store_row(const MxGemmParams& p, long long row, int col, float (&v)[32])
+{
+    using D = Dense<DT>;
+    using T = typename D::T;
+    T* y = static_cast<T*>(p.y) + row * p.y_stride + col;
+    const T* res = p.residual ? static_cast<const T*>(p.residual) + row * p.residual_stride + col : nullptr;
+    if (p.vec && col + 32 <= p.N) {
+        constexpr int kPer = 16 / sizeof(T);  // values of a 16-byte access
+#pragma unroll
+        for (int i = 0; i < 32; i += kPer) {
+            if (res) {
+                const uint4 w = *reinterpret_cast<const uint4*>(res + i);
+                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if constexpr (DT == kMxF32) {
+                        v[i + k] += __uint_as_float(u[k]);
+                    } else {
+                        float a, b;
+                        D::unpack(u[k], a, b);
+                        v[i + 2 * k] += a;
+                        v[i + 2 * k + 1] += b;
+                    }
+                }
+            }
+            uint32_t o[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if constexpr (DT == kMxF32)
+                    o[k] = __float_as_uint(v[i + k]);
+                else
+                    o[k] = D::pack2(v[i + 2 * k], v[i + 2 * k + 1]);
+            }
+            *reinterpret_cast<uint4*>(y + i) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+        if (col + i < p.N)
+            y[i] = D::pack(res ? v[i] + D::load(res + i) : v[i]);
+}
+
+__device__ __forceinline__ void mx_finish(const MxGemmParams& p, long long row, int col, const uint32_t (&acc)[32])
+{
+    if (row >= p.M || col >= p.N)
+        return;
+    float v[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        const float b = p.bias && col + i < p.N ? p.bias[col + i] : 0.0f;
+        const float t = fmaf(__uint_as_float(acc[i]), p.alpha, b);
+        v[i] = t >= 0.0f ? t : t * p.slope;
+    }
+    if (p.y_dtype == kMxF16)
+        mx_store_row<kMxF16>(p, row, col, v);
+    else if (p.y_dtype == kMxBf16)
+        mx_store_row<kMxBf16>(p, row, col, v);
+    else
+        mx_store_row<kMxF32>(p, row, col, v);
+}
+
+constexpr int kMxGemmThreads = 320;  // warp 0 copies, warp 1 MMA, warps 2..9 epilogue
+constexpr int kMxMaxStages = 8;
+
+struct MxShared {
+    uint64_t full[kMxMaxStages];
+    uint64_t empty[kMxMaxStages];
+    uint64_t tmem_full[2];
+    uint64_t tmem_empty[2];
+    uint64_t drain;
+    uint32_t tmem_base;
+    int abort_flag;
+};
+
+// Stage: A panel (128 rows), B panel (BN rows), their scale tiles.
+template <int F, int BN>
+struct MxTile {
+    static constexpr int kBands = (BN + 127) / 128;  // 128-row bands of B's scales
+    static constexpr uint32_t kA = 128 * 128, kB = BN * 128;
+    static constexpr uint32_t kSA = Mx<F>::kWords * 512, kSB = kBands * kSA;
+    static constexpr uint32_t kStage = (kA + kB + kSA + kSB + 1023) / 1024 * 1024;
+    static constexpr int kStages = (227 * 1024 - 2048) / kStage < kMxMaxStages ? (227 * 1024 - 2048) / kStage : kMxMaxStages;
+};
+
+// Tiles in bands of 8 row tiles, so that the tiles in flight share operands.
+__device__ __forceinline__ void mx_tile_at(const MxGemmParams& p, int t, int& m, int& n)
+{
+    const int band = 8 * p.n_tiles;
+    const int g = t / band, r = t - g * band;
+    const int high = min(8, p.m_tiles - 8 * g);
+    n = r / high;
+    m = 8 * g + r - n * high;
+}
+
+template <int F, int BN>
+__device__ __forceinline__ void mx_gemm(const MxGemmParams& p)
+{
+    using T = MxTile<F, BN>;
+    constexpr int kWords = Mx<F>::kWords;
+    extern __shared__ __align__(1024) uint8_t smem_dyn[];
+    uint8_t* base = align_smem_1024(smem_dyn);
+    MxShared* sh = reinterpret_cast<MxShared*>(base);
+    uint8_t* stages = base + 1024;
+    static_assert(sizeof(MxShared) <= 1024, "header");
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < T::kStages; ++s) {
+            mbar_init(&sh->full[s], 1);
+            mbar_init(&sh->empty[s], 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&sh->tmem_full[s], 1);
+            mbar_init(&sh->tmem_empty[s], 256);
+        }
+        mbar_init(&sh->drain, 1);
+        sh->abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1)
+        tmem_alloc(&sh->tmem_base, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh->tmem_base;
+    const int total = p.m_tiles * p.n_tiles;
+    bool issuer = false;
+    uint32_t issued = 0;
+
+    if (warp == 0) {
+        if (elect_one()) {
+            uint32_t armed = 0, parity = 0;
+            int stage = 0;
+            uint32_t phase = 0;
+            for (int t = blockIdx.x; t < total && !sh->abort_flag; t += gridDim.x) {
+                int mt, nt;
+                mx_tile_at(p, t, mt, nt);
+                for (int k = 0; k < p.k_stages; ++k) {
+                    if (!mbar_wait(&sh->empty[stage], phase ^ 1u, &sh->abort_flag, kErrMxProducer))
+                        break;
+                    uint8_t* s = stages + stage * T::kStage;
+                    uint64_t* bar = &sh->full[stage];
+                    const uint32_t sbytes = 512u * (k + 1 == p.k_stages ? p.last_words : kWords);
+                    // bands past the last row of B have no scales
+                    const int bands = min(T::kBands, (p.N - nt * BN + 127) / 128);
+                    mbar_arrive_expect_tx(bar, T::kA + T::kB + sbytes * (1 + bands));
+                    tma_load_2d(s, &p.map_a, bar, k * 128, mt * 128);
+                    tma_load_2d(s + T::kA, &p.map_b, bar, k * 128, nt * BN);
+                    const long long word = static_cast<long long>(k) * kWords;
+                    bulk_load(s + T::kA + T::kB, p.scales_a + (static_cast<long long>(mt) * p.k_tiles + word) * 512,
+                              sbytes, bar);
+                    for (int b = 0; b < bands; ++b)
+                        bulk_load(s + T::kA + T::kB + T::kSA * (1 + b),
+                                  p.scales_b + ((static_cast<long long>(nt) * BN / 128 + b) * p.k_tiles + word) * 512, sbytes,
+                                  bar);
+                    armed |= 1u << stage;
+                    parity = (parity & ~(1u << stage)) | (phase << stage);
+                    if (++stage == T::kStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            if (sh->abort_flag) {  // no copy may land after this CTA has gone
+                volatile int never = 0;
+                for (int s = 0; s < T::kStages; ++s)
+                    if ((armed >> s) & 1u)
+                        mbar_wait(&sh->full[s], (parity >> s) & 1u, &never, kErrMxProducer);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (elect_one()) {
+            issuer = true;
+            constexpr uint32_t idesc = mx_idesc<F>(128, BN);
+            const uint32_t tmem_sa = tmem + 2 * BN, tmem_sb = tmem_sa + 4 * kWords;
+            int stage = 0;
+            uint32_t phase = 0, acc = 0, acc_phase = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
+                if (!mbar_wait(&sh->tmem_empty[acc], acc_phase ^ 1u, &sh->abort_flag, kErrMxMma))
+                    break;
+                tc_fence_after();
+                // rows of B inside its 128-row band of scales (BN = 64: the second half)
+                const uint32_t d = tmem + acc * BN;
+                int mt, nt;
+                mx_tile_at(p, t, mt, nt);
+                const uint32_t in_band = BN < 128 ? (nt * BN % 128) / 32 : 0;
+                for (int k = 0; k < p.k_stages; ++k) {
+                    if (!mbar_wait(&sh->full[stage], phase, &sh->abort_flag, kErrMxMma)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t s = smem_u32(stages + stage * T::kStage);
+                    const bool last = k + 1 == p.k_stages;
+                    const int words = last ? p.last_words : kWords, steps = last ? p.last_steps : 4;
+                    for (int w = 0; w < words; ++w) {
+                        tmem_copy_scales(tmem_sa + 4 * w, s + T::kA + T::kB + 512 * w);
+#pragma unroll
+                        for (int b = 0; b < T::kBands; ++b)
+                            tmem_copy_scales(tmem_sb + 4 * (w * T::kBands + b), s + T::kA + T::kB + T::kSA * (1 + b) + 512 * w);
+                    }
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks) {
+                        if (ks >= steps)
+                            break;
+                        const uint32_t w = ks * kWords / 4, id = kWords == 4 ? 0 : kWords == 2 ? (ks & 1) * 2 : ks;
+                        umma_mx<F>(d, smem_desc(s + ks * 32, 16, 1024, 2), smem_desc(s + T::kA + ks * 32, 16, 1024, 2), idesc,
+                                   id, tmem_sa + 4 * w, tmem_sb + 4 * w * T::kBands + in_band, (k | ks) != 0);
+                        ++issued;
+                    }
+                    umma_commit(&sh->empty[stage]);
+                    if (++stage == T::kStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok)
+                    break;
+                umma_commit(&sh->tmem_full[acc]);
+                acc ^= 1u;
+                acc_phase ^= acc == 0;
+            }
+        }
+        __syncwarp();
+    } else {
+        const int quadrant = warp & 3, group = (warp - 2) / 4;
+        uint32_t acc = 0, acc_phase = 0;
+        for (int t = blockIdx.x; t < total; t += gridDim.x) {
+            int mt, nt;
+            mx_tile_at(p, t, mt, nt);
+            // the whole warp goes on or none of it: the TMEM loads are collective
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait(&sh->tmem_full[acc], acc_phase, &sh->abort_flag, kErrMxEpilogue)))
+                break;
+            tc_fence_after();
+            for (int c = group * 32; c < BN; c += 64) {
+                uint32_t v[32];
+                tmem_ld32_nowait(tmem + acc * BN + c + (static_cast<uint32_t>(quadrant * 32) << 16), v);
+                tmem_wait_ld();
+                mx_finish(p, static_cast<long long>(mt) * 128 + quadrant * 32 + lane, nt * BN + c, v);
+                __syncwarp();
+            }
+            tc_fence_before();
+            mbar_arrive(&sh->tmem_empty[acc]);
+            acc ^= 1u;
+            acc_phase ^= acc == 0;
+        }
+        __syncwarp();
+    }
+    if (issuer && sh->abort_flag && issued) {  // MMAs in flight end before TMEM is freed
+        umma_commit(&sh->drain);
+        volatile int never = 0;
+        mbar_wait(&sh->drain, 0, &never, kErrMxMma);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+#define MLVC_MX_GEMM(NAME, F, BN)                                                                              \
+    extern "C" __global__ void __launch_bounds__(kMxGemmThreads, 1) NAME(const __grid_constant__ MxGemmParams p) \
+    {                                                                                                          \
+        mx_gemm<F, BN>(p);                                                                                     \
+    }
+MLVC_MX_GEMM(mlvc_mx_gemm64_mxfp4, kMxFp4, 64)
+MLVC_MX_GEMM(mlvc_mx_gemm64_nvfp4, kNvFp4, 64)
+MLVC_MX_GEMM(mlvc_mx_gemm64_mxfp8, kMxFp8, 64)
+MLVC_MX_GEMM(mlvc_mx_gemm128_mxfp4, kMxFp4, 128)
+MLVC_MX_GEMM(mlvc_mx_gemm128_nvfp4, kNvFp4, 128)
+MLVC_MX_GEMM(mlvc_mx_gemm128_mxfp8, kMxFp8, 128)
+
+}  // namespace mlvc_b200

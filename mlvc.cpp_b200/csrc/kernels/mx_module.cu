@@ -1,0 +1,9 @@
+// Translation unit of the microscaled kernels' cubin: a module of its own, so
+// that a program that never calls them does not load them.
+#include "sm100.cuh"
+
+extern "C" __device__ unsigned int mlvc_b200_status = 0;
+extern "C" __device__ unsigned long long mlvc_b200_wait_limit_ns = mlvc_b200::kWaitLimitNs;
+
+#include "mx_convert.cu"
+#include "mx_gemm.cu"

@@ -1,0 +1,69 @@
+// Parameter blocks of the microscaled kernels, shared by host and device.
+#pragma once
+
+#include <cuda.h>
+#include <stdint.h>
+
+namespace mlvc_b200 {
+
+// Element type of a dense matrix (the C ABI's dtype codes).
+enum MxDtype : int { kMxF16 = 0, kMxBf16 = 2, kMxF32 = 3 };
+
+// Formats: values are code * scale * tensor scale, one scale per block of a row.
+enum MxFormat : int {
+    kMxFp4 = 0,  // codes E2M1, blocks of 32, scales E8M0 (powers of two)
+    kNvFp4 = 1,  // codes E2M1, blocks of 16, scales E4M3, a float per tensor
+    kMxFp8 = 2,  // codes E4M3, blocks of 32, scales E8M0
+};
+
+// A dense matrix against its quantised form.  A chunk is 16 values of a row;
+// a row of the quantised form has an even number of chunks (columns are padded
+// to 32 with zeros).  Scales of a matrix lie in tiles of 128 rows x 4 scales,
+// 512 bytes each: byte (row % 32) * 16 + (row / 32 % 4) * 4 + column % 4, the
+// order in which the tensor core takes them; tiles of one 128-row band are
+// consecutive.  Scales of a cache lie row after row.
+struct MxConvertParams {
+    void* dense;
+    long long row_stride, col_stride;  // elements
+    long long rows;
+    int cols;
+    int chunks;                        // chunks of a quantised row (even)
+    int cta_rows, cta_chunks;          // what one CTA handles (cta_chunks even)
+    int vec;                           // dense rows begin on 32-byte boundaries and are contiguous
+    uint8_t* data;
+    uint8_t* scales;
+    long long pitch;                   // bytes of a quantised row
+    int k_tiles;                       // matrix: scale tiles of a 128-row band
+    int scale_pitch;                   // cache: scales of a row
+    float tensor_scale, six_tensor_scale;
+    // cache: where row t of the packed rows lies
+    const int* pages;                  // [sequences, pages_per_sequence], < 0: no page
+    const int* offsets;                // [sequences + 1]: first packed row of each sequence
+    const int* starts;                 // [sequences] position of a sequence's first packed row, or null for 0
+    int sequences, pages_per_sequence, page_rows, page_count;
+};
+
+constexpr int kMxCacheRowsMax = 64;  // rows of one CTA of a cache kernel
+
+// y = leaky(alpha * a . b^T + bias) + residual
+struct MxGemmParams {
+    CUtensorMap map_a, map_b;          // bytes [rows, pitch], boxes of 128 bytes x the tile's rows, 128-byte swizzle
+    const uint8_t* scales_a;
+    const uint8_t* scales_b;
+    int k_tiles;                       // scale tiles of a 128-row band
+    int k_stages;                      // 128-byte panels of a row
+    int last_steps;                    // MMA steps of the last panel (32 bytes each)
+    int last_words;                    // scale tiles of the last panel
+    int M, N;
+    int m_tiles, n_tiles;
+    const float* bias;                 // [N] or null
+    const void* residual;              // y's type, or null
+    long long residual_stride;
+    void* y;
+    long long y_stride;
+    int y_dtype;
+    int vec;                           // y and residual rows begin on 16-byte boundaries
+    float alpha, slope;
+};
+
+}  // namespace mlvc_b200

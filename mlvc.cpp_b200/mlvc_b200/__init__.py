@@ -19,6 +19,8 @@ from pathlib import Path
 
 import numpy as np
 
+from . import mx
+
 _PKG_ROOT = Path(__file__).resolve().parent.parent
 LIB_PATH = _PKG_ROOT / "lib" / "libmlvc_b200.so"
 _lib = None
@@ -106,6 +108,7 @@ EXPORTS = {
     "mlvc_b200_set_debug_tensors": ([ctypes.c_void_p, ctypes.c_int], ctypes.c_int),
     "mlvc_b200_read_tensor": ([ctypes.c_void_p, ctypes.c_char_p, ctypes.c_void_p, ctypes.c_size_t,
                                ctypes.POINTER(ctypes.c_int)], ctypes.c_int),
+    **mx.EXPORTS,
 }
 
 
@@ -263,6 +266,32 @@ class Backend:
         wait); the device uint32 at out_of_range_ptr, zeroed by the caller,
         becomes non-zero when a value is out of range."""
         _check(lib().mlvc_b200_integer_values_device(self._h, values_ptr, count, symbols_ptr, out_of_range_ptr))
+
+    # ------------------------------------------------------ microscaled
+    def _mx(self, fn, *args, stream):
+        _check(fn(self._h, *args, self.stream or 0 if stream is None else stream))
+
+    def mx_quantise(self, x, out, stream=None):
+        """Quantises the dense matrix x into the MxMatrix `out` of its shape."""
+        self._mx(lib().mlvc_b200_mx_quantise, ctypes.byref(mx._fill(mx.Matrix(), x)), ctypes.byref(out.c), stream=stream)
+
+    def mx_dequantise(self, m, y, stream=None):
+        """Reads the MxMatrix m back into the dense matrix y of its shape."""
+        self._mx(lib().mlvc_b200_mx_dequantise, ctypes.byref(m.c), ctypes.byref(mx._fill(mx.Matrix(), y)), stream=stream)
+
+    def mx_cache_write(self, cache, x, pages, offsets, starts=None, stream=None):
+        """Quantises the packed rows of several sequences into their places:
+        rows offsets[s] .. offsets[s + 1] of x become positions starts[s] ... of
+        sequence s, whose pages are pages[s] (device int32 arrays [sequences,
+        pages], [sequences + 1], [sequences]; starts None: all zero)."""
+        self._mx(lib().mlvc_b200_mx_cache_write, ctypes.byref(cache.c), ctypes.byref(mx._fill(mx.Matrix(), x)),
+                 ctypes.byref(mx.rows_of(pages, offsets, starts)), stream=stream)
+
+    def mx_cache_read(self, cache, y, pages, offsets, starts=None, stream=None):
+        """Reads packed rows back into the dense matrix y, addressed as in
+        mx_cache_write; rows that have no place are zeros."""
+        self._mx(lib().mlvc_b200_mx_cache_read, ctypes.byref(cache.c), ctypes.byref(mx._fill(mx.Matrix(), y)),
+                 ctypes.byref(mx.rows_of(pages, offsets, starts)), stream=stream)
 
     # ----------------------------------------------------------- slots
     def configure_slots(self, n):

@@ -1,0 +1,241 @@
+"""Microscaled matrices, linear layers on them and a paged cache of rows.
+
+Rows are held in blocks that share a scale, value = code * scale * tensor_scale:
+
+    "mxfp4"  codes E2M1, blocks of 32, scales powers of two (E8M0)
+    "nvfp4"  codes E2M1, blocks of 16, scales E4M3, one float per tensor
+    "mxfp8"  codes E4M3, blocks of 32, scales powers of two (E8M0)
+
+The memory is the caller's: dense operands and buffers are objects with
+data_ptr(), and for matrices shape, stride() and dtype (a torch tensor, for
+one), on the backend's device.  Work is enqueued on `stream` (a CUDA stream
+handle; None: the backend's own stream, 0: the legacy default stream) without a
+wait.  The calls are those of include/mlvc_b200.h, whose rules on layouts,
+non-finite values and cache rows without a place hold here too:
+
+    weight = MxMatrix.allocate("nvfp4", outputs, inputs, alloc, tensor_scale)
+    backend.mx_quantise(w, weight, stream=stream)
+    layer = MxLinear(backend, weight, bias=bias, slope=0.01, tensor_scale=gx)
+    layer(x, y, workspace=alloc(layer.workspace_bytes(rows)), stream=stream)
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple
+
+FORMATS = {"mxfp4": 0, "nvfp4": 1, "mxfp8": 2}
+_DTYPES = {"float16": 0, "bfloat16": 2, "float32": 3}
+_dtype_codes = {}  # dtype object -> code
+
+
+class Matrix(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_uint64), ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32),
+                ("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("row_stride", ctypes.c_int64),
+                ("col_stride", ctypes.c_int64)]
+
+
+class MxMatrixC(ctypes.Structure):
+    _fields_ = [("format", ctypes.c_int32), ("tensor_scale", ctypes.c_float), ("rows", ctypes.c_int64),
+                ("cols", ctypes.c_int64), ("data", ctypes.c_uint64), ("scales", ctypes.c_uint64)]
+
+
+class MxCacheC(ctypes.Structure):
+    _fields_ = [("format", ctypes.c_int32), ("tensor_scale", ctypes.c_float), ("pages", ctypes.c_int64),
+                ("page_rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("data", ctypes.c_uint64),
+                ("scales", ctypes.c_uint64)]
+
+
+class MxRows(ctypes.Structure):
+    _fields_ = [("pages", ctypes.c_uint64), ("pages_per_sequence", ctypes.c_int64), ("offsets", ctypes.c_uint64),
+                ("starts", ctypes.c_uint64), ("sequences", ctypes.c_int64)]
+
+
+class LinearArgs(ctypes.Structure):
+    _fields_ = [("x", Matrix), ("a", MxMatrixC), ("w", MxMatrixC), ("y", Matrix), ("residual", Matrix),
+                ("bias", ctypes.c_uint64), ("slope", ctypes.c_float), ("tensor_scale", ctypes.c_float),
+                ("workspace", ctypes.c_uint64), ("workspace_bytes", ctypes.c_size_t)]
+
+
+_P = ctypes.POINTER
+EXPORTS = {
+    "mlvc_b200_mx_layout": ([ctypes.c_int, ctypes.c_int64, ctypes.c_int64] + [_P(ctypes.c_size_t)] * 3, ctypes.c_int),
+    "mlvc_b200_mx_cache_layout": ([ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64] +
+                                  [_P(ctypes.c_size_t)] * 3, ctypes.c_int),
+    "mlvc_b200_mx_quantise": ([ctypes.c_void_p, _P(Matrix), _P(MxMatrixC), ctypes.c_uint64], ctypes.c_int),
+    "mlvc_b200_mx_dequantise": ([ctypes.c_void_p, _P(MxMatrixC), _P(Matrix), ctypes.c_uint64], ctypes.c_int),
+    "mlvc_b200_mx_linear_workspace": ([ctypes.c_int64, _P(MxMatrixC), _P(ctypes.c_size_t)], ctypes.c_int),
+    "mlvc_b200_mx_linear": ([ctypes.c_void_p, _P(LinearArgs), ctypes.c_uint64], ctypes.c_int),
+    "mlvc_b200_mx_cache_write": ([ctypes.c_void_p, _P(MxCacheC), _P(Matrix), _P(MxRows), ctypes.c_uint64],
+                                 ctypes.c_int),
+    "mlvc_b200_mx_cache_read": ([ctypes.c_void_p, _P(MxCacheC), _P(Matrix), _P(MxRows), ctypes.c_uint64],
+                                ctypes.c_int),
+}
+
+
+def _code(dtype):
+    code = _dtype_codes.get(dtype)
+    if code is None:
+        code = _DTYPES.get(str(dtype).rsplit(".", 1)[-1])
+        if code is None:
+            raise RuntimeError(f"mlvc-b200: a dense matrix is float16, bfloat16 or float32, not {dtype}")
+        _dtype_codes[dtype] = code
+    return code
+
+
+def _fill(m, t):
+    """Describes the matrix `t` in the structure `m`."""
+    shape = t.shape
+    if len(shape) != 2:
+        raise RuntimeError(f"mlvc-b200: a dense matrix has two dimensions, not {len(shape)}")
+    m.data = t.data_ptr()
+    m.dtype = _code(t.dtype)
+    m.rows, m.cols = shape
+    m.row_stride, m.col_stride = t.stride()
+    return m
+
+
+def _format(name):
+    if name not in FORMATS:
+        raise RuntimeError(f"mlvc-b200: unknown microscaled format {name!r}")
+    return FORMATS[name]
+
+
+def _ints(t, what, dims):
+    """Address of a contiguous int32 device array (None: 0)."""
+    if t is None:
+        return 0
+    if str(t.dtype).rsplit(".", 1)[-1] != "int32" or len(t.shape) != dims or not t.is_contiguous():
+        raise RuntimeError(f"mlvc-b200: {what} must be a contiguous int32 array of {dims} dimension(s)")
+    return t.data_ptr()
+
+
+def _room(buffer, need, what):
+    have = buffer.nbytes if hasattr(buffer, "nbytes") else need
+    if have < need:
+        raise RuntimeError(f"mlvc-b200: {what} needs {need} bytes and has {have}")
+
+
+class MxLayout(NamedTuple):
+    pitch: int        # bytes of a quantised row
+    data_bytes: int   # of all codes
+    scale_bytes: int  # of all scales
+
+
+def _layout(fn, *args):
+    from . import _check, lib
+    out = [ctypes.c_size_t() for _ in range(3)]
+    _check(getattr(lib(), fn)(*args, *[ctypes.byref(o) for o in out]))
+    return MxLayout(*(o.value for o in out))
+
+
+class MxMatrix:
+    """A quantised matrix [rows, cols] in the caller's buffers `data` and
+    `scales` (objects with data_ptr(), at least layout()'s bytes each)."""
+
+    def __init__(self, format, rows, cols, data, scales, tensor_scale=1.0):
+        lay = self.layout(format, rows, cols)
+        _room(data, lay.data_bytes, "a quantised matrix's data")
+        _room(scales, lay.scale_bytes, "a quantised matrix's scales")
+        self.format, self.rows, self.cols, self.tensor_scale = format, int(rows), int(cols), float(tensor_scale)
+        self.data, self.scales = data, scales
+        self.c = MxMatrixC(_format(format), tensor_scale, rows, cols, data.data_ptr(), scales.data_ptr())
+
+    @staticmethod
+    def layout(format, rows, cols):
+        return _layout("mlvc_b200_mx_layout", _format(format), rows, cols)
+
+    @classmethod
+    def allocate(cls, format, rows, cols, alloc, tensor_scale=1.0):
+        """With buffers from alloc(bytes)."""
+        lay = cls.layout(format, rows, cols)
+        return cls(format, rows, cols, alloc(lay.data_bytes), alloc(lay.scale_bytes), tensor_scale)
+
+
+class MxCache:
+    """A cache of pages * page_rows quantised rows of `cols` values in the
+    caller's buffers: of the features, keys or values of many sequences, whose
+    pages a table names."""
+
+    def __init__(self, format, pages, page_rows, cols, data, scales, tensor_scale=1.0):
+        lay = self.layout(format, pages, page_rows, cols)
+        _room(data, lay.data_bytes, "a cache's data")
+        _room(scales, lay.scale_bytes, "a cache's scales")
+        self.format, self.pages, self.page_rows, self.cols = format, int(pages), int(page_rows), int(cols)
+        self.tensor_scale, self.data, self.scales = float(tensor_scale), data, scales
+        self.c = MxCacheC(_format(format), tensor_scale, pages, page_rows, cols, data.data_ptr(), scales.data_ptr())
+
+    @staticmethod
+    def layout(format, pages, page_rows, cols):
+        return _layout("mlvc_b200_mx_cache_layout", _format(format), pages, page_rows, cols)
+
+    @classmethod
+    def allocate(cls, format, pages, page_rows, cols, alloc, tensor_scale=1.0):
+        """With buffers from alloc(bytes)."""
+        lay = cls.layout(format, pages, page_rows, cols)
+        return cls(format, pages, page_rows, cols, alloc(lay.data_bytes), alloc(lay.scale_bytes), tensor_scale)
+
+
+def rows_of(pages, offsets, starts):
+    """The C description of where packed rows lie (see mlvc_b200_mx_rows)."""
+    r = MxRows()
+    r.pages = _ints(pages, "the page table", 2)
+    r.offsets = _ints(offsets, "offsets", 1)
+    r.starts = _ints(starts, "starts", 1)
+    r.sequences, r.pages_per_sequence = pages.shape
+    if offsets.shape[0] != r.sequences + 1 or (starts is not None and starts.shape[0] != r.sequences):
+        raise RuntimeError("mlvc-b200: offsets has one entry more than there are sequences, starts as many")
+    return r
+
+
+class MxLinear:
+    """y = leaky(x . weight^T + bias) + residual on a quantised weight [outputs,
+    inputs]: the 1x1 convolution of the codec's graphs on low-precision operands.
+
+    bias: float32 [outputs]; slope: factor of negative results (1: none);
+    tensor_scale: of x, when a call quantises it (nvfp4)."""
+
+    def __init__(self, backend, weight, bias=None, slope=1.0, tensor_scale=1.0):
+        from . import _check, lib
+        if bias is not None and (_code(bias.dtype) != 3 or tuple(bias.shape) != (weight.rows,) or
+                                 not bias.is_contiguous()):
+            raise RuntimeError("mlvc-b200: bias must be a contiguous float32 vector, one value for each output")
+        self._keep = (weight, bias)
+        self._check, self._lib = _check, lib()
+        self._call, self._backend = self._lib.mlvc_b200_mx_linear, backend
+        a = self._args = LinearArgs()
+        a.w = weight.c
+        a.bias = bias.data_ptr() if bias is not None else 0
+        a.slope, a.tensor_scale = slope, tensor_scale
+        self._x, self._y, self._residual = a.x, a.y, a.residual  # views
+        self._ref = ctypes.byref(a)
+
+    def workspace_bytes(self, rows):
+        """Bytes of workspace that a call on `rows` dense rows needs."""
+        n = ctypes.c_size_t()
+        self._check(self._lib.mlvc_b200_mx_linear_workspace(rows, ctypes.byref(self._args.w), ctypes.byref(n)))
+        return n.value
+
+    def __call__(self, x, y, residual=None, workspace=None, stream=None):
+        """x: dense [rows, inputs], or an MxMatrix of the weight's format; y and
+        residual: dense [rows, outputs] of one type.  Dense x needs a workspace
+        (256-byte boundary) that nothing else uses until the call's work is done."""
+        a = self._args
+        if isinstance(x, MxMatrix):
+            a.a = x.c
+            self._x.data = 0
+        else:
+            a.a.data = 0
+            _fill(self._x, x)
+        _fill(self._y, y)
+        if residual is None:
+            self._residual.data = 0
+        else:
+            _fill(self._residual, residual)
+        if workspace is None:
+            a.workspace = a.workspace_bytes = 0
+        else:
+            a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.nbytes
+        if self._call(self._backend._h, self._ref, self._backend.stream or 0 if stream is None else stream):
+            self._check(-1)
+        return y

@@ -1,0 +1,180 @@
+"""The microscaled operators without a GPU: the oracle's formats against their
+definitions, layouts, and what the calls refuse."""
+
+import ctypes
+
+import numpy as np
+import pytest
+
+import mlvc_b200
+from mlvc_b200 import Backend, mx
+from oracle import mx_oracle
+
+torch = pytest.importorskip("torch")
+FORMATS = ["mxfp4", "nvfp4", "mxfp8"]
+
+
+@pytest.fixture(scope="module")
+def be():
+    return Backend(plan_only_for=(148, 232448))
+
+
+def dense(m, n, dtype=torch.float16):
+    return torch.zeros(m, n, dtype=dtype)
+
+
+# -------------------------------------------------------------- the oracle
+def test_e4m3_table_matches_torch():
+    codes = torch.arange(127, dtype=torch.uint8)
+    assert np.array_equal(codes.view(torch.float8_e4m3fn).double().numpy(), mx_oracle.E4M3)
+
+
+def test_nearest_codes_tie_to_even():
+    mids = [0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.0, 1e9]
+    assert mx_oracle.nearest_code(np.array(mids), mx_oracle.E2M1).tolist() == [0, 2, 2, 4, 4, 6, 6, 7, 7]
+    v = np.random.default_rng(0).standard_normal(20000) * np.exp2(np.random.default_rng(1).integers(-12, 8, 20000))
+    v = v.astype(np.float32)
+    want = torch.from_numpy(np.clip(v, -448, 448)).to(torch.float8_e4m3fn).view(torch.uint8).numpy() & 0x7F
+    assert np.array_equal(mx_oracle.nearest_code(v, mx_oracle.E4M3), want)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_values_are_as_near_as_the_format_allows(fmt):
+    """No value is further off than half the widest step below the block's
+    maximum, or, where the scale is a power of two, than what saturates."""
+    x = np.random.default_rng(4).standard_normal((50, 128))
+    v = mx_oracle.held(x, fmt, 0.01 if fmt == "nvfp4" else 1.0)
+    a = np.abs(x.reshape(50, -1, mx_oracle.BLOCK[fmt])).max(2, keepdims=True)
+    worst = np.abs(v - x).reshape(50, -1, mx_oracle.BLOCK[fmt]) / a
+    # E2M1's widest step is 2 of 6 (scale off by 1/16 at most); with a power of
+    # two the maximum lies in [4, 8) of 6: up to 2 of 8 saturates.  E4M3: 1.75
+    # of 2 is the largest code, up to 1/8 of the maximum saturates.
+    assert worst.max() <= {"nvfp4": 1 / 6 * 17 / 16 + 1 / 16, "mxfp4": 2 / 8, "mxfp8": 1 / 8}[fmt]
+
+
+# ----------------------------------------------------------------- layouts
+@pytest.mark.parametrize("fmt,rows,cols,want", [
+    ("mxfp4", 1, 1, (16, 16, 512)), ("nvfp4", 130, 200, (112, 130 * 112, 2 * 4 * 512)),
+    ("mxfp8", 128, 4096, (4096, 128 * 4096, 32 * 512)), ("nvfp4", 0, 64, (32, 0, 0)),
+    ("mxfp4", 5_000_000, 1024, (512, 5_000_000 * 512, 39063 * 8 * 512))])
+def test_matrix_layout(fmt, rows, cols, want):
+    assert tuple(mx.MxMatrix.layout(fmt, rows, cols)) == want
+
+
+def test_cache_layout():
+    assert tuple(mx.MxCache.layout("mxfp8", 3, 4, 96)) == (96, 12 * 96, 12 * 3)
+    assert tuple(mx.MxCache.layout("nvfp4", 1 << 20, 256, 1024)) == (512, (1 << 28) * 512, (1 << 28) * 64)
+
+
+def test_tiled_scales_of_the_oracle():
+    s = np.arange(200 * 8, dtype=np.int64).reshape(200, 8) % 251
+    t = mx_oracle.tile_scales(s.astype(np.uint8))
+    assert t.shape == (2, 2, 512)
+    assert t[1, 0, (150 - 128) % 32 * 16 + 0 + 3] == s[150, 3]
+    assert t[0, 1, 5 * 16 + 3 * 4 + 2] == s[101, 6]
+
+
+# ---------------------------------------------------------------- refusals
+@pytest.mark.parametrize("call,match", [
+    (lambda: mx.MxMatrix.layout("fp4", 1, 1), "unknown microscaled format"),
+    (lambda: mx.MxMatrix.layout("mxfp4", 1, 0), "columns"),
+    (lambda: mx.MxMatrix.layout("mxfp4", -1, 4), "rows"),
+    (lambda: mx.MxCache.layout("mxfp4", 0, 4, 4), "at least one page"),
+    (lambda: mx.MxCache.layout("mxfp4", 1 << 30, 1 << 20, 4), "at most 2"),
+    (lambda: mx.MxMatrix("mxfp4", 128, 64, dense(1, 8), dense(1, 600)), "needs 4096 bytes"),
+])
+def test_layout_refusals(call, match):
+    with pytest.raises(RuntimeError, match=match):
+        call()
+
+
+def held(fmt, m, n, g=1.0):
+    return mx.MxMatrix.allocate(fmt, m, n, aligned, g)
+
+
+def aligned(n, boundary=256):
+    t = torch.zeros(n + boundary, dtype=torch.uint8)
+    at = -t.data_ptr() % boundary
+    return t[at:at + n]
+
+
+def test_quantise_refusals(be):
+    for x, out, match in [
+        (dense(4, 64), held("mxfp4", 5, 64), "differ in shape"),
+        (dense(4, 64), held("mxfp4", 4, 64, 2.0), "only nvfp4 has a tensor scale"),
+        (dense(4, 64), held("nvfp4", 4, 64, 0.0), "finite and positive"),
+        (dense(4, 64), held("nvfp4", 4, 64, float("nan")), "finite and positive"),
+        (dense(4, 64), held("nvfp4", 4, 64, 2.0**120), "must lie in"),
+        (dense(4, 64, torch.int32), held("mxfp4", 4, 64), "float16, bfloat16 or float32"),
+        (torch.zeros(4, 64, 1), held("mxfp4", 4, 64), "two dimensions"),
+        (dense(4, 64), mx.MxMatrix("mxfp4", 4, 64, aligned(200)[8:], aligned(512)), "16-byte boundaries"),
+        (dense(4, 64), held("mxfp4", 4, 64), "planning-only"),
+    ]:
+        with pytest.raises(RuntimeError, match=match):
+            be.mx_quantise(x, out)
+
+
+def test_dequantise_refusals(be):
+    for y, match in [(dense(4, 1).expand(4, 64), "must not overlap"), (dense(1, 64).expand(4, 64), "must not overlap"),
+                     (dense(4, 63), "differ in shape"), (dense(4, 64), "planning-only")]:
+        with pytest.raises(RuntimeError, match=match):
+            be.mx_dequantise(held("mxfp8", 4, 64), y)
+
+
+def test_linear_refusals(be):
+    w = held("mxfp4", 8, 64)
+    f32 = torch.float32
+    for kw, match in [
+        (dict(x=dense(4, 65)), "differ in columns"),
+        (dict(y=dense(4, 9)), "one column for each row of the weights"),
+        (dict(y=dense(5, 8)), "one column for each row of the weights"),
+        (dict(y=dense(8, 4).t()), "y's columns must be contiguous"),
+        (dict(y=dense(1, 8).expand(4, 8)), "must not overlap"),
+        (dict(residual=dense(4, 8, f32)), "residual must have y's type and shape"),
+        (dict(residual=dense(4, 7)), "residual must have y's type and shape"),
+        (dict(residual=dense(8, 4).t()), "residual's columns must be contiguous"),
+        (dict(x=held("nvfp4", 4, 64)), "differ in format"),
+        (dict(x=held("mxfp4", 4, 96)), "differ in columns"),
+        (dict(slope=float("inf")), "slope must be finite"),
+        (dict(bias=torch.zeros(9)), "bias must be"),
+        (dict(bias=torch.zeros(8, dtype=torch.float16)), "bias must be"),
+        (dict(workspace=aligned(4096)[1:]), "256-byte boundary"),
+        (dict(workspace=aligned(16)), "workspace must hold"),
+        (dict(workspace=None), "workspace must hold"),
+        (dict(tensor_scale=3.0), "only nvfp4"),
+        (dict(), "planning-only"),
+        (dict(x=held("mxfp4", 4, 64), workspace=None), "planning-only"),
+    ]:
+        a = dict(x=dense(4, 64), y=dense(4, 8), residual=None, workspace=aligned(4096), bias=None, slope=1.0, tensor_scale=1.0)
+        a.update(kw)
+        with pytest.raises(RuntimeError, match=match):
+            mx.MxLinear(be, w, bias=a["bias"], slope=a["slope"], tensor_scale=a["tensor_scale"])(
+                a["x"], a["y"], residual=a["residual"], workspace=a["workspace"])
+
+
+def test_cache_refusals(be):
+    cache = mx.MxCache.allocate("nvfp4", 4, 8, 64, aligned)
+    ints = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    for kw, match in [
+        (dict(x=dense(4, 32)), "differ in columns"),
+        (dict(pages=ints(2, 3).t()), "contiguous int32"),
+        (dict(pages=ints(2)), "contiguous int32"),
+        (dict(pages=torch.zeros(2, 3, dtype=torch.int64)), "contiguous int32"),
+        (dict(offsets=ints(2)), "one entry more"),
+        (dict(starts=ints(3)), "starts as many"),
+        (dict(pages=ints(0, 3), offsets=ints(1)), "at least one sequence"),
+        (dict(), "planning-only"),
+    ]:
+        a = dict(x=dense(4, 64), pages=ints(2, 3), offsets=ints(3), starts=None)
+        a.update(kw)
+        for call in (be.mx_cache_write, be.mx_cache_read):
+            with pytest.raises(RuntimeError, match=match):
+                call(cache, a["x"], a["pages"], a["offsets"], starts=a["starts"])
+
+
+def test_null_arguments_are_errors():
+    lib = mlvc_b200.lib()
+    assert lib.mlvc_b200_mx_quantise(None, None, None, 0) == -1
+    assert b"null argument" in lib.mlvc_b200_last_error()
+    assert lib.mlvc_b200_mx_linear(None, ctypes.byref(mx.LinearArgs()), 0) == -1
+    assert b"null backend handle" in lib.mlvc_b200_last_error()

@@ -1,0 +1,407 @@
+"""Microscaled matrices, products and the paged cache on the B200 against the
+64-bit oracle: codes and scales bit for bit, products within the error of 32-bit
+sums, at the sizes, strides and values where they can go wrong.
+
+nvfp4 tensor scales are powers of two where bits are compared, so that the
+64-bit definition and the kernels' 32-bit quotients agree on every tie.
+"""
+
+import numpy as np
+import pytest
+
+from mlvc_b200 import Backend
+from mlvc_b200.mx import MxCache, MxLinear, MxMatrix
+from oracle import mx_oracle as mx
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+FORMATS = ["mxfp4", "nvfp4", "mxfp8"]
+DTYPES = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
+# half the spacing of a rounded result, relative to it
+ROUNDING = {"f16": 2.0**-11, "bf16": 2.0**-8, "f32": 2.0**-24}
+TINY = {"f16": 2.0**-25, "bf16": 2.0**-134, "f32": 2.0**-150}  # half the smallest subnormal
+
+
+@pytest.fixture(scope="module")
+def be():
+    return Backend(0)
+
+
+def alloc(n):
+    """Room that is never zero by chance."""
+    return torch.full((n,), 0xA5, dtype=torch.uint8, device="cuda")
+
+
+def scale_of(fmt):
+    return 0.125 if fmt == "nvfp4" else 1.0
+
+
+def rows(rng, m, k, dtype, scale=1.0):
+    """Values of many sizes; a few blocks are all zero, a few hold one value on
+    a middle between two codes."""
+    x = rng.standard_normal((m, k)) * np.exp2(rng.integers(-6, 6, (m, k))) * scale
+    x[rng.random((m, k)) < 0.02] = 0
+    x[rng.random(m) < 0.1] = 0
+    hit = rng.random((m, k)) < 0.05
+    x[hit] = rng.choice([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.0], int(hit.sum()))
+    return torch.from_numpy(x.astype(np.float32)).to(DTYPES[dtype])
+
+
+def f64(t):
+    return t.detach().cpu().to(torch.float64).numpy()
+
+
+def quantised(be, x, fmt, g=None):
+    m = MxMatrix.allocate(fmt, x.shape[0], x.shape[1], alloc, scale_of(fmt) if g is None else g)
+    be.mx_quantise(x, m, stream=0)
+    return m
+
+
+def check_held(m, x, fmt):
+    """Codes and scales of an MxMatrix equal the oracle's; the rest of the last
+    scale tile's columns is zero."""
+    codes, scales = mx.quantise(f64(x), fmt, m.tensor_scale)
+    got = m.data.cpu().numpy().reshape(x.shape[0], -1)
+    want = mx.pack(codes, fmt)
+    # the sign of a zero code is kept, whatever the scale: compare bits
+    assert got.shape == want.shape
+    assert np.array_equal(got, want), f"{int((got != want).sum())} of {got.size} code bytes differ"
+    blocks = scales.shape[1]
+    tiled = mx.tile_scales(np.pad(scales, ((0, 0), (0, -blocks % 4))))
+    mask = mx.tile_scales(np.pad(np.full_like(scales, 1), ((0, 0), (0, -blocks % 4)), constant_values=1)) == 1
+    have = m.scales.cpu().numpy().reshape(tiled.shape)
+    assert np.array_equal(have[mask], tiled[mask]), f"{int((have != tiled)[mask].sum())} scales differ"
+
+
+SHAPES = [(1, 1), (1, 16), (2, 31), (3, 33), (5, 200), (1, 4097), (129, 64), (130, 8200), (300, 1000)]
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_quantise_bits(be, fmt, dtype, shape):
+    x = rows(np.random.default_rng(shape[1]), *shape, dtype).cuda()
+    check_held(quantised(be, x, fmt), x, fmt)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_quantise_strides(be, fmt, dtype):
+    """A column range, a transposed matrix, one row repeated, every second
+    column and a base that is no multiple of 32 bytes."""
+    rng = np.random.default_rng(3)
+    wide = rows(rng, 40, 300, dtype).cuda()
+    for x in (wide[:, 64:196], wide[:, 3:103], wide.t(), wide[5:6].expand(9, 300), wide[:, ::2], wide[::3, 16:272],
+              wide.flatten()[1:2561].view(40, 64), wide[:, 7:8].expand(40, 70)):
+        check_held(quantised(be, x, fmt), x, fmt)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_quantise_special_values(be, fmt, dtype):
+    """Zeros of both signs, infinities, NaN, the largest and the smallest values
+    of the type, each in a block of its own."""
+    info = torch.finfo(DTYPES[dtype])
+    x = torch.ones(10, 96, dtype=torch.float32)
+    x[0] = 0
+    x[1] = -0.0
+    x[2, 40] = float("inf")
+    x[3, 40] = float("-inf")
+    x[4, 0], x[4, 95] = float("nan"), -float("nan")
+    x[5, :64] = info.max
+    x[5, 3] = info.min
+    x[6] = info.smallest_normal
+    x[7] = 0
+    x[7, 33] = 2.0**-24 if dtype == "f16" else 2.0**-133 if dtype == "bf16" else 2.0**-149
+    x[8] = torch.linspace(-6, 6, 96)
+    x[9, 1::2] = 2.0**-20
+    x = x.to(DTYPES[dtype]).cuda()
+    for g in ([scale_of(fmt)] if fmt != "nvfp4" else [1.0, 2.0**-30, 2.0**40]):
+        m = quantised(be, x, fmt, g)
+        check_held(m, x, fmt)
+        y = torch.empty(10, 96, device="cuda")
+        be.mx_dequantise(m, y, stream=0)
+        want = mx.held(f64(x), fmt, g).astype(np.float32)
+        assert np.array_equal(f64(y), want.astype(np.float64), equal_nan=True)
+        # a non-finite value takes its own block with it and no other
+        bad = np.isnan(f64(y))
+        assert bad[2].sum() == bad[3].sum() == mx.BLOCK[fmt] and bad[4].sum() == 2 * mx.BLOCK[fmt]
+        assert not bad[[0, 1, 5, 6, 7, 8, 9]].any()
+
+
+@pytest.mark.parametrize("out", list(DTYPES))
+@pytest.mark.parametrize("shape", [(1, 1), (3, 33), (130, 200), (17, 4100)])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_dequantise(be, fmt, shape, out):
+    """Values are exact in 32 bits (power-of-two tensor scale) and rounded once."""
+    x = rows(np.random.default_rng(shape[0]), *shape, "f32", 8.0).cuda()
+    m = quantised(be, x, fmt)
+    y = torch.empty(shape, dtype=DTYPES[out], device="cuda")
+    be.mx_dequantise(m, y, stream=0)
+    want = torch.from_numpy(mx.held(f64(x), fmt, m.tensor_scale).astype(np.float32)).to(DTYPES[out])
+    assert torch.equal(y.cpu(), want)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_dequantise_strides(be, fmt):
+    """Column ranges, transposed and spread-out outputs; nothing beside them is written."""
+    x = rows(np.random.default_rng(1), 37, 100, "bf16").cuda()
+    m = quantised(be, x, fmt)
+    want = torch.from_numpy(mx.held(f64(x), fmt, m.tensor_scale).astype(np.float32)).bfloat16()
+    for view in (lambda b: b[:37, 5:105], lambda b: b[:37, 32:132], lambda b: b.view(400, 200)[:100, :37].t(),
+                 lambda b: b[:37, :200:2], lambda b: b.flatten()[3:3703].view(37, 100)):
+        base = torch.full((200, 400), 7.0, dtype=torch.bfloat16, device="cuda")
+        y = view(base)
+        be.mx_dequantise(m, y, stream=0)
+        assert torch.equal(y.cpu(), want)
+        y.fill_(7.0)
+        assert bool((base == 7.0).all())
+
+
+def check_linear(got, x, w, fmt, gx, gw, out, bias=None, slope=1.0, residual=None):
+    """Within the error of 32-bit sums of exact products and one rounding.  A
+    step adds at most 64 products to a running sum; the products of a step and
+    the sum are aligned and may be truncated at 2^-23 of the largest, so each of
+    the k / 32 + 2 additions loses less than 2^-22 of the sum of magnitudes."""
+    n64 = lambda t: None if t is None else f64(t)  # noqa: E731
+    want, size = mx.linear(n64(x), n64(w), fmt, gx, gw, n64(bias), slope, n64(residual))
+    bound = np.abs(want) * ROUNDING[out] + TINY[out] + size * (x.shape[1] / 32 + 4) * 2.0**-22
+    bound *= 1 + 2.0**-10
+    err = np.abs(f64(got) - want)
+    assert np.isfinite(f64(got)).all()
+    worst = np.unravel_index(np.argmax(err - bound), err.shape)
+    assert (err <= bound).all(), f"{int((err > bound).sum())} of {err.size} off, worst at {worst}: {f64(got)[worst]} for {want[worst]}"
+
+
+PRODUCTS = [  # rows, inputs, outputs
+    (1, 1, 1), (1, 32, 8), (1, 4096, 130), (2, 65, 17), (8, 256, 64), (16, 512, 300), (17, 1000, 129), (33, 96, 128),
+    (64, 2048, 257), (65, 300, 40), (127, 128, 63), (128, 256, 128), (129, 257, 129), (200, 640, 1000), (300, 4100, 200),
+    (513, 192, 513), (1000, 1024, 1100),
+]
+
+
+@pytest.mark.parametrize("shape", PRODUCTS)
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_linear(be, fmt, shape):
+    """Dense x; types, bias, slope and residual change with the shape."""
+    m, k, n = shape
+    rng = np.random.default_rng(m * 31 + n)
+    names = list(DTYPES)
+    dtype, out = names[(m + k) % 3], names[(m + n) % 3]
+    x = rows(rng, m, k, dtype, 0.1).cuda()
+    w = rows(rng, n, k, "f32", 0.1).cuda()
+    bias = torch.from_numpy(rng.standard_normal(n).astype(np.float32)).cuda() if n % 2 else None
+    residual = rows(rng, m, n, out).cuda() if m % 2 else None
+    slope = 0.01 if k % 2 == 0 else 1.0
+    gx, gw = scale_of(fmt), scale_of(fmt) / 4 if fmt == "nvfp4" else 1.0
+    layer = MxLinear(be, quantised(be, w, fmt, gw), bias=bias, slope=slope, tensor_scale=gx)
+    y = torch.full((m, n), float("nan"), dtype=DTYPES[out], device="cuda")
+    layer(x, y, residual=residual, workspace=alloc(layer.workspace_bytes(m)), stream=0)
+    check_linear(y, x, w, fmt, gx, gw, out, bias, slope, residual)
+    # x quantised beforehand: the same sums
+    z = torch.full((m, n), float("nan"), dtype=DTYPES[out], device="cuda")
+    layer(quantised(be, x, fmt, gx), z, residual=residual, stream=0)
+    assert torch.equal(y, z)
+
+
+@pytest.mark.parametrize("rows_", [1, 5, 20, 64, 150, 700])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_linear_strides(be, fmt, rows_):
+    """x, y and residual as parts of wider matrices, on and off wide boundaries;
+    nothing beside y is written; y is its own residual."""
+    rng = np.random.default_rng(rows_)
+    k, n = 160, 96
+    w = rows(rng, n, k, "f32", 0.1).cuda()
+    g = scale_of(fmt)
+    layer = MxLinear(be, quantised(be, w, fmt), tensor_scale=g)
+    work = alloc(layer.workspace_bytes(rows_))
+    xs = rows(rng, rows_, 400, "f16", 0.1).cuda()
+    for at, y_at in ((0, 0), (64, 32), (5, 3), (16, 8), (1, 1)):
+        x = xs[:, at:at + k]
+        base = torch.full((rows_ + 1, 2 * n + 1 if y_at == 3 else 2 * n), 3.0, dtype=torch.float16, device="cuda")
+        y = base[:rows_, y_at:y_at + n]
+        layer(x, y, workspace=work, stream=0)
+        check_linear(y, x, w, fmt, g, g, "f16")
+        before = y.clone()
+        layer(x, y, residual=y, workspace=work, stream=0)
+        check_linear(y, x, w, fmt, g, g, "f16", residual=before)
+        y.fill_(3.0)
+        assert bool((base == 3.0).all())
+
+
+@pytest.mark.parametrize("m", [1, 30, 200])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_linear_non_finite(be, fmt, m):
+    """An infinity or a NaN in x makes its row NaN, one in w its column, no other."""
+    rng = np.random.default_rng(9)
+    k, n = 300, 150
+    x, w = rows(rng, m, k, "bf16", 0.1), rows(rng, n, k, "f32", 0.1)
+    x[m // 2, 77], w[101, 299], w[3, 0] = float("inf"), float("nan"), float("-inf")
+    g = scale_of(fmt)
+    layer = MxLinear(be, quantised(be, w.cuda(), fmt), tensor_scale=g)
+    y = torch.zeros(m, n, device="cuda")
+    layer(x.cuda(), y, workspace=alloc(layer.workspace_bytes(m)), stream=0)
+    bad = np.isnan(f64(y))
+    want = np.zeros((m, n), bool)
+    want[m // 2], want[:, [3, 101]] = True, True
+    assert np.array_equal(bad, want)
+
+
+def test_linear_no_rows(be):
+    layer = MxLinear(be, quantised(be, torch.ones(8, 64, device="cuda"), "mxfp4"))
+    layer(torch.ones(0, 64, device="cuda"), torch.ones(0, 8, device="cuda"), stream=0)
+    be.mx_quantise(torch.ones(0, 64, device="cuda"), MxMatrix.allocate("mxfp4", 0, 64, alloc), stream=0)
+    torch.cuda.synchronize()
+
+
+def cache_case(seed, streams, page_rows, longest):
+    rng = np.random.default_rng(seed)
+    old = rng.integers(0, longest + 1, streams)
+    add = rng.integers(0, max(2, longest // 2), streams)
+    add[rng.random(streams) < 0.3] = 0  # streams that bring nothing
+    width = int((old + add).max() // page_rows + 2)
+    pages = rng.permutation(streams * width + 2)[: streams * width].reshape(streams, width).astype(np.int32)
+    return rng, old.astype(np.int32), add.astype(np.int32), pages, streams * width + 2
+
+
+def ends(v):
+    return np.concatenate([[0], np.cumsum(v)]).astype(np.int32)
+
+
+def ints(a):
+    return torch.from_numpy(np.ascontiguousarray(a, np.int32)).cuda()
+
+
+@pytest.mark.parametrize("streams,page_rows,longest,cols", [
+    (1, 1, 1, 1), (1, 16, 40, 64), (3, 4, 9, 96), (33, 5, 12, 40), (70, 16, 30, 1024), (1100, 3, 4, 33), (4, 256, 700, 520),
+    (2, 7, 20, 8200)])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_cache(be, fmt, streams, page_rows, longest, cols):
+    """Histories written, rows appended, everything read back: equal to the rows
+    quantised one by one; rows that were not written keep their bytes."""
+    rng, old, add, pages, count = cache_case(streams + cols, streams, page_rows, longest)
+    g = scale_of(fmt)
+    cache = MxCache.allocate(fmt, count, page_rows, cols, alloc, g)
+    history = rows(rng, int(old.sum()), cols, "bf16").cuda()
+    new = rows(rng, int(add.sum()), cols, "bf16").cuda()
+    table = ints(pages)
+    be.mx_cache_write(cache, history, table, ints(ends(old)), stream=0)
+    be.mx_cache_write(cache, new, table, ints(ends(add)), starts=ints(old), stream=0)
+    total = int((old + add).sum())
+    y = torch.full((total, cols), 5.0, device="cuda")
+    be.mx_cache_read(cache, y, table, ints(ends(old + add)), stream=0)
+    parts = []
+    for s in range(streams):
+        parts += [f64(history)[ends(old)[s]:ends(old)[s + 1]], f64(new)[ends(add)[s]:ends(add)[s + 1]]]
+    x = np.concatenate(parts)
+    assert np.array_equal(f64(y), mx.held(x, fmt, g))
+    # the bytes, row by row; the others are untouched
+    slots = mx.cache_slots(pages, page_rows, ends(old + add), None, total)
+    codes, scales = mx.quantise(x, fmt, g)
+    data, held = cache.data.cpu().numpy().reshape(count * page_rows, -1), cache.scales.cpu().numpy().reshape(count * page_rows, -1)
+    assert np.array_equal(data[slots], mx.pack(codes, fmt)) and np.array_equal(held[slots], scales)
+    rest = np.setdiff1d(np.arange(count * page_rows), slots)
+    assert (data[rest] == 0xA5).all() and (held[rest] == 0xA5).all()
+    be.synchronize()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_cache_parts(be, fmt):
+    """Reading from a position on, as f16 into part of a wider matrix, from
+    strided rows; rows without a place read as zeros and are not written."""
+    g, page_rows, cols = scale_of(fmt), 8, 64
+    rng = np.random.default_rng(5)
+    pages = np.array([[4, 1, -1], [0, -1, 3], [2, 5, 6]], np.int32)
+    cache = MxCache.allocate(fmt, 7, page_rows, cols, alloc, g)
+    x = rows(rng, 66, 200, "f16").cuda()[:, 17:17 + cols]
+    offsets = np.array([0, 20, 44, 64], np.int32)  # rows 64 and 65 belong to none
+    be.mx_cache_write(cache, x, ints(pages), ints(offsets), stream=0)
+    slots = mx.cache_slots(pages, page_rows, offsets, None, 66)
+    assert (slots < 0).sum() == 4 + 8 + 2  # two unmapped pages (one partly used), two rows of none
+    want = mx.held(f64(x), fmt, g)
+    want[slots < 0] = 0
+    base = torch.full((66, 100), 9.0, dtype=torch.float16, device="cuda")
+    y = base[:, 9:9 + cols]
+    be.mx_cache_read(cache, y, ints(pages), ints(offsets), stream=0)
+    assert np.array_equal(f64(y), want.astype(np.float16).astype(np.float64))
+    y.fill_(9.0)
+    assert bool((base == 9.0).all())
+    # from positions 5, 0 and 19 on
+    starts, counts = np.array([5, 0, 19], np.int32), np.array([6, 0, 1], np.int32)
+    z = torch.empty(7, cols, device="cuda")
+    be.mx_cache_read(cache, z, ints(pages), ints(ends(counts)), starts=ints(starts), stream=0)
+    assert np.array_equal(f64(z), np.concatenate([want[5:11], want[63:64]]))
+    be.synchronize()
+
+
+@pytest.mark.parametrize("bad", ["page", "position", "negative"])
+def test_cache_reports_rows_without_a_place(be, bad):
+    """A page outside the cache and a position outside the table touch nothing
+    and are reported once."""
+    pages = np.array([[1, 2], [0, 7 if bad == "page" else 3]], np.int32)
+    cache = MxCache.allocate("mxfp8", 4, 4, 32, alloc)
+    x = torch.ones(16, 32, device="cuda")
+    starts = {"page": [0, 0], "position": [0, 1], "negative": [-1, 0]}[bad]
+    counts = ints(ends([8, 8]))
+    be.mx_cache_write(cache, x, ints(pages), counts, starts=ints(starts), stream=0)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="cache row outside the page table"):
+        be.synchronize()
+    y = torch.full((16, 32), 5.0, device="cuda")
+    be.mx_cache_read(cache, y, ints(pages), counts, starts=ints(starts), stream=0)
+    torch.cuda.synchronize()
+    slots = {"page": list(range(12)), "position": list(range(15)), "negative": list(range(1, 16))}[bad]
+    want = torch.zeros(16, 32, device="cuda")
+    want[slots] = 1
+    assert torch.equal(y, want)
+    with pytest.raises(RuntimeError, match="cache row outside the page table"):
+        be.synchronize()
+    be.synchronize()
+
+
+def test_cache_past_32_bits(be):
+    """Rows beyond 4 GiB of codes and beyond 2^32 / 32 scales."""
+    cols, page_rows, count = 2048, 512, 4352  # 4.25 GiB of codes
+    data = torch.empty(count * page_rows * cols, dtype=torch.uint8, device="cuda")
+    scales = torch.empty(count * page_rows * cols // 32, dtype=torch.uint8, device="cuda")
+    cache = MxCache("mxfp8", count, page_rows, cols, data, scales)
+    pages = ints([[count - 1, 0], [count - 2, 2200]])
+    x = rows(np.random.default_rng(0), 1400, cols, "bf16").cuda()
+    offsets = ints([0, 700, 1400])
+    be.mx_cache_write(cache, x, pages, offsets, stream=0)
+    y = torch.empty(1400, cols, device="cuda")
+    be.mx_cache_read(cache, y, pages, offsets, stream=0)
+    assert np.array_equal(f64(y), mx.held(f64(x), "mxfp8"))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_other_streams(be, fmt):
+    """The backend's own stream and a second one: each call's work is on the
+    stream it was given."""
+    rng = np.random.default_rng(2)
+    x, w = rows(rng, 40, 512, "bf16", 0.1).cuda(), rows(rng, 256, 512, "f32", 0.1).cuda()
+    g = scale_of(fmt)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    weight = MxMatrix.allocate(fmt, 256, 512, alloc, g)
+    torch.cuda.synchronize()
+    be.mx_quantise(w, weight)  # the backend's stream
+    be.synchronize()
+    layer = MxLinear(be, weight, tensor_scale=g)
+    y = torch.zeros(40, 256, device="cuda")
+    work = alloc(layer.workspace_bytes(40))
+    torch.cuda.synchronize()
+    layer(x, y, workspace=work, stream=side.cuda_stream)
+    side.synchronize()
+    check_linear(y, x, w, fmt, g, g, "f32")
+
+
+def test_refusals_leave_the_backend_usable(be):
+    x = torch.ones(4, 64, device="cuda")
+    m = MxMatrix.allocate("mxfp4", 5, 64, alloc)
+    with pytest.raises(RuntimeError, match="differ in shape"):
+        be.mx_quantise(x, m, stream=0)
+    with pytest.raises(RuntimeError, match="workspace must hold"):
+        MxLinear(be, m)(x, torch.ones(4, 5, device="cuda"), stream=0)
+    check_held(quantised(be, x, "mxfp4"), x, "mxfp4")
