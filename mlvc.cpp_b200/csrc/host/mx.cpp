@@ -85,7 +85,7 @@ int wide(const MxDense& d)
 }
 
 // Order of functions_: the four conversions by type and format, then products.
-enum { kQuantise = 0, kDequantise = 9, kCacheWrite = 18, kCacheRead = 27, kGemm64 = 36, kGemm128 = 39, kFunctions = 42 };
+enum { kQuantise = 0, kDequantise = 9, kCacheWrite = 18, kCacheRead = 27, kGemm64 = 36, kGemm128 = 39, kRows = 42, kFunctions = 54 };
 
 int convert_index(int base, int dtype, int format) { return base + (dtype == kMxF16 ? 0 : dtype == kMxBf16 ? 3 : 6) + format; }
 
@@ -95,6 +95,9 @@ std::string function_name(int i)
     static const int types[3] = {kMxF16, kMxBf16, kMxF32};
     if (i < kGemm64)
         return std::string("mlvc_mx_") + conversions[i / 9] + "_" + kTypeNames[types[i % 9 / 3]] + "_" + kFormatNames[i % 3];
+    if (i >= kRows)
+        return std::string("mlvc_mx_rows_") + (i < kRows + 3 ? "quantised" : kTypeNames[types[(i - kRows) / 3 - 1]]) + "_" +
+               kFormatNames[i % 3];
     return std::string(i < kGemm128 ? "mlvc_mx_gemm64_" : "mlvc_mx_gemm128_") + kFormatNames[i % 3];
 }
 
@@ -179,6 +182,31 @@ unsigned int Mx::take_status()
     return status;
 }
 
+// Kernels start while the one before drains (programmatic dependent launch);
+// they wait for it before they touch memory.
+void Mx::launch(int index, unsigned grid_x, unsigned grid_y, unsigned block, unsigned smem, unsigned cluster, void* params,
+                CUstream stream)
+{
+    CUlaunchAttribute attrs[2]{};
+    attrs[0].id = CU_LAUNCH_ATTRIBUTE_PROGRAMMATIC_STREAM_SERIALIZATION;
+    attrs[0].value.programmaticStreamSerializationAllowed = 1;
+    attrs[1].id = CU_LAUNCH_ATTRIBUTE_CLUSTER_DIMENSION;
+    attrs[1].value.clusterDim.x = cluster;
+    attrs[1].value.clusterDim.y = attrs[1].value.clusterDim.z = 1;
+    CUlaunchConfig cfg{};
+    cfg.gridDimX = grid_x;
+    cfg.gridDimY = grid_y;
+    cfg.gridDimZ = 1;
+    cfg.blockDimX = block;
+    cfg.blockDimY = cfg.blockDimZ = 1;
+    cfg.sharedMemBytes = smem;
+    cfg.hStream = stream;
+    cfg.attrs = attrs;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    void* args[] = {params};
+    check(cuLaunchKernelEx(&cfg, fn(index), args, nullptr), "cuLaunchKernelEx(mx)");
+}
+
 // A CTA of 256 threads takes up to 1024 chunks: up to 256 of a row, as many
 // rows as that leaves.  Small calls get fewer rows a CTA, down to one chunk a
 // thread, so that they reach more SMs.
@@ -210,7 +238,7 @@ void Mx::convert(const MxDense& d, int format, float tensor_scale, uint64_t data
     p.k_tiles = static_cast<int>(k_tiles_of(format, d.cols));
     p.scale_pitch = format == kNvFp4 ? p.chunks : p.chunks / 2;
     p.tensor_scale = tensor_scale;
-    p.six_tensor_scale = 6.0f * tensor_scale;
+    p.inv_six_scale = 1.0f / (6.0f * tensor_scale);
     if (cache) {
         p.pages = reinterpret_cast<const int*>(rows->pages);
         p.offsets = reinterpret_cast<const int*>(rows->offsets);
@@ -225,10 +253,7 @@ void Mx::convert(const MxDense& d, int format, float tensor_scale, uint64_t data
     const int64_t grid = ceil_div(d.rows, p.cta_rows);
     if (grid > 0x7FFFFFFF)
         refuse("too many rows for one call");
-    void* args[] = {&p};
-    check(cuLaunchKernel(fn(index), static_cast<unsigned>(grid), static_cast<unsigned>(columns), 1, 256, 1, 1, 0, stream, args,
-                         nullptr),
-          "cuLaunchKernel(mx convert)");
+    launch(index, static_cast<unsigned>(grid), static_cast<unsigned>(columns), 256, 0, 1, &p, stream);
 }
 
 void Mx::quantise(const MxDense& x, const MxMatrix& out, CUstream stream)
@@ -338,13 +363,17 @@ void Mx::linear(const MxLinear& l, CUstream stream)
     if (rows == 0)
         return;
     if (!dense) {
-        product(l, l.a, stream);
+        if (!few_rows(l, &l.a, stream))
+            product(l, l.a, stream);
         return;
     }
+    if (few_rows(l, nullptr, stream))
+        return;
     const MxLayout lay = mx_layout(w.format, rows, cols);
     const MxMatrix a{w.format, l.tensor_scale, rows, cols, l.workspace, l.workspace + (lay.data_bytes + 255) / 256 * 256};
     quantise(l.x, a, stream);
-    product(l, a, stream);
+    if (!few_rows(l, &a, stream))
+        product(l, a, stream);
 }
 
 namespace {
@@ -360,34 +389,105 @@ void encode_rows(CUtensorMap* map, uint64_t data, size_t pitch, int64_t rows, in
 }
 }  // namespace
 
-void Mx::product(const MxLinear& l, const MxMatrix& a, CUstream stream)
+namespace {
+MxPanels panels_of(int format, int64_t cols)
 {
-    ContextGuard guard(ctx_);
-    const MxMatrix& w = l.w;
-    const int panel = w.format == kMxFp8 ? 128 : 256, step = panel / 4, words = panel / block_of(w.format) / 4;
-    MxGemmParams p{};
-    const size_t pitch = pitch_of(w.format, w.cols);
-    p.scales_a = reinterpret_cast<const uint8_t*>(a.scales);
-    p.scales_b = reinterpret_cast<const uint8_t*>(w.scales);
-    p.k_tiles = static_cast<int>(k_tiles_of(w.format, w.cols));
-    p.k_stages = static_cast<int>(ceil_div(w.cols, panel));
-    p.last_steps = static_cast<int>(ceil_div(w.cols - static_cast<int64_t>(p.k_stages - 1) * panel, step));
-    p.last_words = p.k_tiles - (p.k_stages - 1) * words;
-    p.M = static_cast<int>(a.rows);
-    p.N = static_cast<int>(w.rows);
-    p.bias = reinterpret_cast<const float*>(l.bias);
-    p.residual = reinterpret_cast<const void*>(l.residual.data);
-    p.residual_stride = l.residual.row_stride;
-    p.y = reinterpret_cast<void*>(l.y.data);
-    p.y_stride = l.y.row_stride;
-    p.y_dtype = l.y.dtype;
+    const int panel = format == kMxFp8 ? 128 : 256, words = panel / block_of(format) / 4;
+    MxPanels k{};
+    k.k_tiles = static_cast<int>(k_tiles_of(format, cols));
+    k.count = static_cast<int>(ceil_div(cols, panel));
+    k.last_steps = static_cast<int>(ceil_div(cols - static_cast<int64_t>(k.count - 1) * panel, panel / 4));
+    k.last_words = k.k_tiles - (k.count - 1) * words;
+    return k;
+}
+
+MxEpilogue epilogue_of(const MxLinear& l, int64_t rows, float x_scale)
+{
+    MxEpilogue e{};
+    e.M = static_cast<int>(rows);
+    e.N = static_cast<int>(l.w.rows);
+    e.bias = reinterpret_cast<const float*>(l.bias);
+    e.residual = reinterpret_cast<const void*>(l.residual.data);
+    e.residual_stride = l.residual.row_stride;
+    e.y = reinterpret_cast<void*>(l.y.data);
+    e.y_stride = l.y.row_stride;
+    e.y_dtype = l.y.dtype;
     const size_t size = elem_size(l.y.dtype);
     auto aligned = [&](const MxDense& d) {
         return d.data % 16 == 0 && (d.rows <= 1 || static_cast<size_t>(d.row_stride) * size % 16 == 0);
     };
-    p.vec = aligned(l.y) && (!l.residual.data || aligned(l.residual));
-    p.alpha = a.tensor_scale * w.tensor_scale;
-    p.slope = l.slope;
+    e.vec = aligned(l.y) && (!l.residual.data || aligned(l.residual));
+    e.alpha = x_scale * l.w.tensor_scale;
+    e.slope = l.slope;
+    return e;
+}
+}  // namespace
+
+bool Mx::few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream)
+{
+    const MxMatrix& w = l.w;
+    const int64_t rows = a ? a->rows : l.x.rows;
+    if (rows > kMxRowsMax)
+        return false;
+    MxRowsParams p{};
+    p.k = panels_of(w.format, w.cols);
+    const int64_t n_tiles = ceil_div(w.rows, 128);
+    // as many CTAs on k as keep all SMs at work, a power of two so that
+    // clusters fill the groups of SMs
+    p.splits = 1;
+    while (p.splits < 8 && n_tiles * p.splits * 2 <= sm_count_ && p.splits * 2 <= p.k.count)
+        p.splits *= 2;
+    const int64_t grid = n_tiles * p.splits;
+    p.row_tile = static_cast<int>(ceil_div(rows, 8) * 8);
+    const size_t x_bytes = static_cast<size_t>(p.row_tile) * 128, most = ceil_div(p.k.count, p.splits);
+    const size_t scale_bytes = static_cast<size_t>(w.format == kNvFp4 ? 4 : w.format == kMxFp4 ? 2 : 1) * 512;
+    const size_t stage = ceil_div(128 * 128 + scale_bytes + (a ? x_bytes + scale_bytes : 0), 1024) * 1024;
+    const size_t fixed = 2048 + (a ? 0 : most * x_bytes + ceil_div(most * scale_bytes, 1024) * 1024);
+    // two CTAs an SM where there are more than SMs, if that leaves a ring of four
+    const size_t whole = kGemmSmem, half = 113 * 1024;
+    const size_t room = grid > sm_count_ && fixed + 4 * stage <= half ? half : whole;
+    if (fixed + std::min<size_t>(most, 3) * stage > room)
+        return false;
+    p.stages = static_cast<int>(std::min({most, (room - fixed) / stage, size_t{12}}));
+    size_t smem = fixed + p.stages * stage;
+    if (p.splits > 1)
+        smem = std::max(smem, fixed + static_cast<size_t>(p.row_tile) * 512);
+    if (smem > whole)
+        return false;
+    ContextGuard guard(ctx_);
+    const size_t pitch = pitch_of(w.format, w.cols);
+    encode_rows(&p.map_w, w.data, pitch, w.rows, 128);
+    p.scales_w = reinterpret_cast<const uint8_t*>(w.scales);
+    const float x_scale = a ? a->tensor_scale : l.tensor_scale;
+    if (a) {
+        encode_rows(&p.map_x, a->data, pitch, a->rows, p.row_tile);
+        p.scales_x = reinterpret_cast<const uint8_t*>(a->scales);
+    } else {
+        p.x = reinterpret_cast<const void*>(l.x.data);
+        p.row_stride = l.x.row_stride;
+        p.col_stride = l.x.col_stride;
+        p.cols = static_cast<int>(l.x.cols);
+        p.vec = wide(l.x);
+        p.tensor_scale = x_scale;
+        p.inv_six_scale = 1.0f / (6.0f * x_scale);
+    }
+    p.e = epilogue_of(l, rows, x_scale);
+    const int type = a ? 0 : l.x.dtype == kMxF16 ? 1 : l.x.dtype == kMxBf16 ? 2 : 3;
+    launch(kRows + 3 * type + w.format, static_cast<unsigned>(grid), 1, 320, static_cast<unsigned>(smem),
+           static_cast<unsigned>(p.splits), &p, stream);
+    return true;
+}
+
+void Mx::product(const MxLinear& l, const MxMatrix& a, CUstream stream)
+{
+    ContextGuard guard(ctx_);
+    const MxMatrix& w = l.w;
+    MxGemmParams p{};
+    const size_t pitch = pitch_of(w.format, w.cols);
+    p.scales_a = reinterpret_cast<const uint8_t*>(a.scales);
+    p.scales_b = reinterpret_cast<const uint8_t*>(w.scales);
+    p.k = panels_of(w.format, w.cols);
+    p.e = epilogue_of(l, a.rows, a.tensor_scale);
     p.m_tiles = static_cast<int>(ceil_div(a.rows, 128));
     const bool narrow = p.m_tiles * ceil_div(w.rows, 128) < sm_count_;
     const int bn = narrow ? 64 : 128;
@@ -396,10 +496,8 @@ void Mx::product(const MxLinear& l, const MxMatrix& a, CUstream stream)
         refuse("too many output tiles for one call");
     encode_rows(&p.map_a, a.data, pitch, a.rows, 128);
     encode_rows(&p.map_b, w.data, pitch, w.rows, bn);
-    void* args[] = {&p};
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>(sm_count_, static_cast<int64_t>(p.m_tiles) * p.n_tiles));
-    check(cuLaunchKernel(fn((narrow ? kGemm64 : kGemm128) + w.format), grid, 1, 1, 320, 1, 1, kGemmSmem, stream, args, nullptr),
-          "cuLaunchKernel(mx product)");
+    launch((narrow ? kGemm64 : kGemm128) + w.format, grid, 1, 320, kGemmSmem, 1, &p, stream);
 }
 
 }  // namespace mlvc_b200

@@ -80,7 +80,12 @@ private:
     CUfunction fn(int index);
     void convert(const MxDense& d, int format, float tensor_scale, uint64_t data, uint64_t scales, const MxCache* cache,
                  const MxRows* rows, bool read, CUstream stream);
+    // y from rows quantised in `a`, or (a null) from dense rows quantised by the
+    // product's kernel itself; false: there is no such kernel for these sizes.
+    bool few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream);
     void product(const MxLinear& l, const MxMatrix& a, CUstream stream);
+    void launch(int index, unsigned grid_x, unsigned grid_y, unsigned block, unsigned smem, unsigned cluster, void* params,
+                CUstream stream);
     void require_device() const;
 
     CUcontext ctx_ = nullptr;

@@ -73,34 +73,77 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8])
                  : "memory");
 }
 
-// 16 values of a dense row from column `col`; columns from `cols` on read as 0.
+// A chunk of a dense row as it lies in memory: 16 values.
 template <int DT>
-__device__ __forceinline__ void load_chunk(const void* dense, long long row_at, long long col_stride, int col, int cols,
-                                           int vec, float (&v)[16])
+struct Raw {
+    static constexpr int kWords = DT == kMxF32 ? 16 : 8;
+    uint32_t w[kWords];
+};
+
+// The chunk from column `col`; columns from `cols` on read as 0.  `vec`: the
+// row is contiguous and begins on a 32-byte boundary.
+template <int DT>
+__device__ __forceinline__ void load_raw(const void* dense, long long row_at, long long col_stride, int col, int cols,
+                                         int vec, Raw<DT>& x)
 {
-    using D = Dense<DT>;
-    const typename D::T* p = static_cast<const typename D::T*>(dense) + row_at;
+    using T = typename Dense<DT>::T;
+    const T* p = static_cast<const T*>(dense) + row_at;
     if (vec && col + 16 <= cols) {
-        uint32_t w[8];
-        load32(p + col, w);
-        if constexpr (DT == kMxF32) {
-            uint32_t u[8];
-            load32(p + col + 8, u);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                v[i] = __uint_as_float(w[i]);
-                v[8 + i] = __uint_as_float(u[i]);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                D::unpack(w[i], v[2 * i], v[2 * i + 1]);
-        }
+        for (int i = 0; i < Raw<DT>::kWords; i += 8)
+            load32(reinterpret_cast<const uint32_t*>(p + col) + i, reinterpret_cast<uint32_t(&)[8]>(x.w[i]));
         return;
     }
+    if constexpr (DT == kMxF32) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-        v[i] = col + i < cols ? D::load(p + (col + i) * col_stride) : 0.0f;
+        for (int i = 0; i < 16; ++i)
+            x.w[i] = col + i < cols ? reinterpret_cast<const uint32_t*>(p)[(col + i) * col_stride] : 0u;
+    } else {
+        const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t lo = col + 2 * i < cols ? u[(col + 2 * i) * col_stride] : 0u;
+            const uint32_t hi = col + 2 * i + 1 < cols ? u[(col + 2 * i + 1) * col_stride] : 0u;
+            x.w[i] = lo | (hi << 16);
+        }
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ void unpack_raw(const Raw<DT>& x, float (&v)[16])
+{
+    if constexpr (DT == kMxF32) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            v[i] = __uint_as_float(x.w[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            Dense<DT>::unpack(x.w[i], v[2 * i], v[2 * i + 1]);
+    }
+}
+
+// Bits of the float that is the chunk's largest magnitude.  Magnitudes order
+// like their bits, infinity above the finite and NaN above infinity, so 16-bit
+// values are compared two at a time as they lie.
+template <int DT>
+__device__ __forceinline__ uint32_t largest_raw(const Raw<DT>& x)
+{
+    uint32_t m = 0;
+    if constexpr (DT == kMxF32) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            m = max(m, x.w[i] & 0x7FFFFFFFu);
+        return m;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            m = __vmaxu2(m, x.w[i] & 0x7FFF7FFFu);
+        m = max(m & 0xFFFFu, m >> 16);
+        float a, b;
+        Dense<DT>::unpack(m, a, b);
+        return __float_as_uint(a);
+    }
 }
 
 template <int DT>
@@ -191,26 +234,26 @@ __device__ __forceinline__ float scale_value(uint32_t s)
 //
 //   mx: e = max(floor(log2 max|v|) - emax, -127): the exponent field of the
 //       float is that floor; codes of v * 2^-e, an exact product.
-//   nv: s = e4m3(max|v| / (6 g)); codes of v / (s g).  The quotient is the
-//       correctly rounded one (reciprocal, product, one correction by the
-//       remainder), because values on the middle between two codes are common
-//       in 16-bit inputs and v * (1 / (s g)) alone would leave that middle.
+//   nv: s = e4m3(max|v| * (1 / (6 g))), the reciprocal rounded once for the
+//       tensor; codes of v / (s g).  That quotient is the correctly rounded one
+//       (reciprocal, product, one correction by the remainder), because values
+//       on the middle between two codes are common in 16-bit inputs and
+//       v * (1 / (s g)) alone would leave that middle.
 //
 // A block with an infinity or a NaN gets the NaN scale and zero codes: all of
 // it reads back as NaN and so does every product with it.
-template <int F>
-__device__ __forceinline__ void quantise_chunk(float (&v)[16], float tensor_scale, float six_tensor_scale,
+template <int F, int DT>
+__device__ __forceinline__ void quantise_chunk(const Raw<DT>& x, float tensor_scale, float inv_six_scale,
                                                uint32_t (&codes)[4], uint32_t& scale)
 {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-        m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);  // orders NaN above infinity above the finite
+    uint32_t m = largest_raw<DT>(x);
+    float v[16];
+    unpack_raw<DT>(x, v);
     if constexpr (!Mx<F>::kIsNv)
         m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
     const bool finite = m < 0x7F800000u;
     if constexpr (Mx<F>::kIsNv) {
-        const float want = __fdiv_rn(__uint_as_float(m), six_tensor_scale);
+        const float want = __uint_as_float(m) * inv_six_scale;
         const float w4[4] = {want, 0.0f, 0.0f, 0.0f};
         scale = finite ? e4m3x4(w4) & 0xFFu : 0x7Fu;
         const float r = scale_value<F>(scale) * tensor_scale;

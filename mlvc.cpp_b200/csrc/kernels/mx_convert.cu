@@ -45,6 +45,8 @@ __device__ __forceinline__ long long cache_slot(const MxConvertParams& p, long l
 template <int DT, int F, bool kCache, bool kRead>
 __device__ __forceinline__ void mx_convert(const MxConvertParams& p)
 {
+    pdl_launch_dependents();
+    pdl_wait();
     __shared__ long long slots[kCache ? kMxCacheRowsMax : 1];
     const long long row0 = static_cast<long long>(blockIdx.x) * p.cta_rows;
     const int rows = static_cast<int>(min(static_cast<long long>(p.cta_rows), p.rows - row0));
@@ -69,7 +71,6 @@ __device__ __forceinline__ void mx_convert(const MxConvertParams& p)
             held = valid ? slots[r] : -1;
         const int column = Mx<F>::kIsNv ? c : c >> 1;
         uint32_t codes[4] = {0, 0, 0, 0}, scale = 0;
-        float v[16];
         uint8_t* data = p.data + held * p.pitch + c * Mx<F>::kChunkBytes;
         uint8_t* at = p.scales + (kCache ? held * p.scale_pitch + column : scale_at(held, column, p.k_tiles));
         if constexpr (kRead) {
@@ -82,16 +83,14 @@ __device__ __forceinline__ void mx_convert(const MxConvertParams& p)
                     *reinterpret_cast<uint2*>(codes) = *reinterpret_cast<const uint2*>(data);
                 scale = *at;
             }
+            float v[16];
             read_chunk<F>(codes, scale, p.tensor_scale, v);
             store_chunk<DT>(p.dense, row * p.row_stride, p.col_stride, c * 16, p.cols, p.vec, v);
         } else {
+            Raw<DT> x{};
             if (valid)
-                load_chunk<DT>(p.dense, row * p.row_stride, p.col_stride, c * 16, p.cols, p.vec, v);
-            else
-#pragma unroll
-                for (int k = 0; k < 16; ++k)
-                    v[k] = 0.0f;
-            quantise_chunk<F>(v, p.tensor_scale, p.six_tensor_scale, codes, scale);
+                load_raw<DT>(p.dense, row * p.row_stride, p.col_stride, c * 16, p.cols, p.vec, x);
+            quantise_chunk<F, DT>(x, p.tensor_scale, p.inv_six_scale, codes, scale);
             if (!valid || (kCache && held < 0))
                 continue;
             if constexpr (Mx<F>::kIs8)

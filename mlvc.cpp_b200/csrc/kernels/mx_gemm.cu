@@ -12,7 +12,7 @@ constexpr unsigned int kErrMxEpilogue = 0x4u;
 
 // 32 results of one row from column `col`.
 template <int DT>
-__device__ __forceinline__ void mx_store_row(const MxGemmParams& p, long long row, int col, float (&v)[32])
+__device__ __forceinline__ void mx_store_row(const MxEpilogue& p, long long row, int col, float (&v)[32])
 {
     using D = Dense<DT>;
     using T = typename D::T;
@@ -55,7 +55,7 @@ __device__ __forceinline__ void mx_store_row(const MxGemmParams& p, long long ro
             y[i] = D::pack(res ? v[i] + D::load(res + i) : v[i]);
 }
 
-__device__ __forceinline__ void mx_finish(const MxGemmParams& p, long long row, int col, const uint32_t (&acc)[32])
+__device__ __forceinline__ void mx_finish(const MxEpilogue& p, long long row, int col, const uint32_t (&acc)[32])
 {
     if (row >= p.M || col >= p.N)
         return;
@@ -131,11 +131,15 @@ __device__ __forceinline__ void mx_gemm(const MxGemmParams& p)
         sh->abort_flag = 0;
         fence_barrier_init();
     }
+    // TMEM is taken once the kernel before has ended: one that allocates after
+    // it let this one start would otherwise wait for columns held here
+    pdl_wait();
     if (warp == 1)
         tmem_alloc(&sh->tmem_base, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_launch_dependents();
     const uint32_t tmem = sh->tmem_base;
     const int total = p.m_tiles * p.n_tiles;
     bool issuer = false;
@@ -149,23 +153,23 @@ __device__ __forceinline__ void mx_gemm(const MxGemmParams& p)
             for (int t = blockIdx.x; t < total && !sh->abort_flag; t += gridDim.x) {
                 int mt, nt;
                 mx_tile_at(p, t, mt, nt);
-                for (int k = 0; k < p.k_stages; ++k) {
+                for (int k = 0; k < p.k.count; ++k) {
                     if (!mbar_wait(&sh->empty[stage], phase ^ 1u, &sh->abort_flag, kErrMxProducer))
                         break;
                     uint8_t* s = stages + stage * T::kStage;
                     uint64_t* bar = &sh->full[stage];
-                    const uint32_t sbytes = 512u * (k + 1 == p.k_stages ? p.last_words : kWords);
+                    const uint32_t sbytes = 512u * (k + 1 == p.k.count ? p.k.last_words : kWords);
                     // bands past the last row of B have no scales
-                    const int bands = min(T::kBands, (p.N - nt * BN + 127) / 128);
+                    const int bands = min(T::kBands, (p.e.N - nt * BN + 127) / 128);
                     mbar_arrive_expect_tx(bar, T::kA + T::kB + sbytes * (1 + bands));
                     tma_load_2d(s, &p.map_a, bar, k * 128, mt * 128);
                     tma_load_2d(s + T::kA, &p.map_b, bar, k * 128, nt * BN);
                     const long long word = static_cast<long long>(k) * kWords;
-                    bulk_load(s + T::kA + T::kB, p.scales_a + (static_cast<long long>(mt) * p.k_tiles + word) * 512,
+                    bulk_load(s + T::kA + T::kB, p.scales_a + (static_cast<long long>(mt) * p.k.k_tiles + word) * 512,
                               sbytes, bar);
                     for (int b = 0; b < bands; ++b)
                         bulk_load(s + T::kA + T::kB + T::kSA * (1 + b),
-                                  p.scales_b + ((static_cast<long long>(nt) * BN / 128 + b) * p.k_tiles + word) * 512, sbytes,
+                                  p.scales_b + ((static_cast<long long>(nt) * BN / 128 + b) * p.k.k_tiles + word) * 512, sbytes,
                                   bar);
                     armed |= 1u << stage;
                     parity = (parity & ~(1u << stage)) | (phase << stage);
@@ -200,15 +204,15 @@ __device__ __forceinline__ void mx_gemm(const MxGemmParams& p)
                 int mt, nt;
                 mx_tile_at(p, t, mt, nt);
                 const uint32_t in_band = BN < 128 ? (nt * BN % 128) / 32 : 0;
-                for (int k = 0; k < p.k_stages; ++k) {
+                for (int k = 0; k < p.k.count; ++k) {
                     if (!mbar_wait(&sh->full[stage], phase, &sh->abort_flag, kErrMxMma)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
                     const uint32_t s = smem_u32(stages + stage * T::kStage);
-                    const bool last = k + 1 == p.k_stages;
-                    const int words = last ? p.last_words : kWords, steps = last ? p.last_steps : 4;
+                    const bool last = k + 1 == p.k.count;
+                    const int words = last ? p.k.last_words : kWords, steps = last ? p.k.last_steps : 4;
                     for (int w = 0; w < words; ++w) {
                         tmem_copy_scales(tmem_sa + 4 * w, s + T::kA + T::kB + 512 * w);
 #pragma unroll
@@ -252,7 +256,7 @@ __device__ __forceinline__ void mx_gemm(const MxGemmParams& p)
                 uint32_t v[32];
                 tmem_ld32_nowait(tmem + acc * BN + c + (static_cast<uint32_t>(quadrant * 32) << 16), v);
                 tmem_wait_ld();
-                mx_finish(p, static_cast<long long>(mt) * 128 + quadrant * 32 + lane, nt * BN + c, v);
+                mx_finish(p.e, static_cast<long long>(mt) * 128 + quadrant * 32 + lane, nt * BN + c, v);
                 __syncwarp();
             }
             tc_fence_before();

@@ -35,7 +35,7 @@ struct MxConvertParams {
     long long pitch;                   // bytes of a quantised row
     int k_tiles;                       // matrix: scale tiles of a 128-row band
     int scale_pitch;                   // cache: scales of a row
-    float tensor_scale, six_tensor_scale;
+    float tensor_scale, inv_six_scale;
     // cache: where row t of the packed rows lies
     const int* pages;                  // [sequences, pages_per_sequence], < 0: no page
     const int* offsets;                // [sequences + 1]: first packed row of each sequence
@@ -45,17 +45,9 @@ struct MxConvertParams {
 
 constexpr int kMxCacheRowsMax = 64;  // rows of one CTA of a cache kernel
 
-// y = leaky(alpha * a . b^T + bias) + residual
-struct MxGemmParams {
-    CUtensorMap map_a, map_b;          // bytes [rows, pitch], boxes of 128 bytes x the tile's rows, 128-byte swizzle
-    const uint8_t* scales_a;
-    const uint8_t* scales_b;
-    int k_tiles;                       // scale tiles of a 128-row band
-    int k_stages;                      // 128-byte panels of a row
-    int last_steps;                    // MMA steps of the last panel (32 bytes each)
-    int last_words;                    // scale tiles of the last panel
-    int M, N;
-    int m_tiles, n_tiles;
+// What becomes of a product's sums: y = leaky(alpha * sum + bias) + residual.
+struct MxEpilogue {
+    int M, N;                          // rows and columns of y
     const float* bias;                 // [N] or null
     const void* residual;              // y's type, or null
     long long residual_stride;
@@ -64,6 +56,44 @@ struct MxGemmParams {
     int y_dtype;
     int vec;                           // y and residual rows begin on 16-byte boundaries
     float alpha, slope;
+};
+
+// How rows of both operands are cut along k: panels of 128 bytes, the last one
+// with fewer MMA steps (32 bytes each) and scale tiles.
+struct MxPanels {
+    int k_tiles;                       // scale tiles of a 128-row band
+    int count;
+    int last_steps;
+    int last_words;
+};
+
+struct MxGemmParams {
+    CUtensorMap map_a, map_b;          // bytes [rows, pitch], boxes of 128 bytes x the tile's rows, 128-byte swizzle
+    const uint8_t* scales_a;
+    const uint8_t* scales_b;
+    MxPanels k;
+    int m_tiles, n_tiles;
+    MxEpilogue e;
+};
+
+// Products of at most 128 rows (see mx_rows): weights are the tensor core's
+// first operand, rows its second.
+constexpr int kMxRowsMax = 128;
+struct MxRowsParams {
+    CUtensorMap map_w;                 // weights, boxes of 128 bytes x 128 rows
+    CUtensorMap map_x;                 // quantised rows, boxes of 128 bytes x row_tile rows
+    const uint8_t* scales_w;
+    const uint8_t* scales_x;
+    MxPanels k;
+    int splits;                        // CTAs of a cluster, each with its share of the panels
+    int row_tile;                      // rows rounded up to 8
+    int stages;
+    // dense rows
+    const void* x;
+    long long row_stride, col_stride;
+    int cols, vec;
+    float tensor_scale, inv_six_scale;
+    MxEpilogue e;
 };
 
 }  // namespace mlvc_b200
