@@ -94,6 +94,8 @@ MLVC_FWD(cuLaunchKernel,
           extra))
 MLVC_FWD(cuLaunchKernelEx, (const CUlaunchConfig* config, CUfunction f, void** kernelParams, void** extra),
          (config, f, kernelParams, extra))
+MLVC_FWD(cuOccupancyMaxActiveClusters, (int* numClusters, CUfunction func, const CUlaunchConfig* config),
+         (numClusters, func, config))
 MLVC_FWD(cuStreamBeginCapture, (CUstream hStream, CUstreamCaptureMode mode), (hStream, mode))
 MLVC_FWD(cuStreamEndCapture, (CUstream hStream, CUgraph* phGraph), (hStream, phGraph))
 MLVC_FWD(cuGraphInstantiateWithFlags, (CUgraphExec * phGraphExec, CUgraph hGraph, unsigned long long flags),

@@ -207,6 +207,30 @@ void Mx::launch(int index, unsigned grid_x, unsigned grid_y, unsigned block, uns
     check(cuLaunchKernelEx(&cfg, fn(index), args, nullptr), "cuLaunchKernelEx(mx)");
 }
 
+// Clusters of this many one-CTA-an-SM blocks that run at once.
+int Mx::clusters(int size)
+{
+    int& known = clusters_[size];
+    if (!known) {
+        CUlaunchAttribute attr{};
+        attr.id = CU_LAUNCH_ATTRIBUTE_CLUSTER_DIMENSION;
+        attr.value.clusterDim.x = size;
+        attr.value.clusterDim.y = attr.value.clusterDim.z = 1;
+        CUlaunchConfig cfg{};
+        cfg.gridDimX = size;
+        cfg.gridDimY = cfg.gridDimZ = 1;
+        cfg.blockDimX = 320;
+        cfg.blockDimY = cfg.blockDimZ = 1;
+        cfg.sharedMemBytes = kGemmSmem;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        check(cuOccupancyMaxActiveClusters(&n, fn(kRows), &cfg), "cuOccupancyMaxActiveClusters");
+        known = std::max(n, 1);
+    }
+    return known;
+}
+
 // A CTA of 256 threads takes up to 1024 chunks: up to 256 of a row, as many
 // rows as that leaves.  Small calls get fewer rows a CTA, down to one chunk a
 // thread, so that they reach more SMs.
@@ -429,14 +453,15 @@ bool Mx::few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream)
     const int64_t rows = a ? a->rows : l.x.rows;
     if (rows > kMxRowsMax)
         return false;
+    ContextGuard guard(ctx_);
     MxRowsParams p{};
     p.k = panels_of(w.format, w.cols);
     const int64_t n_tiles = ceil_div(w.rows, 128);
-    // as many CTAs on k as keep all SMs at work, a power of two so that
-    // clusters fill the groups of SMs
-    p.splits = 1;
-    while (p.splits < 8 && n_tiles * p.splits * 2 <= sm_count_ && p.splits * 2 <= p.k.count)
-        p.splits *= 2;
+    // as many CTAs on k as there are SMs for at once: clusters take SMs of one
+    // group, so fewer of them fit than SMs divided by their size
+    p.splits = static_cast<int>(std::min<int64_t>(8, p.k.count));
+    while (p.splits > 1 && n_tiles > clusters(p.splits))
+        --p.splits;
     const int64_t grid = n_tiles * p.splits;
     p.row_tile = static_cast<int>(ceil_div(rows, 8) * 8);
     const size_t x_bytes = static_cast<size_t>(p.row_tile) * 128, most = ceil_div(p.k.count, p.splits);
@@ -454,7 +479,6 @@ bool Mx::few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream)
         smem = std::max(smem, fixed + static_cast<size_t>(p.row_tile) * 512);
     if (smem > whole)
         return false;
-    ContextGuard guard(ctx_);
     const size_t pitch = pitch_of(w.format, w.cols);
     encode_rows(&p.map_w, w.data, pitch, w.rows, 128);
     p.scales_w = reinterpret_cast<const uint8_t*>(w.scales);
@@ -470,6 +494,8 @@ bool Mx::few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream)
         p.vec = wide(l.x);
         p.tensor_scale = x_scale;
         p.inv_six_scale = 1.0f / (6.0f * x_scale);
+        const int64_t panel_chunks = rows * (w.format == kMxFp8 ? 8 : 16);
+        p.group = static_cast<int>(std::max({int64_t{1}, 1024 / panel_chunks, ceil_div(most, 32)}));
     }
     p.e = epilogue_of(l, rows, x_scale);
     const int type = a ? 0 : l.x.dtype == kMxF16 ? 1 : l.x.dtype == kMxBf16 ? 2 : 3;

@@ -84,6 +84,7 @@ private:
     // product's kernel itself; false: there is no such kernel for these sizes.
     bool few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream);
     void product(const MxLinear& l, const MxMatrix& a, CUstream stream);
+    int clusters(int size);
     void launch(int index, unsigned grid_x, unsigned grid_y, unsigned block, unsigned smem, unsigned cluster, void* params,
                 CUstream stream);
     void require_device() const;
@@ -93,6 +94,7 @@ private:
     CUdeviceptr status_ = 0;
     int sm_count_ = 0;
     CUfunction functions_[64] = {};
+    int clusters_[9] = {};  // by size, 0: not asked yet
 };
 
 }  // namespace mlvc_b200

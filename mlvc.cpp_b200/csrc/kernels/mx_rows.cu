@@ -21,12 +21,13 @@ namespace mlvc_b200 {
 
 constexpr int kMxRowsThreads = 320;
 constexpr int kMxRowsMaxStages = 12;
+constexpr int kMxRowsMaxGroups = 32;  // of panels of x (see MxRowsParams::group)
 constexpr int kMxRowsHeader = 1024;
 
 struct MxRowsShared {
     uint64_t full[kMxRowsMaxStages];
     uint64_t empty[kMxRowsMaxStages];
-    uint64_t x_full;
+    uint64_t x_full[kMxRowsMaxGroups];
     uint64_t sums;
     uint64_t drain;
     uint32_t tmem_base;
@@ -39,12 +40,13 @@ __device__ __forceinline__ void cluster_barrier()
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-__device__ __forceinline__ float load_cluster(uint32_t saddr, uint32_t rank)
+__device__ __forceinline__ float4 load_cluster(uint32_t saddr, uint32_t rank)
 {
-    float v;
+    float4 v;
     asm volatile(
-        "{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}"
-        : "=f"(v)
+        "{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\t"
+        "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
+        : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
         : "r"(saddr), "r"(rank));
     return v;
 }
@@ -103,7 +105,9 @@ __device__ __forceinline__ void mx_rows(const MxRowsParams& p)
             mbar_init(&sh->full[s], 1);
             mbar_init(&sh->empty[s], 1);
         }
-        mbar_init(&sh->x_full, 256);
+        if constexpr (kDense)
+            for (int g = 0; g * p.group < panels; ++g)
+                mbar_init(&sh->x_full[g], 256);
         mbar_init(&sh->sums, 1);
         mbar_init(&sh->drain, 1);
         sh->abort_flag = 0;
@@ -166,8 +170,13 @@ __device__ __forceinline__ void mx_rows(const MxRowsParams& p)
             const uint32_t tmem_sw = tmem + p.row_tile, tmem_sx = tmem_sw + 4 * kWords;
             int stage = 0;
             uint32_t phase = 0;
-            bool ok = !kDense || mbar_wait(&sh->x_full, 0, &sh->abort_flag, kErrMxMma);
-            for (int k = k0; ok && k < k1; ++k) {
+            bool ok = true;
+            for (int k = k0, g = 0; ok && k < k1; ++k) {
+                if (kDense && k - k0 == g * p.group &&
+                    !mbar_wait(&sh->x_full[g++], 0, &sh->abort_flag, kErrMxMma)) {
+                    ok = false;
+                    break;
+                }
                 if (!mbar_wait(&sh->full[stage], phase, &sh->abort_flag, kErrMxMma)) {
                     ok = false;
                     break;
@@ -204,31 +213,48 @@ __device__ __forceinline__ void mx_rows(const MxRowsParams& p)
     } else {
         const int t = threadIdx.x - 64;  // 0..255
         if constexpr (kDense) {
+            // a group of panels at a time, four chunks a thread under way at once
             constexpr int kChunks = Mx<F>::kPanelValues / 16;  // of a panel
-            const int row_chunks = panels * kChunks, items = M * row_chunks;
-            for (int i = t; i < ((items + 31) & ~31); i += 256) {
-                const int m = i / row_chunks, c = i - m * row_chunks;
-                Raw<DT> x{};
-                if (i < items)
-                    load_raw<DT>(p.x, m * p.row_stride, p.col_stride, (k0 * kChunks + c) * 16, p.cols, p.vec, x);
-                uint32_t codes[4], scale;
-                quantise_chunk<F, DT>(x, p.tensor_scale, p.inv_six_scale, codes, scale);
-                if (i >= items)
-                    continue;
-                const int panel = c / kChunks, in = c % kChunks;
-                const int byte = in * Mx<F>::kChunkBytes;
-                uint8_t* to = x_tiles + panel * x_bytes + m * 128 + (((byte >> 4) ^ (m & 7)) << 4) + (byte & 15);
-                if constexpr (Mx<F>::kIs8)
-                    *reinterpret_cast<uint4*>(to) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
-                else
-                    *reinterpret_cast<uint2*>(to) = make_uint2(codes[0], codes[1]);
-                const int column = Mx<F>::kIsNv ? in : in >> 1;
-                if (Mx<F>::kIsNv || !(in & 1))
-                    x_scales[panel * kS + (column >> 2) * 512 + (m & 31) * 16 + (m >> 5) * 4 + (column & 3)] =
-                        static_cast<uint8_t>(scale);
+            constexpr int kBatch = 4;
+            for (int g = 0; g * p.group < panels; ++g) {
+                const int first = g * p.group;  // panel
+                const int row_chunks = min(p.group, panels - first) * kChunks, items = M * row_chunks;
+                for (int i0 = t; i0 < ((items + 31) & ~31); i0 += 256 * kBatch) {
+                    Raw<DT> x[kBatch];
+#pragma unroll
+                    for (int b = 0; b < kBatch; ++b) {
+                        const int i = i0 + 256 * b, m = i / row_chunks, c = i - m * row_chunks;
+                        if (i < items)
+                            load_raw<DT>(p.x, m * p.row_stride, p.col_stride, ((k0 + first) * kChunks + c) * 16, p.cols, p.vec,
+                                         x[b]);
+                        else
+                            x[b] = Raw<DT>{};
+                    }
+#pragma unroll
+                    for (int b = 0; b < kBatch; ++b) {
+                        const int i = i0 + 256 * b, m = i / row_chunks, c = i - m * row_chunks;
+                        if ((i & ~31) >= items)  // whole warps
+                            break;
+                        uint32_t codes[4], scale;
+                        quantise_chunk<F, DT>(x[b], p.tensor_scale, p.inv_six_scale, codes, scale);
+                        if (i >= items)
+                            continue;
+                        const int panel = first + c / kChunks, in = c % kChunks;
+                        const int byte = in * Mx<F>::kChunkBytes;
+                        uint8_t* to = x_tiles + panel * x_bytes + m * 128 + (((byte >> 4) ^ (m & 7)) << 4) + (byte & 15);
+                        if constexpr (Mx<F>::kIs8)
+                            *reinterpret_cast<uint4*>(to) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+                        else
+                            *reinterpret_cast<uint2*>(to) = make_uint2(codes[0], codes[1]);
+                        const int column = Mx<F>::kIsNv ? in : in >> 1;
+                        if (Mx<F>::kIsNv || !(in & 1))
+                            x_scales[panel * kS + (column >> 2) * 512 + (m & 31) * 16 + (m >> 5) * 4 + (column & 3)] =
+                                static_cast<uint8_t>(scale);
+                    }
+                }
+                fence_proxy_async_smem();  // the tensor core reads through the async proxy
+                mbar_arrive(&sh->x_full[g]);
             }
-            fence_proxy_async_smem();  // the tensor core reads through the async proxy
-            mbar_arrive(&sh->x_full);
         }
         // the warp's quadrant of the 128 weight rows, half of the columns (rows
         // of x, 32 at a time)
@@ -266,15 +292,25 @@ __device__ __forceinline__ void mx_rows(const MxRowsParams& p)
     if (p.splits > 1) {
         cluster_barrier();  // every CTA's part is written
         if (warp >= 2) {
-            const int n = threadIdx.x & 127, half = (threadIdx.x - 64) >> 7;
-            if (n0 + n < p.e.N) {
-                const float bias = p.e.bias ? p.e.bias[n0 + n] : 0.0f;
-                const uint32_t part = smem_u32(ring);
-                for (int m = static_cast<int>(rank) + p.splits * half; m < M; m += 2 * p.splits) {
-                    float sum = 0.0f;
-                    for (int r = 0; r < p.splits; ++r)
-                        sum += load_cluster(part + (m * 128 + n) * 4, r);
-                    mx_finish_one(p.e, m, n0 + n, sum, bias);
+            // a warp takes a row of x: four columns a lane, all parts under way at once
+            const uint32_t part = smem_u32(ring) + lane * 16;
+            for (int m = static_cast<int>(rank) + p.splits * (warp - 2); m < M; m += 8 * p.splits) {
+                float4 v[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (r < p.splits)
+                        v[r] = load_cluster(part + m * 512, r);
+                float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (r < p.splits)
+                        sum = make_float4(sum.x + v[r].x, sum.y + v[r].y, sum.z + v[r].z, sum.w + v[r].w);
+                const float s[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int n = n0 + lane * 4 + i;
+                    if (n < p.e.N)
+                        mx_finish_one(p.e, m, n, s[i], p.e.bias ? p.e.bias[n] : 0.0f);
                 }
             }
         }
