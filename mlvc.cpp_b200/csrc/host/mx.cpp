@@ -184,8 +184,7 @@ unsigned int Mx::take_status()
 
 // Kernels start while the one before drains (programmatic dependent launch);
 // they wait for it before they touch memory.
-void Mx::launch(int index, unsigned grid_x, unsigned grid_y, unsigned block, unsigned smem, unsigned cluster, void* params,
-                CUstream stream)
+void Mx::launch(int index, unsigned grid, unsigned block, unsigned smem, unsigned cluster, void* params, CUstream stream)
 {
     CUlaunchAttribute attrs[2]{};
     attrs[0].id = CU_LAUNCH_ATTRIBUTE_PROGRAMMATIC_STREAM_SERIALIZATION;
@@ -194,9 +193,8 @@ void Mx::launch(int index, unsigned grid_x, unsigned grid_y, unsigned block, uns
     attrs[1].value.clusterDim.x = cluster;
     attrs[1].value.clusterDim.y = attrs[1].value.clusterDim.z = 1;
     CUlaunchConfig cfg{};
-    cfg.gridDimX = grid_x;
-    cfg.gridDimY = grid_y;
-    cfg.gridDimZ = 1;
+    cfg.gridDimX = grid;
+    cfg.gridDimY = cfg.gridDimZ = 1;
     cfg.blockDimX = block;
     cfg.blockDimY = cfg.blockDimZ = 1;
     cfg.sharedMemBytes = smem;
@@ -231,9 +229,6 @@ int Mx::clusters(int size)
     return known;
 }
 
-// A CTA of 256 threads takes up to 1024 chunks: up to 256 of a row, as many
-// rows as that leaves.  Small calls get fewer rows a CTA, down to one chunk a
-// thread, so that they reach more SMs.
 void Mx::convert(const MxDense& d, int format, float tensor_scale, uint64_t data, uint64_t scales, const MxCache* cache,
                  const MxRows* rows, bool read, CUstream stream)
 {
@@ -248,13 +243,27 @@ void Mx::convert(const MxDense& d, int format, float tensor_scale, uint64_t data
     p.rows = d.rows;
     p.cols = static_cast<int>(d.cols);
     p.chunks = chunks_of(d.cols);
-    p.cta_chunks = std::min(p.chunks, 256);
-    const int64_t columns = ceil_div(p.chunks, p.cta_chunks);
-    int64_t cta_rows = std::max(1, 1024 / p.cta_chunks);
-    const int64_t least = std::max(1, 256 / p.cta_chunks);
-    while (cta_rows > least && ceil_div(d.rows, cta_rows) * columns < 4 * sm_count_)
-        cta_rows = std::max(least, cta_rows / 2);
-    p.cta_rows = static_cast<int>(std::min<int64_t>(cta_rows, kMxCacheRowsMax));
+    // the widest warp that leaves the fewest lanes idle, at least a row's
+    // chunks or 8 (256 bytes of 16-bit values in one piece)
+    int idle = 1 << 30;
+    for (int bits = 5; bits >= 1; --bits) {
+        const int lanes = 1 << bits, segments = static_cast<int>(ceil_div(p.chunks, lanes));
+        if (bits < 3 && p.chunks > lanes)
+            break;
+        if (segments * lanes - p.chunks < idle) {
+            idle = segments * lanes - p.chunks;
+            p.lane_bits = bits;
+            p.segments = segments;
+        }
+    }
+    // up to four groups of rows a warp (FP32: two, they are twice the bytes),
+    // fewer where that leaves SMs without work; the cache's kernels name a
+    // warp's rows with its lanes, so 32 rows at most
+    const int group_rows = 32 >> p.lane_bits;
+    p.steps = std::min(d.dtype == kMxF32 ? 2 : 4, 1 << p.lane_bits);
+    while (p.steps > 1 && ceil_div(d.rows, 8 * group_rows * p.steps) * p.segments < 2 * sm_count_)
+        p.steps /= 2;
+    const int64_t grid = ceil_div(d.rows, 8 * group_rows * p.steps) * p.segments;
     p.vec = wide(d);
     p.data = reinterpret_cast<uint8_t*>(data);
     p.scales = reinterpret_cast<uint8_t*>(scales);
@@ -274,10 +283,9 @@ void Mx::convert(const MxDense& d, int format, float tensor_scale, uint64_t data
     }
     const int base = cache ? (read ? kCacheRead : kCacheWrite) : (read ? kDequantise : kQuantise);
     const int index = convert_index(base, d.dtype, format);
-    const int64_t grid = ceil_div(d.rows, p.cta_rows);
     if (grid > 0x7FFFFFFF)
         refuse("too many rows for one call");
-    launch(index, static_cast<unsigned>(grid), static_cast<unsigned>(columns), 256, 0, 1, &p, stream);
+    launch(index, static_cast<unsigned>(grid), 256, 0, 1, &p, stream);
 }
 
 void Mx::quantise(const MxDense& x, const MxMatrix& out, CUstream stream)
@@ -499,7 +507,7 @@ bool Mx::few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream)
     }
     p.e = epilogue_of(l, rows, x_scale);
     const int type = a ? 0 : l.x.dtype == kMxF16 ? 1 : l.x.dtype == kMxBf16 ? 2 : 3;
-    launch(kRows + 3 * type + w.format, static_cast<unsigned>(grid), 1, 320, static_cast<unsigned>(smem),
+    launch(kRows + 3 * type + w.format, static_cast<unsigned>(grid), 320, static_cast<unsigned>(smem),
            static_cast<unsigned>(p.splits), &p, stream);
     return true;
 }
@@ -523,7 +531,7 @@ void Mx::product(const MxLinear& l, const MxMatrix& a, CUstream stream)
     encode_rows(&p.map_a, a.data, pitch, a.rows, 128);
     encode_rows(&p.map_b, w.data, pitch, w.rows, bn);
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>(sm_count_, static_cast<int64_t>(p.m_tiles) * p.n_tiles));
-    launch((narrow ? kGemm64 : kGemm128) + w.format, grid, 1, 320, kGemmSmem, 1, &p, stream);
+    launch((narrow ? kGemm64 : kGemm128) + w.format, grid, 320, kGemmSmem, 1, &p, stream);
 }
 
 }  // namespace mlvc_b200

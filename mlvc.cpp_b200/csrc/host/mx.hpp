@@ -85,8 +85,7 @@ private:
     bool few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream);
     void product(const MxLinear& l, const MxMatrix& a, CUstream stream);
     int clusters(int size);
-    void launch(int index, unsigned grid_x, unsigned grid_y, unsigned block, unsigned smem, unsigned cluster, void* params,
-                CUstream stream);
+    void launch(int index, unsigned grid, unsigned block, unsigned smem, unsigned cluster, void* params, CUstream stream);
     void require_device() const;
 
     CUcontext ctx_ = nullptr;

@@ -177,6 +177,30 @@ __device__ __forceinline__ void store_chunk(void* dense, long long row_at, long 
             p[(col + i) * col_stride] = D::pack(v[i]);
 }
 
+// Two floats in a register pair: one instruction for both.
+__device__ __forceinline__ uint64_t pair(float a, float b)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void split(uint64_t p, float& a, float& b)
+{
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
 // ------------------------------------------------------ block arithmetic
 // Eight E2M1 codes of v[0..7], the first in the lowest four bits; nearest,
 // ties to even, larger magnitudes become 6.
@@ -235,10 +259,10 @@ __device__ __forceinline__ float scale_value(uint32_t s)
 //   mx: e = max(floor(log2 max|v|) - emax, -127): the exponent field of the
 //       float is that floor; codes of v * 2^-e, an exact product.
 //   nv: s = e4m3(max|v| * (1 / (6 g))), the reciprocal rounded once for the
-//       tensor; codes of v / (s g).  That quotient is the correctly rounded one
-//       (reciprocal, product, one correction by the remainder), because values
-//       on the middle between two codes are common in 16-bit inputs and
-//       v * (1 / (s g)) alone would leave that middle.
+//       tensor; codes of v / (s g).  Values on the middle between two codes are
+//       common in 16-bit inputs, and v * (1 / (s g)) alone would leave that
+//       middle, so the reciprocal is held in two floats: h + l is 1 / (s g) to
+//       2^-47, and v h + v l, rounded once, meets the middle exactly.
 //
 // A block with an infinity or a NaN gets the NaN scale and zero codes: all of
 // it reads back as NaN and so does every product with it.
@@ -257,31 +281,38 @@ __device__ __forceinline__ void quantise_chunk(const Raw<DT>& x, float tensor_sc
         const float w4[4] = {want, 0.0f, 0.0f, 0.0f};
         scale = finite ? e4m3x4(w4) & 0xFFu : 0x7Fu;
         const float r = scale_value<F>(scale) * tensor_scale;
-        if (!finite || !(r > 0.0f)) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                v[i] = finite ? v[i] * 0.0f : 0.0f;  // zeros keep their sign
-        } else if (scale != 0x7Eu && r > 0x1p-100f && r < 0x1p100f) {
+        if (scale < 0x7Eu && r > 0x1p-100f && r < 0x1p100f) {
             // |v / r| stays below 8 here, so nothing overflows, and what
             // underflows is far below the smallest code's half
-            const float inv = __frcp_rn(r);
+            const float h = __frcp_rd(r);  // rounded down: l >= 0, and a zero keeps its sign
+            const float l = fmaf(-r, h, 1.0f) * h;
+            const uint64_t hh = pair(h, h), ll = pair(l, l);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float q = v[i] * inv;
-                v[i] = fmaf(-fmaf(q, r, -v[i]), inv, q);  // a zero keeps its sign this way round
+            for (int i = 0; i < 16; i += 2) {
+                const uint64_t vv = pair(v[i], v[i + 1]);
+                split(fma2(vv, hh, mul2(vv, ll)), v[i], v[i + 1]);
             }
-        } else {
+        } else if (r > 0.0f && finite) {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 v[i] = __fdiv_rn(v[i], r);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                v[i] = finite ? v[i] * 0.0f : 0.0f;  // zeros keep their sign
         }
     } else {
         const int e = static_cast<int>(m >> 23) - Mx<F>::kExponentMax;
         scale = finite ? static_cast<uint32_t>(max(e, 0)) : 255u;
         const float inv = finite ? __uint_as_float((254u - scale) << 23) : 0.0f;
+        const uint64_t ii = pair(inv, inv);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            v[i] = finite ? v[i] * inv : 0.0f;
+        for (int i = 0; i < 16; i += 2)
+            split(mul2(pair(v[i], v[i + 1]), ii), v[i], v[i + 1]);
+        if (!finite)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                v[i] = 0.0f;
     }
     if constexpr (Mx<F>::kIs8) {
 #pragma unroll
@@ -300,36 +331,43 @@ template <int F>
 __device__ __forceinline__ void read_chunk(const uint32_t (&codes)[4], uint32_t scale, float tensor_scale,
                                            float (&v)[16])
 {
-    const float s = scale_value<F>(scale);
+    uint32_t h[8];  // the codes as pairs of halves
     if constexpr (Mx<F>::kIs8) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            e4m3x2_to_floats(codes[i] & 0xFFFFu, v[4 * i], v[4 * i + 1]);
-            e4m3x2_to_floats(codes[i] >> 16, v[4 * i + 2], v[4 * i + 3]);
-        }
+        for (int i = 0; i < 4; ++i)
+            asm("{\n\t.reg .b16 l, u;\n\tmov.b32 {l, u}, %2;\n\t"
+                "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, u;\n\t}"
+                : "=r"(h[2 * i]), "=r"(h[2 * i + 1])
+                : "r"(codes[i]));
     } else {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            uint32_t h0, h1, h2, h3;
+        for (int i = 0; i < 2; ++i)
             asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
                 "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
                 "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
                 "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
                 "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
                 "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
-                : "=r"(h0), "=r"(h1), "=r"(h2), "=r"(h3)
+                : "=r"(h[4 * i]), "=r"(h[4 * i + 1]), "=r"(h[4 * i + 2]), "=r"(h[4 * i + 3])
                 : "r"(codes[i]));
-            unpack_h2(h0, v[8 * i], v[8 * i + 1]);
-            unpack_h2(h1, v[8 * i + 2], v[8 * i + 3]);
-            unpack_h2(h2, v[8 * i + 4], v[8 * i + 5]);
-            unpack_h2(h3, v[8 * i + 6], v[8 * i + 7]);
-        }
     }
+    float f = scale_value<F>(scale);
+    if constexpr (Mx<F>::kIsNv) {
+        // E2M1 times E4M3 has at most 6 digits and lies in [2^-10, 2688]: a half holds it
+        const __half2 s = __float2half2_rn(f);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        v[i] *= s;
-        if constexpr (Mx<F>::kIsNv)
-            v[i] *= tensor_scale;
+        for (int i = 0; i < 8; ++i) {
+            const __half2 p = __hmul2(*reinterpret_cast<const __half2*>(&h[i]), s);
+            h[i] = *reinterpret_cast<const uint32_t*>(&p);
+        }
+        f = tensor_scale;
+    }
+    const uint64_t ff = pair(f, f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        float a, b;
+        unpack_h2(h[i], a, b);
+        split(mul2(pair(a, b), ff), v[2 * i], v[2 * i + 1]);
     }
 }
 

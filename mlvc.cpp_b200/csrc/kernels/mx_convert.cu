@@ -12,97 +12,132 @@ namespace mlvc_b200 {
 
 constexpr int kMxThreads = 256;
 
-// The place of packed row t in the cache, or -1 (no page, or no such row); by
-// one warp.  The sequence is the last one that begins at or before t: each
-// round asks 32 offsets at once, so 1024 sequences take two dependent loads.
-__device__ __forceinline__ long long cache_slot(const MxConvertParams& p, long long t)
+// The places of a warp's packed rows in the cache: lane j * share + ... of the
+// result holds row t0 + j's (share = 32 / rows, at least 1), -1 where it has
+// none.  The sequence is the last one that begins at or before the row: each
+// round a row's lanes ask `share` offsets at once.
+__device__ __forceinline__ long long cache_slots(const MxConvertParams& p, long long t0, int rows, int share_bits)
 {
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, share = 1 << share_bits;
+    const int mine = lane >> share_bits, in = lane & (share - 1);
+    const long long t = t0 + mine;
     int lo = 0, hi = p.sequences;
-    if (t < p.offsets[0] || t >= p.offsets[hi])
-        return -1;
-    while (hi - lo > 1) {
-        const int step = (hi - lo + 31) / 32;
-        const long long at = lo + static_cast<long long>(lane + 1) * step;
-        const int below = __popc(__ballot_sync(0xFFFFFFFFu, at < hi && p.offsets[at] <= t));
+    const bool asked = mine < rows && t < p.rows && t >= p.offsets[0] && t < p.offsets[hi];
+    if (!asked)
+        hi = 1;  // nothing to search
+    while (__any_sync(0xFFFFFFFFu, hi - lo > 1)) {
+        const int step = (hi - lo + share) / (share + 1);
+        const long long at = lo + static_cast<long long>(in + 1) * step;
+        const uint32_t votes = __ballot_sync(0xFFFFFFFFu, hi - lo > 1 && at < hi && p.offsets[at] <= t);
+        const int below = __popc(votes >> (mine << share_bits) & (share == 32 ? 0xFFFFFFFFu : (1u << share) - 1u));
         lo += below * step;
         hi = min(hi, lo + step);
     }
+    if (!asked)
+        return -1;
     const long long position = (p.starts ? p.starts[lo] : 0) + (t - p.offsets[lo]);
-    const long long place = position >= 0 ? position / p.page_rows : -1;
+    const int place = position >= 0 && position <= 0x7FFFFFFF ? static_cast<int>(position) / p.page_rows : -1;
     int page = 0;
     const bool inside = place >= 0 && place < p.pages_per_sequence;
     if (inside)
         page = p.pages[static_cast<long long>(lo) * p.pages_per_sequence + place];
     if (!inside || page >= p.page_count) {
-        if (lane == 0)
-            atomicOr(&mlvc_b200_status, kStatusCachePage);
+        atomicOr(&mlvc_b200_status, kStatusCachePage);
         return -1;
     }
-    return page < 0 ? -1 : static_cast<long long>(page) * p.page_rows + (position - place * p.page_rows);
+    return page < 0 ? -1
+                    : static_cast<long long>(page) * p.page_rows +
+                          (position - static_cast<long long>(place) * p.page_rows);
 }
 
+// A warp takes `steps` groups of 32 / lanes rows, `lanes` chunks wide; a lane's
+// chunk column is the same in all of them.
 template <int DT, int F, bool kCache, bool kRead>
 __device__ __forceinline__ void mx_convert(const MxConvertParams& p)
 {
     pdl_launch_dependents();
     pdl_wait();
-    __shared__ long long slots[kCache ? kMxCacheRowsMax : 1];
-    const long long row0 = static_cast<long long>(blockIdx.x) * p.cta_rows;
-    const int rows = static_cast<int>(min(static_cast<long long>(p.cta_rows), p.rows - row0));
-    const int chunk0 = blockIdx.y * p.cta_chunks;
-    const int chunks = min(p.cta_chunks, p.chunks - chunk0);
-    if constexpr (kCache) {
-        for (int r = threadIdx.x / 32; r < rows; r += kMxThreads / 32) {
-            const long long s = cache_slot(p, row0 + r);
-            if (threadIdx.x % 32 == 0)
-                slots[r] = s;
-        }
-        __syncthreads();
-    }
-    const int items = rows * chunks;
-    // whole warps: the shuffle of the 32-value formats
-    for (int i = threadIdx.x; i < ((items + 31) & ~31); i += kMxThreads) {
-        const int r = i / chunks, c = chunk0 + i - r * chunks;
-        const long long row = row0 + r;
-        const bool valid = i < items;
-        long long held = row;  // row of the quantised form
-        if constexpr (kCache)
-            held = valid ? slots[r] : -1;
-        const int column = Mx<F>::kIsNv ? c : c >> 1;
-        uint32_t codes[4] = {0, 0, 0, 0}, scale = 0;
-        uint8_t* data = p.data + held * p.pitch + c * Mx<F>::kChunkBytes;
-        uint8_t* at = p.scales + (kCache ? held * p.scale_pitch + column : scale_at(held, column, p.k_tiles));
-        if constexpr (kRead) {
-            if (!valid)
-                continue;
-            if (!kCache || held >= 0) {
-                if constexpr (Mx<F>::kIs8)
-                    *reinterpret_cast<uint4*>(codes) = *reinterpret_cast<const uint4*>(data);
-                else
-                    *reinterpret_cast<uint2*>(codes) = *reinterpret_cast<const uint2*>(data);
-                scale = *at;
-            }
-            float v[16];
-            read_chunk<F>(codes, scale, p.tensor_scale, v);
-            store_chunk<DT>(p.dense, row * p.row_stride, p.col_stride, c * 16, p.cols, p.vec, v);
-        } else {
-            Raw<DT> x{};
-            if (valid)
-                load_raw<DT>(p.dense, row * p.row_stride, p.col_stride, c * 16, p.cols, p.vec, x);
-            quantise_chunk<F, DT>(x, p.tensor_scale, p.inv_six_scale, codes, scale);
-            if (!valid || (kCache && held < 0))
-                continue;
-            if constexpr (Mx<F>::kIs8)
-                *reinterpret_cast<uint4*>(data) = *reinterpret_cast<const uint4*>(codes);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    const int lanes = 1 << p.lane_bits, group_bits = 5 - p.lane_bits;
+    const unsigned block = blockIdx.x / p.segments;
+    const int chunk = (blockIdx.x - block * p.segments) * lanes + (lane & (lanes - 1));
+    const int warp_rows = p.steps << group_bits;
+    const long long row0 = (static_cast<long long>(block) * (kMxThreads / 32) + warp) * warp_rows;
+    if (row0 >= p.rows)
+        return;
+    const long long row = row0 + (lane >> p.lane_bits);
+    const int column = Mx<F>::kIsNv ? chunk : chunk >> 1;
+    constexpr int kSteps = DT == kMxF32 ? 2 : 4;
+
+    Raw<DT> x[kRead ? 1 : kSteps];
+    if constexpr (!kRead) {
+#pragma unroll
+        for (int u = 0; u < kSteps; ++u) {
+            const long long r = row + (u << group_bits);
+            if (u < p.steps && r < p.rows && chunk < p.chunks)
+                load_raw<DT>(p.dense, r * p.row_stride, p.col_stride, chunk * 16, p.cols, p.vec, x[u]);
             else
-                *reinterpret_cast<uint2*>(data) = *reinterpret_cast<const uint2*>(codes);
-            if (Mx<F>::kIsNv || !(c & 1))
-                *at = static_cast<uint8_t>(scale);
+                x[u] = Raw<DT>{};
+        }
+    }
+    long long held[kSteps];  // row of the quantised form, or -1
+    if constexpr (kCache) {
+        // a row's lanes: 32 / warp_rows rounded down to a power of two
+        const int share_bits = warp_rows >= 32 ? 0 : 31 - __clz(32 / warp_rows);
+        const long long slot = cache_slots(p, row0, warp_rows, share_bits);
+#pragma unroll
+        for (int u = 0; u < kSteps; ++u) {
+            const int j = (u << group_bits) + (lane >> p.lane_bits);
+            held[u] = __shfl_sync(0xFFFFFFFFu, slot, (j << share_bits) & 31);
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < kSteps; ++u)
+            held[u] = row + (u << group_bits);
+    }
+    uint32_t codes[kSteps][4], scale[kSteps];
+    if constexpr (kRead) {
+#pragma unroll
+        for (int u = 0; u < kSteps; ++u) {
+            scale[u] = 0;
+            codes[u][0] = codes[u][1] = codes[u][2] = codes[u][3] = 0;
+            if (u < p.steps && row + (u << group_bits) < p.rows && chunk < p.chunks && (!kCache || held[u] >= 0)) {
+                const uint8_t* data = p.data + held[u] * p.pitch + chunk * Mx<F>::kChunkBytes;
+                if constexpr (Mx<F>::kIs8)
+                    *reinterpret_cast<uint4*>(codes[u]) = *reinterpret_cast<const uint4*>(data);
+                else
+                    *reinterpret_cast<uint2*>(codes[u]) = *reinterpret_cast<const uint2*>(data);
+                scale[u] = p.scales[kCache ? held[u] * p.scale_pitch + column : scale_at(held[u], column, p.k_tiles)];
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kSteps; ++u) {
+        if (u >= p.steps)
+            break;
+        const long long r = row + (u << group_bits);
+        const bool valid = r < p.rows && chunk < p.chunks;
+        if constexpr (kRead) {
+            float v[16];
+            read_chunk<F>(codes[u], scale[u], p.tensor_scale, v);
+            if (valid)
+                store_chunk<DT>(p.dense, r * p.row_stride, p.col_stride, chunk * 16, p.cols, p.vec, v);
+        } else {
+            quantise_chunk<F, DT>(x[u], p.tensor_scale, p.inv_six_scale, codes[u], scale[u]);
+            if (!valid || (kCache && held[u] < 0))
+                continue;
+            uint8_t* data = p.data + held[u] * p.pitch + chunk * Mx<F>::kChunkBytes;
+            if constexpr (Mx<F>::kIs8)
+                *reinterpret_cast<uint4*>(data) = *reinterpret_cast<const uint4*>(codes[u]);
+            else
+                *reinterpret_cast<uint2*>(data) = *reinterpret_cast<const uint2*>(codes[u]);
+            if (Mx<F>::kIsNv || !(chunk & 1))
+                p.scales[kCache ? held[u] * p.scale_pitch + column : scale_at(held[u], column, p.k_tiles)] =
+                    static_cast<uint8_t>(scale[u]);
             // the rest of the last scale tile: the product reads whole words
-            if (!kCache && c == p.chunks - 1)
+            if (!kCache && chunk == p.chunks - 1)
                 for (int k = column + 1; k < 4 * p.k_tiles; ++k)
-                    p.scales[scale_at(held, k, p.k_tiles)] = 0;
+                    p.scales[scale_at(held[u], k, p.k_tiles)] = 0;
         }
     }
 }

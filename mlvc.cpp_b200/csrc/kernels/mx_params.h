@@ -28,7 +28,9 @@ struct MxConvertParams {
     long long rows;
     int cols;
     int chunks;                        // chunks of a quantised row (even)
-    int cta_rows, cta_chunks;          // what one CTA handles (cta_chunks even)
+    int lane_bits;                     // a warp is 2^lane_bits chunks wide
+    int segments;                      // of that width in a row
+    int steps;                         // groups of 32 / 2^lane_bits rows of a warp
     int vec;                           // dense rows begin on 32-byte boundaries and are contiguous
     uint8_t* data;
     uint8_t* scales;
@@ -42,8 +44,6 @@ struct MxConvertParams {
     const int* starts;                 // [sequences] position of a sequence's first packed row, or null for 0
     int sequences, pages_per_sequence, page_rows, page_count;
 };
-
-constexpr int kMxCacheRowsMax = 64;  // rows of one CTA of a cache kernel
 
 // What becomes of a product's sums: y = leaky(alpha * sum + bias) + residual.
 struct MxEpilogue {
