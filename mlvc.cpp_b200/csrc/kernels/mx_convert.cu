@@ -142,16 +142,18 @@ __device__ __forceinline__ void mx_convert(const MxConvertParams& p)
     }
 }
 
-#define MLVC_MX_CONVERT(NAME, DT, F, CACHE, READ)                                                       \
-    extern "C" __global__ void __launch_bounds__(kMxThreads) NAME(const __grid_constant__ MxConvertParams p) \
-    {                                                                                                   \
-        mx_convert<DT, F, CACHE, READ>(p);                                                              \
+#define MLVC_MX_CONVERT(NAME, BOUNDS, DT, F, CACHE, READ)                                    \
+    extern "C" __global__ void __launch_bounds__ BOUNDS NAME(const __grid_constant__ MxConvertParams p) \
+    {                                                                                        \
+        mx_convert<DT, F, CACHE, READ>(p);                                                   \
     }
-#define MLVC_MX_CONVERT_ALL(T, DT, FN, F)                              \
-    MLVC_MX_CONVERT(mlvc_mx_quantise_##T##_##FN, DT, F, false, false)  \
-    MLVC_MX_CONVERT(mlvc_mx_dequantise_##T##_##FN, DT, F, false, true) \
-    MLVC_MX_CONVERT(mlvc_mx_cache_write_##T##_##FN, DT, F, true, false) \
-    MLVC_MX_CONVERT(mlvc_mx_cache_read_##T##_##FN, DT, F, true, true)
+// Quantising is bound by 64 registers a thread, four CTAs an SM; reading back
+// needs fewer of itself, and is slower when the compiler is told so.
+#define MLVC_MX_CONVERT_ALL(T, DT, FN, F)                                                     \
+    MLVC_MX_CONVERT(mlvc_mx_quantise_##T##_##FN, (kMxThreads, 4), DT, F, false, false)        \
+    MLVC_MX_CONVERT(mlvc_mx_dequantise_##T##_##FN, (kMxThreads), DT, F, false, true)          \
+    MLVC_MX_CONVERT(mlvc_mx_cache_write_##T##_##FN, (kMxThreads, 4), DT, F, true, false)      \
+    MLVC_MX_CONVERT(mlvc_mx_cache_read_##T##_##FN, (kMxThreads), DT, F, true, true)
 
 MLVC_MX_CONVERT_ALL(f16, kMxF16, mxfp4, kMxFp4)
 MLVC_MX_CONVERT_ALL(f16, kMxF16, nvfp4, kNvFp4)
