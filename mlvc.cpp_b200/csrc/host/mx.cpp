@@ -25,9 +25,10 @@ void check_format(int format, float tensor_scale)
     if (format == kNvFp4 ? !(std::isfinite(tensor_scale) && tensor_scale > 0.0f) : tensor_scale != 1.0f)
         refuse(format == kNvFp4 ? "the tensor scale must be finite and positive"
                                 : "only nvfp4 has a tensor scale: it must be 1");
-    // 6 g and s g stay finite and normal
-    if (format == kNvFp4 && (tensor_scale > 0x1p100f || tensor_scale < 0x1p-100f))
-        refuse("the tensor scale must lie in [2^-100, 2^100]");
+    // a block's scale times g lies in [2^-99, 2^99], where its reciprocal is
+    // exact enough without a test
+    if (format == kNvFp4 && (tensor_scale > 0x1p90f || tensor_scale < 0x1p-90f))
+        refuse("the tensor scale must lie in [2^-90, 2^90]");
 }
 
 constexpr int64_t kMaxCols = int64_t{1} << 24, kMaxRows = int64_t{1} << 36;
@@ -76,6 +77,9 @@ size_t pitch_of(int format, int64_t cols) { return static_cast<size_t>(chunks_of
 
 int64_t k_tiles_of(int format, int64_t cols) { return ceil_div(ceil_div(cols, block_of(format)), 4); }
 
+// 1 / (6 g), rounded once.
+float inverse_six(float tensor_scale) { return static_cast<float>(1.0 / (6.0 * tensor_scale)); }
+
 // Rows are contiguous and every chunk of 16 values begins on a 32-byte
 // boundary, so that a lane moves its chunk with one (FP32: two) accesses.
 int wide(const MxDense& d)
@@ -85,7 +89,7 @@ int wide(const MxDense& d)
 }
 
 // Order of functions_: the four conversions by type and format, then products.
-enum { kQuantise = 0, kDequantise = 9, kCacheWrite = 18, kCacheRead = 27, kGemm64 = 36, kGemm128 = 39, kRows = 42, kFunctions = 54 };
+enum { kQuantise = 0, kDequantise = 9, kCacheWrite = 18, kCacheRead = 27, kGemm64 = 36, kGemm128 = 39, kRows = 42, kPair = 54, kFunctions = 57 };
 
 int convert_index(int base, int dtype, int format) { return base + (dtype == kMxF16 ? 0 : dtype == kMxBf16 ? 3 : 6) + format; }
 
@@ -95,6 +99,8 @@ std::string function_name(int i)
     static const int types[3] = {kMxF16, kMxBf16, kMxF32};
     if (i < kGemm64)
         return std::string("mlvc_mx_") + conversions[i / 9] + "_" + kTypeNames[types[i % 9 / 3]] + "_" + kFormatNames[i % 3];
+    if (i >= kPair)
+        return std::string("mlvc_mx_pair_") + kFormatNames[i % 3];
     if (i >= kRows)
         return std::string("mlvc_mx_rows_") + (i < kRows + 3 ? "quantised" : kTypeNames[types[(i - kRows) / 3 - 1]]) + "_" +
                kFormatNames[i % 3];
@@ -261,9 +267,9 @@ void Mx::convert(const MxDense& d, int format, float tensor_scale, uint64_t data
     // warp's rows with its lanes, so 32 rows at most
     const int group_rows = 32 >> p.lane_bits;
     p.steps = std::min(d.dtype == kMxF32 ? 2 : 4, 1 << p.lane_bits);
-    while (p.steps > 1 && ceil_div(d.rows, 8 * group_rows * p.steps) * p.segments < 2 * sm_count_)
+    while (p.steps > 1 && ceil_div(d.rows, 4 * group_rows * p.steps) * p.segments < 2 * sm_count_)
         p.steps /= 2;
-    const int64_t grid = ceil_div(d.rows, 8 * group_rows * p.steps) * p.segments;
+    const int64_t grid = ceil_div(d.rows, 4 * group_rows * p.steps) * p.segments;
     p.vec = wide(d);
     p.data = reinterpret_cast<uint8_t*>(data);
     p.scales = reinterpret_cast<uint8_t*>(scales);
@@ -271,7 +277,7 @@ void Mx::convert(const MxDense& d, int format, float tensor_scale, uint64_t data
     p.k_tiles = static_cast<int>(k_tiles_of(format, d.cols));
     p.scale_pitch = format == kNvFp4 ? p.chunks : p.chunks / 2;
     p.tensor_scale = tensor_scale;
-    p.inv_six_scale = 1.0f / (6.0f * tensor_scale);
+    p.inv_six_scale = inverse_six(tensor_scale);
     if (cache) {
         p.pages = reinterpret_cast<const int*>(rows->pages);
         p.offsets = reinterpret_cast<const int*>(rows->offsets);
@@ -285,7 +291,7 @@ void Mx::convert(const MxDense& d, int format, float tensor_scale, uint64_t data
     const int index = convert_index(base, d.dtype, format);
     if (grid > 0x7FFFFFFF)
         refuse("too many rows for one call");
-    launch(index, static_cast<unsigned>(grid), 256, 0, 1, &p, stream);
+    launch(index, static_cast<unsigned>(grid), 128, 0, 1, &p, stream);
 }
 
 void Mx::quantise(const MxDense& x, const MxMatrix& out, CUstream stream)
@@ -455,6 +461,20 @@ MxEpilogue epilogue_of(const MxLinear& l, int64_t rows, float x_scale)
 }
 }  // namespace
 
+namespace {
+// Scale tiles [bands, tiles, 512 bytes] as 16-bit values: a box is at most 256 of them wide.
+void encode_scales(CUtensorMap* map, uint64_t scales, int k_tiles, int64_t bands, int box_tiles, int box_bands)
+{
+    const cuuint64_t dims[3] = {256, static_cast<cuuint64_t>(k_tiles), static_cast<cuuint64_t>(bands)};
+    const cuuint64_t strides[2] = {512, static_cast<cuuint64_t>(k_tiles) * 512};
+    const cuuint32_t box[3] = {256, static_cast<cuuint32_t>(box_tiles), static_cast<cuuint32_t>(box_bands)}, elem[3] = {1, 1, 1};
+    check(cuTensorMapEncodeTiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, reinterpret_cast<void*>(scales), dims, strides, box, elem,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
+          "cuTensorMapEncodeTiled(mx scales)");
+}
+}  // namespace
+
 bool Mx::few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream)
 {
     const MxMatrix& w = l.w;
@@ -501,7 +521,7 @@ bool Mx::few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream)
         p.cols = static_cast<int>(l.x.cols);
         p.vec = wide(l.x);
         p.tensor_scale = x_scale;
-        p.inv_six_scale = 1.0f / (6.0f * x_scale);
+        p.inv_six_scale = inverse_six(x_scale);
         const int64_t panel_chunks = rows * (w.format == kMxFp8 ? 8 : 16);
         p.group = static_cast<int>(std::max({int64_t{1}, 1024 / panel_chunks, ceil_div(most, 32)}));
     }
@@ -512,9 +532,31 @@ bool Mx::few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream)
     return true;
 }
 
+void Mx::pair(const MxLinear& l, const MxMatrix& a, CUstream stream)
+{
+    const MxMatrix& w = l.w;
+    MxPairParams p{};
+    const size_t pitch = pitch_of(w.format, w.cols);
+    p.k = panels_of(w.format, w.cols);
+    p.e = epilogue_of(l, a.rows, a.tensor_scale);
+    p.m_tiles = static_cast<int>(ceil_div(a.rows, 256));
+    p.n_tiles = static_cast<int>(ceil_div(w.rows, 256));
+    encode_rows(&p.map_a, a.data, pitch, a.rows, 128);
+    encode_rows(&p.map_b, w.data, pitch, w.rows, 128);
+    const int words = w.format == kNvFp4 ? 4 : w.format == kMxFp4 ? 2 : 1;
+    encode_scales(&p.map_sa, a.scales, p.k.k_tiles, ceil_div(a.rows, 128), words, 1);
+    encode_scales(&p.map_sb, w.scales, p.k.k_tiles, ceil_div(w.rows, 128), words, 2);
+    const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
+    launch(kPair + w.format, static_cast<unsigned>(2 * std::min<int64_t>(clusters(2), tiles)), 320, kGemmSmem, 2, &p, stream);
+}
+
 void Mx::product(const MxLinear& l, const MxMatrix& a, CUstream stream)
 {
     ContextGuard guard(ctx_);
+    if (ceil_div(a.rows, 256) * ceil_div(l.w.rows, 256) >= 1) {
+        pair(l, a, stream);
+        return;
+    }
     const MxMatrix& w = l.w;
     MxGemmParams p{};
     const size_t pitch = pitch_of(w.format, w.cols);

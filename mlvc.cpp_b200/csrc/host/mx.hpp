@@ -84,6 +84,7 @@ private:
     // product's kernel itself; false: there is no such kernel for these sizes.
     bool few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream);
     void product(const MxLinear& l, const MxMatrix& a, CUstream stream);
+    void pair(const MxLinear& l, const MxMatrix& a, CUstream stream);
     int clusters(int size);
     void launch(int index, unsigned grid, unsigned block, unsigned smem, unsigned cluster, void* params, CUstream stream);
     void require_device() const;

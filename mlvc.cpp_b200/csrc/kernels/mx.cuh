@@ -83,11 +83,9 @@ struct Raw {
 // The chunk from column `col`; columns from `cols` on read as 0.  `vec`: the
 // row is contiguous and begins on a 32-byte boundary.
 template <int DT>
-__device__ __forceinline__ void load_raw(const void* dense, long long row_at, long long col_stride, int col, int cols,
-                                         int vec, Raw<DT>& x)
+__device__ __forceinline__ void load_raw(const typename Dense<DT>::T* p, long long col_stride, int col, int cols, int vec,
+                                         Raw<DT>& x)
 {
-    using T = typename Dense<DT>::T;
-    const T* p = static_cast<const T*>(dense) + row_at;
     if (vec && col + 16 <= cols) {
 #pragma unroll
         for (int i = 0; i < Raw<DT>::kWords; i += 8)
@@ -123,8 +121,22 @@ __device__ __forceinline__ void unpack_raw(const Raw<DT>& x, float (&v)[16])
     }
 }
 
+// The larger of m and |x| in each half, NaN where either is.
+template <int DT>
+__device__ __forceinline__ uint32_t largest2(uint32_t m, uint32_t x)
+{
+    if constexpr (DT == kMxF16) {
+        const __half2 r = __hmax2_nan(*reinterpret_cast<__half2*>(&m), __habs2(*reinterpret_cast<__half2*>(&x)));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    } else {
+        const __nv_bfloat162 r =
+            __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&m), __habs2(*reinterpret_cast<__nv_bfloat162*>(&x)));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+}
+
 // Bits of the float that is the chunk's largest magnitude.  Magnitudes order
-// like their bits, infinity above the finite and NaN above infinity, so 16-bit
+// like their bits, infinity above the finite and NaN above infinity; 16-bit
 // values are compared two at a time as they lie.
 template <int DT>
 __device__ __forceinline__ uint32_t largest_raw(const Raw<DT>& x)
@@ -138,7 +150,7 @@ __device__ __forceinline__ uint32_t largest_raw(const Raw<DT>& x)
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            m = __vmaxu2(m, x.w[i] & 0x7FFF7FFFu);
+            m = largest2<DT>(m, x.w[i]);
         m = max(m & 0xFFFFu, m >> 16);
         float a, b;
         Dense<DT>::unpack(m, a, b);
@@ -147,11 +159,10 @@ __device__ __forceinline__ uint32_t largest_raw(const Raw<DT>& x)
 }
 
 template <int DT>
-__device__ __forceinline__ void store_chunk(void* dense, long long row_at, long long col_stride, int col, int cols,
-                                            int vec, const float (&v)[16])
+__device__ __forceinline__ void store_chunk(typename Dense<DT>::T* p, long long col_stride, int col, int cols, int vec,
+                                            const float (&v)[16])
 {
     using D = Dense<DT>;
-    typename D::T* p = static_cast<typename D::T*>(dense) + row_at;
     if (vec && col + 16 <= cols) {
         uint32_t w[8];
         if constexpr (DT == kMxF32) {
@@ -281,10 +292,14 @@ __device__ __forceinline__ void quantise_chunk(const Raw<DT>& x, float tensor_sc
         const float w4[4] = {want, 0.0f, 0.0f, 0.0f};
         scale = finite ? e4m3x4(w4) & 0xFFu : 0x7Fu;
         const float r = scale_value<F>(scale) * tensor_scale;
-        if (scale < 0x7Eu && r > 0x1p-100f && r < 0x1p100f) {
-            // |v / r| stays below 8 here, so nothing overflows, and what
-            // underflows is far below the smallest code's half
-            const float h = __frcp_rd(r);  // rounded down: l >= 0, and a zero keeps its sign
+        if (scale - 1u < 0x7Du) {
+            // neither zero, NaN nor the largest: |v / r| stays below 8, so
+            // nothing overflows (r lies in [2^-99, 2^99]), and what underflows
+            // is far below the smallest code's half.  h is below 1 / r by a few
+            // of its last places, so l >= 0 and a zero keeps its sign.
+            float h;
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(h) : "f"(r));
+            h = __uint_as_float(__float_as_uint(h) - 2u);
             const float l = fmaf(-r, h, 1.0f) * h;
             const uint64_t hh = pair(h, h), ll = pair(l, l);
 #pragma unroll
@@ -292,7 +307,7 @@ __device__ __forceinline__ void quantise_chunk(const Raw<DT>& x, float tensor_sc
                 const uint64_t vv = pair(v[i], v[i + 1]);
                 split(fma2(vv, hh, mul2(vv, ll)), v[i], v[i + 1]);
             }
-        } else if (r > 0.0f && finite) {
+        } else if (scale == 0x7Eu) {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 v[i] = __fdiv_rn(v[i], r);
@@ -424,6 +439,103 @@ __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t saddr)
 {
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(smem_desc(saddr, 16, 128, 0))
                  : "memory");
+}
+
+// ---- the same over a pair of CTAs (cta_group::2): one thread of the even CTA
+// issues for both; each CTA's shared memory and TMEM hold its half at the same
+// offsets.
+template <int F>
+__device__ __forceinline__ void umma_mx_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t id,
+                                             uint32_t tmem_sa, uint32_t tmem_sb, uint32_t accumulate)
+{
+    idesc |= (id << 4) | (id << 29);
+    if constexpr (F == kNvFp4)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+                tmem_d),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
+            : "memory");
+    else if constexpr (F == kMxFp4)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+                tmem_d),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+                tmem_d),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
+            : "memory");
+}
+
+__device__ __forceinline__ void tmem_copy_scales_pair(uint32_t taddr, uint32_t saddr)
+{
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(smem_desc(saddr, 16, 128, 0))
+                 : "memory");
+}
+
+// Arrives on `bar` in both CTAs when the MMAs issued so far are complete.
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar)
+{
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst_smem, uint32_t ncols)
+{
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)), "r"(ncols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols)
+{
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+
+// Address in the cluster of `p` as the CTA of that rank has it.
+__device__ __forceinline__ uint32_t cluster_address(const void* p, uint32_t rank)
+{
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    return a;
+}
+
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar)
+{
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// Tiled copies into this CTA's shared memory, completing on a barrier of either
+// CTA of the pair.
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+        "[%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
+        "[%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+__device__ __forceinline__ void cluster_barrier()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // Untiled copy into shared memory (16-byte multiples), completing on `bar`.

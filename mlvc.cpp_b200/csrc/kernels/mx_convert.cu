@@ -10,7 +10,7 @@
 
 namespace mlvc_b200 {
 
-constexpr int kMxThreads = 256;
+constexpr int kMxThreads = 128;
 
 // The places of a warp's packed rows in the cache: lane j * share + ... of the
 // result holds row t0 + j's (share = 32 / rows, at least 1), -1 where it has
@@ -51,10 +51,13 @@ __device__ __forceinline__ long long cache_slots(const MxConvertParams& p, long 
 }
 
 // A warp takes `steps` groups of 32 / lanes rows, `lanes` chunks wide; a lane's
-// chunk column is the same in all of them.
+// chunk column is the same in all of them.  The warp's rows are a power of two
+// at a multiple of it, at most 32, so they share a band of the scale tiles and
+// each group's scales lie 16 bytes a row further on.
 template <int DT, int F, bool kCache, bool kRead>
 __device__ __forceinline__ void mx_convert(const MxConvertParams& p)
 {
+    using T = typename Dense<DT>::T;
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
@@ -65,35 +68,49 @@ __device__ __forceinline__ void mx_convert(const MxConvertParams& p)
     const long long row0 = (static_cast<long long>(block) * (kMxThreads / 32) + warp) * warp_rows;
     if (row0 >= p.rows)
         return;
-    const long long row = row0 + (lane >> p.lane_bits);
+    const int in_group = lane >> p.lane_bits;
+    const long long row = row0 + in_group;
     const int column = Mx<F>::kIsNv ? chunk : chunk >> 1;
     constexpr int kSteps = DT == kMxF32 ? 2 : 4;
+    // rows of the lane that exist, none past the last column
+    const int left = chunk < p.chunks ? static_cast<int>(min(p.rows - row0, 32ll)) - in_group : 0;
+    const int count = min(p.steps, (left + (1 << group_bits) - 1) >> group_bits);
 
+    T* dense = static_cast<T*>(p.dense) + row * p.row_stride;
+    const long long dense_step = p.row_stride << group_bits;
     Raw<DT> x[kRead ? 1 : kSteps];
     if constexpr (!kRead) {
+        const T* from = dense;
 #pragma unroll
-        for (int u = 0; u < kSteps; ++u) {
-            const long long r = row + (u << group_bits);
-            if (u < p.steps && r < p.rows && chunk < p.chunks)
-                load_raw<DT>(p.dense, r * p.row_stride, p.col_stride, chunk * 16, p.cols, p.vec, x[u]);
+        for (int u = 0; u < kSteps; ++u, from += dense_step)
+            if (u < count)
+                load_raw<DT>(from, p.col_stride, chunk * 16, p.cols, p.vec, x[u]);
             else
                 x[u] = Raw<DT>{};
-        }
     }
-    long long held[kSteps];  // row of the quantised form, or -1
+    uint8_t* data[kSteps];   // the lane's chunk in the quantised form, null: none
+    uint8_t* scale_[kSteps];
     if constexpr (kCache) {
         // a row's lanes: 32 / warp_rows rounded down to a power of two
         const int share_bits = warp_rows >= 32 ? 0 : 31 - __clz(32 / warp_rows);
         const long long slot = cache_slots(p, row0, warp_rows, share_bits);
 #pragma unroll
         for (int u = 0; u < kSteps; ++u) {
-            const int j = (u << group_bits) + (lane >> p.lane_bits);
-            held[u] = __shfl_sync(0xFFFFFFFFu, slot, (j << share_bits) & 31);
+            const long long held = __shfl_sync(0xFFFFFFFFu, slot, (((u << group_bits) + in_group) << share_bits) & 31);
+            const bool there = u < count && held >= 0;
+            data[u] = there ? p.data + held * p.pitch + chunk * Mx<F>::kChunkBytes : nullptr;
+            scale_[u] = p.scales + held * p.scale_pitch + column;
         }
     } else {
+        uint8_t* to = p.data + row * p.pitch + chunk * Mx<F>::kChunkBytes;
+        uint8_t* at = p.scales + scale_at(row, column, p.k_tiles);
 #pragma unroll
-        for (int u = 0; u < kSteps; ++u)
-            held[u] = row + (u << group_bits);
+        for (int u = 0; u < kSteps; ++u) {
+            data[u] = u < count ? to : nullptr;
+            scale_[u] = at;
+            to += p.pitch << group_bits;
+            at += 16 << group_bits;
+        }
     }
     uint32_t codes[kSteps][4], scale[kSteps];
     if constexpr (kRead) {
@@ -101,43 +118,40 @@ __device__ __forceinline__ void mx_convert(const MxConvertParams& p)
         for (int u = 0; u < kSteps; ++u) {
             scale[u] = 0;
             codes[u][0] = codes[u][1] = codes[u][2] = codes[u][3] = 0;
-            if (u < p.steps && row + (u << group_bits) < p.rows && chunk < p.chunks && (!kCache || held[u] >= 0)) {
-                const uint8_t* data = p.data + held[u] * p.pitch + chunk * Mx<F>::kChunkBytes;
+            if (data[u]) {
                 if constexpr (Mx<F>::kIs8)
-                    *reinterpret_cast<uint4*>(codes[u]) = *reinterpret_cast<const uint4*>(data);
+                    *reinterpret_cast<uint4*>(codes[u]) = *reinterpret_cast<const uint4*>(data[u]);
                 else
-                    *reinterpret_cast<uint2*>(codes[u]) = *reinterpret_cast<const uint2*>(data);
-                scale[u] = p.scales[kCache ? held[u] * p.scale_pitch + column : scale_at(held[u], column, p.k_tiles)];
+                    *reinterpret_cast<uint2*>(codes[u]) = *reinterpret_cast<const uint2*>(data[u]);
+                scale[u] = *scale_[u];
             }
         }
-    }
 #pragma unroll
-    for (int u = 0; u < kSteps; ++u) {
-        if (u >= p.steps)
-            break;
-        const long long r = row + (u << group_bits);
-        const bool valid = r < p.rows && chunk < p.chunks;
-        if constexpr (kRead) {
-            float v[16];
-            read_chunk<F>(codes[u], scale[u], p.tensor_scale, v);
-            if (valid)
-                store_chunk<DT>(p.dense, r * p.row_stride, p.col_stride, chunk * 16, p.cols, p.vec, v);
-        } else {
+        for (int u = 0; u < kSteps; ++u, dense += dense_step)
+            if (u < count) {
+                float v[16];
+                read_chunk<F>(codes[u], scale[u], p.tensor_scale, v);
+                store_chunk<DT>(dense, p.col_stride, chunk * 16, p.cols, p.vec, v);
+            }
+    } else {
+        // the product reads whole words: the rest of the last scale tile is zero
+        const bool pads = !kCache && chunk == p.chunks - 1 && (column & 3) != 3;
+#pragma unroll
+        for (int u = 0; u < kSteps; ++u) {
+            if (u >= p.steps)
+                break;
             quantise_chunk<F, DT>(x[u], p.tensor_scale, p.inv_six_scale, codes[u], scale[u]);
-            if (!valid || (kCache && held[u] < 0))
+            if (!data[u])
                 continue;
-            uint8_t* data = p.data + held[u] * p.pitch + chunk * Mx<F>::kChunkBytes;
             if constexpr (Mx<F>::kIs8)
-                *reinterpret_cast<uint4*>(data) = *reinterpret_cast<const uint4*>(codes[u]);
+                *reinterpret_cast<uint4*>(data[u]) = *reinterpret_cast<const uint4*>(codes[u]);
             else
-                *reinterpret_cast<uint2*>(data) = *reinterpret_cast<const uint2*>(codes[u]);
+                *reinterpret_cast<uint2*>(data[u]) = *reinterpret_cast<const uint2*>(codes[u]);
             if (Mx<F>::kIsNv || !(chunk & 1))
-                p.scales[kCache ? held[u] * p.scale_pitch + column : scale_at(held[u], column, p.k_tiles)] =
-                    static_cast<uint8_t>(scale[u]);
-            // the rest of the last scale tile: the product reads whole words
-            if (!kCache && chunk == p.chunks - 1)
-                for (int k = column + 1; k < 4 * p.k_tiles; ++k)
-                    p.scales[scale_at(held[u], k, p.k_tiles)] = 0;
+                *scale_[u] = static_cast<uint8_t>(scale[u]);
+            if (pads)
+                for (int k = 1; (column & 3) + k < 4; ++k)
+                    scale_[u][k] = 0;
         }
     }
 }
@@ -147,12 +161,12 @@ __device__ __forceinline__ void mx_convert(const MxConvertParams& p)
     {                                                                                        \
         mx_convert<DT, F, CACHE, READ>(p);                                                   \
     }
-// Quantising is bound by 64 registers a thread, four CTAs an SM; reading back
+// Quantising is bound by 64 registers a thread, eight CTAs an SM; reading back
 // needs fewer of itself, and is slower when the compiler is told so.
 #define MLVC_MX_CONVERT_ALL(T, DT, FN, F)                                                     \
-    MLVC_MX_CONVERT(mlvc_mx_quantise_##T##_##FN, (kMxThreads, 4), DT, F, false, false)        \
+    MLVC_MX_CONVERT(mlvc_mx_quantise_##T##_##FN, (kMxThreads, 8), DT, F, false, false)        \
     MLVC_MX_CONVERT(mlvc_mx_dequantise_##T##_##FN, (kMxThreads), DT, F, false, true)          \
-    MLVC_MX_CONVERT(mlvc_mx_cache_write_##T##_##FN, (kMxThreads, 4), DT, F, true, false)      \
+    MLVC_MX_CONVERT(mlvc_mx_cache_write_##T##_##FN, (kMxThreads, 8), DT, F, true, false)      \
     MLVC_MX_CONVERT(mlvc_mx_cache_read_##T##_##FN, (kMxThreads), DT, F, true, true)
 
 MLVC_MX_CONVERT_ALL(f16, kMxF16, mxfp4, kMxFp4)

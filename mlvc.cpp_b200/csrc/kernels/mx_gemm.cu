@@ -98,11 +98,11 @@ struct MxTile {
 };
 
 // Tiles in bands of 8 row tiles, so that the tiles in flight share operands.
-__device__ __forceinline__ void mx_tile_at(const MxGemmParams& p, int t, int& m, int& n)
+__device__ __forceinline__ void mx_tile_at(int m_tiles, int n_tiles, int t, int& m, int& n)
 {
-    const int band = 8 * p.n_tiles;
+    const int band = 8 * n_tiles;
     const int g = t / band, r = t - g * band;
-    const int high = min(8, p.m_tiles - 8 * g);
+    const int high = min(8, m_tiles - 8 * g);
     n = r / high;
     m = 8 * g + r - n * high;
 }
@@ -152,7 +152,7 @@ __device__ __forceinline__ void mx_gemm(const MxGemmParams& p)
             uint32_t phase = 0;
             for (int t = blockIdx.x; t < total && !sh->abort_flag; t += gridDim.x) {
                 int mt, nt;
-                mx_tile_at(p, t, mt, nt);
+                mx_tile_at(p.m_tiles, p.n_tiles, t, mt, nt);
                 for (int k = 0; k < p.k.count; ++k) {
                     if (!mbar_wait(&sh->empty[stage], phase ^ 1u, &sh->abort_flag, kErrMxProducer))
                         break;
@@ -202,7 +202,7 @@ __device__ __forceinline__ void mx_gemm(const MxGemmParams& p)
                 // rows of B inside its 128-row band of scales (BN = 64: the second half)
                 const uint32_t d = tmem + acc * BN;
                 int mt, nt;
-                mx_tile_at(p, t, mt, nt);
+                mx_tile_at(p.m_tiles, p.n_tiles, t, mt, nt);
                 const uint32_t in_band = BN < 128 ? (nt * BN % 128) / 32 : 0;
                 for (int k = 0; k < p.k.count; ++k) {
                     if (!mbar_wait(&sh->full[stage], phase, &sh->abort_flag, kErrMxMma)) {
@@ -247,7 +247,7 @@ __device__ __forceinline__ void mx_gemm(const MxGemmParams& p)
         uint32_t acc = 0, acc_phase = 0;
         for (int t = blockIdx.x; t < total; t += gridDim.x) {
             int mt, nt;
-            mx_tile_at(p, t, mt, nt);
+            mx_tile_at(p.m_tiles, p.n_tiles, t, mt, nt);
             // the whole warp goes on or none of it: the TMEM loads are collective
             if (!__all_sync(0xFFFFFFFFu, mbar_wait(&sh->tmem_full[acc], acc_phase, &sh->abort_flag, kErrMxEpilogue)))
                 break;

@@ -7,4 +7,5 @@ extern "C" __device__ unsigned long long mlvc_b200_wait_limit_ns = mlvc_b200::kW
 
 #include "mx_convert.cu"
 #include "mx_gemm.cu"
+#include "mx_pair.cu"
 #include "mx_rows.cu"

@@ -1,0 +1,231 @@
+// Large products of microscaled matrices: 256 x 256 tiles by pairs of CTAs.
+//
+// The tensor core takes 4-bit operands faster than one SM can bring them in: a
+// 128 x 128 tile needs 2 bytes of operands for every 128 products, a pair's
+// 256 x 256 tile half of that, because each CTA loads 128 rows of A and 128
+// rows of B and the pair's MMA reads both halves of both.  Each CTA keeps its
+// 128 rows of the sums in its own TMEM (256 columns).
+//
+// Two accumulators of 256 columns and the scales (up to 48 columns) exceed the
+// 512 columns, so the second accumulator begins at column 192, inside the
+// first: whoever empties an accumulator empties the shared 64 columns first,
+// and the next tile's MMAs start as soon as those are out.
+//
+// Warps: 0 copies (both CTAs, completing on the even CTA's barriers), 1 MMA
+// (even CTA), 2..9 empty the accumulators.
+#include "mx.cuh"
+
+namespace mlvc_b200 {
+
+constexpr int kMxPairThreads = 320;
+constexpr int kMxPairMaxStages = 6;
+
+struct MxPairShared {
+    uint64_t full[kMxPairMaxStages];   // even CTA: both CTAs' copies of a stage
+    uint64_t empty[kMxPairMaxStages];  // each CTA: the stage's MMAs are complete
+    uint64_t sums;                     // each CTA: an accumulator is complete
+    uint64_t shared_out;               // even CTA: all 16 warps have emptied the shared columns
+    uint64_t drain;
+    uint32_t tmem_base;
+    int abort_flag;
+};
+
+template <int F>
+struct MxPairTile {
+    static constexpr uint32_t kOperand = 128 * 128;          // 128 rows of a panel
+    static constexpr uint32_t kSA = Mx<F>::kWords * 512, kSB = 2 * kSA;
+    static constexpr uint32_t kStage = (2 * kOperand + kSA + kSB + 1023) / 1024 * 1024;
+    static constexpr int kStages =
+        (227 * 1024 - 2048) / kStage < kMxPairMaxStages ? (227 * 1024 - 2048) / kStage : kMxPairMaxStages;
+    static constexpr uint32_t kTx = 2 * (2 * kOperand + kSA + kSB);
+};
+
+template <int F>
+__device__ __forceinline__ void mx_pair(const MxPairParams& p)
+{
+    using T = MxPairTile<F>;
+    constexpr int kWords = Mx<F>::kWords;
+    extern __shared__ __align__(1024) uint8_t smem_dyn[];
+    uint8_t* base = align_smem_1024(smem_dyn);
+    MxPairShared* sh = reinterpret_cast<MxPairShared*>(base);
+    static_assert(sizeof(MxPairShared) <= 1024, "header");
+    uint8_t* stages = base + 1024;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t rank = blockIdx.x & 1u;
+    const int pair_id = blockIdx.x / 2, pairs = gridDim.x / 2;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < T::kStages; ++s) {
+            mbar_init(&sh->full[s], 1);
+            mbar_init(&sh->empty[s], 1);
+        }
+        mbar_init(&sh->sums, 1);
+        mbar_init(&sh->shared_out, 16);
+        mbar_init(&sh->drain, 1);
+        sh->abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 0 && elect_one()) {
+        tma_prefetch_desc(&p.map_a);
+        tma_prefetch_desc(&p.map_b);
+        tma_prefetch_desc(&p.map_sa);
+        tma_prefetch_desc(&p.map_sb);
+    }
+    // TMEM is taken once the kernel before has ended (see mx_gemm)
+    pdl_wait();
+    if (warp == 1)
+        tmem_alloc_pair(&sh->tmem_base, 512);
+    tc_fence_before();
+    __syncthreads();
+    cluster_barrier();  // the other CTA's barriers exist, its TMEM is there
+    tc_fence_after();
+    pdl_launch_dependents();
+    const uint32_t tmem = sh->tmem_base;
+    const int total = p.m_tiles * p.n_tiles;
+    bool issuer = false;
+    uint32_t issued = 0;
+
+    if (warp == 0) {
+        if (elect_one()) {
+            uint32_t armed = 0, parity = 0;
+            int stage = 0;
+            uint32_t phase = 0;
+            for (int t = pair_id; t < total && !sh->abort_flag; t += pairs) {
+                int mt, nt;
+                mx_tile_at(p.m_tiles, p.n_tiles, t, mt, nt);
+                for (int k = 0; k < p.k.count; ++k) {
+                    if (!mbar_wait(&sh->empty[stage], phase ^ 1u, &sh->abort_flag, kErrMxProducer))
+                        break;
+                    uint8_t* s = stages + stage * T::kStage;
+                    const uint32_t bar = cluster_address(&sh->full[stage], 0);
+                    // every box counts in full, rows and tiles outside are zeros
+                    if (rank == 0) {
+                        mbar_arrive_expect_tx(&sh->full[stage], T::kTx);
+                        armed |= 1u << stage;
+                        parity = (parity & ~(1u << stage)) | (phase << stage);
+                    }
+                    tma_load_2d_pair(s, &p.map_a, bar, k * 128, mt * 256 + rank * 128);
+                    tma_load_2d_pair(s + T::kOperand, &p.map_b, bar, k * 128, nt * 256 + rank * 128);
+                    tma_load_3d_pair(s + 2 * T::kOperand, &p.map_sa, bar, 0, k * kWords, mt * 2 + rank);
+                    tma_load_3d_pair(s + 2 * T::kOperand + T::kSA, &p.map_sb, bar, 0, k * kWords, nt * 2);
+                    if (++stage == T::kStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            if (sh->abort_flag) {  // no copy may land after these CTAs have gone
+                volatile int never = 0;
+                for (int s = 0; s < T::kStages; ++s)
+                    if ((armed >> s) & 1u)
+                        mbar_wait(&sh->full[s], (parity >> s) & 1u, &never, kErrMxProducer);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (rank == 0 && elect_one()) {
+            issuer = true;
+            constexpr uint32_t idesc = mx_idesc<F>(256, 256);
+            const uint32_t tmem_sa = tmem + 448, tmem_sb = tmem_sa + 4 * kWords;
+            int stage = 0;
+            uint32_t phase = 0, tile = 0;
+            bool ok = true;
+            for (int t = pair_id; ok && t < total; t += pairs, ++tile) {
+                // the tile before has left the columns that this one shares with it
+                if (tile && !mbar_wait(&sh->shared_out, (tile - 1) & 1u, &sh->abort_flag, kErrMxMma))
+                    break;
+                tc_fence_after();
+                const uint32_t d = tmem + (tile & 1u) * 192;
+                for (int k = 0; k < p.k.count; ++k) {
+                    if (!mbar_wait(&sh->full[stage], phase, &sh->abort_flag, kErrMxMma)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t s = smem_u32(stages + stage * T::kStage), sa = s + 2 * T::kOperand, sb = sa + T::kSA;
+                    const bool last = k + 1 == p.k.count;
+                    const int words = last ? p.k.last_words : kWords, steps = last ? p.k.last_steps : 4;
+#pragma unroll
+                    for (int w = 0; w < kWords; ++w) {
+                        if (w >= words)
+                            break;
+                        tmem_copy_scales_pair(tmem_sa + 4 * w, sa + 512 * w);
+                        tmem_copy_scales_pair(tmem_sb + 8 * w, sb + 512 * w);
+                        tmem_copy_scales_pair(tmem_sb + 8 * w + 4, sb + T::kSA + 512 * w);
+                    }
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks) {
+                        if (ks >= steps)
+                            break;
+                        const uint32_t w = ks * kWords / 4, id = kWords == 4 ? 0 : kWords == 2 ? (ks & 1) * 2 : ks;
+                        umma_mx_pair<F>(d, smem_desc(s + ks * 32, 16, 1024, 2),
+                                        smem_desc(s + T::kOperand + ks * 32, 16, 1024, 2), idesc, id, tmem_sa + 4 * w,
+                                        tmem_sb + 8 * w, (k | ks) != 0);
+                        ++issued;
+                    }
+                    umma_commit_pair(&sh->empty[stage]);
+                    if (++stage == T::kStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok)
+                    break;
+                umma_commit_pair(&sh->sums);
+            }
+        }
+        __syncwarp();
+    } else {
+        const int quadrant = warp & 3, group = (warp - 2) / 4;
+        const uint32_t out = cluster_address(&sh->shared_out, 0);
+        uint32_t tile = 0;
+        for (int t = pair_id; t < total; t += pairs, ++tile) {
+            int mt, nt;
+            mx_tile_at(p.m_tiles, p.n_tiles, t, mt, nt);
+            // the whole warp goes on or none of it: the TMEM loads are collective
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait(&sh->sums, tile & 1u, &sh->abort_flag, kErrMxEpilogue)))
+                break;
+            tc_fence_after();
+            const long long row = static_cast<long long>(mt) * 256 + rank * 128 + quadrant * 32 + lane;
+            const int odd = tile & 1u;
+            for (int c = 0; c < 4; ++c) {
+                // the shared columns 192..255 first
+                const int at = c == 0 ? 192 + 32 * group : (odd ? 256 : 0) + 96 * group + 32 * (c - 1);
+                uint32_t v[32];
+                tmem_ld32_nowait(tmem + at + (static_cast<uint32_t>(quadrant * 32) << 16), v);
+                tmem_wait_ld();
+                if (c == 0) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0)
+                        mbar_arrive_cluster(out);
+                }
+                mx_finish(p.e, row, nt * 256 + at - (odd ? 192 : 0), v);
+                __syncwarp();
+            }
+        }
+        __syncwarp();
+    }
+    if (issuer && sh->abort_flag && issued) {  // MMAs in flight end before TMEM is freed
+        umma_commit_pair(&sh->drain);
+        volatile int never = 0;
+        mbar_wait(&sh->drain, 0, &never, kErrMxMma);
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_barrier();  // neither CTA leaves while the other's MMAs, copies or arrivals may reach it
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem, 512);
+    }
+}
+
+#define MLVC_MX_PAIR(NAME, F)                                                                                  \
+    extern "C" __global__ void __launch_bounds__(kMxPairThreads, 1) NAME(const __grid_constant__ MxPairParams p) \
+    {                                                                                                          \
+        mx_pair<F>(p);                                                                                         \
+    }
+MLVC_MX_PAIR(mlvc_mx_pair_mxfp4, kMxFp4)
+MLVC_MX_PAIR(mlvc_mx_pair_nvfp4, kNvFp4)
+MLVC_MX_PAIR(mlvc_mx_pair_mxfp8, kMxFp8)
+
+}  // namespace mlvc_b200

@@ -76,6 +76,17 @@ struct MxGemmParams {
     MxEpilogue e;
 };
 
+// Products in 256 x 256 tiles by pairs of CTAs (see mx_pair).
+struct MxPairParams {
+    CUtensorMap map_a, map_b;          // bytes [rows, pitch], boxes of 128 bytes x 128 rows, 128-byte swizzle
+    // scale tiles as 16-bit values [bands, tiles of a band, 256]; boxes of a
+    // panel's tiles, one band of A and two of B
+    CUtensorMap map_sa, map_sb;
+    MxPanels k;
+    int m_tiles, n_tiles;
+    MxEpilogue e;
+};
+
 // Products of at most 128 rows (see mx_rows): weights are the tensor core's
 // first operand, rows its second.
 constexpr int kMxRowsMax = 128;

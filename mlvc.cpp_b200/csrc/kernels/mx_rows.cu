@@ -35,11 +35,6 @@ struct MxRowsShared {
 };
 static_assert(sizeof(MxRowsShared) <= kMxRowsHeader, "header");
 
-__device__ __forceinline__ void cluster_barrier()
-{
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
 __device__ __forceinline__ float4 load_cluster(uint32_t saddr, uint32_t rank)
 {
     float4 v;
@@ -225,8 +220,8 @@ __device__ __forceinline__ void mx_rows(const MxRowsParams& p)
                     for (int b = 0; b < kBatch; ++b) {
                         const int i = i0 + 256 * b, m = i / row_chunks, c = i - m * row_chunks;
                         if (i < items)
-                            load_raw<DT>(p.x, m * p.row_stride, p.col_stride, ((k0 + first) * kChunks + c) * 16, p.cols, p.vec,
-                                         x[b]);
+                            load_raw<DT>(static_cast<const typename Dense<DT>::T*>(p.x) + m * p.row_stride, p.col_stride,
+                                         ((k0 + first) * kChunks + c) * 16, p.cols, p.vec, x[b]);
                         else
                             x[b] = Raw<DT>{};
                     }
