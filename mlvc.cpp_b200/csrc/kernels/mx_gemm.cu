@@ -2,77 +2,13 @@
 //     y[m, n] = leaky(alpha * sum_k a[m, k] b[n, k] + bias[n]) + residual[m, n]
 // with a and b quantised along k, alpha the product of their tensor scales,
 // sums in 32 bits in tensor memory and one rounding to y's type.
-#include "mx.cuh"
+#include "mx_epilogue.cuh"
 
 namespace mlvc_b200 {
 
 constexpr unsigned int kErrMxProducer = 0x1u;
 constexpr unsigned int kErrMxMma = 0x2u;
 constexpr unsigned int kErrMxEpilogue = 0x4u;
-
-// 32 results of one row from column `col`.
-template <int DT>
-__device__ __forceinline__ void mx_store_row(const MxEpilogue& p, long long row, int col, float (&v)[32])
-{
-    using D = Dense<DT>;
-    using T = typename D::T;
-    T* y = static_cast<T*>(p.y) + row * p.y_stride + col;
-    const T* res = p.residual ? static_cast<const T*>(p.residual) + row * p.residual_stride + col : nullptr;
-    if (p.vec && col + 32 <= p.N) {
-        constexpr int kPer = 16 / sizeof(T);  // values of a 16-byte access
-#pragma unroll
-        for (int i = 0; i < 32; i += kPer) {
-            if (res) {
-                const uint4 w = *reinterpret_cast<const uint4*>(res + i);
-                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if constexpr (DT == kMxF32) {
-                        v[i + k] += __uint_as_float(u[k]);
-                    } else {
-                        float a, b;
-                        D::unpack(u[k], a, b);
-                        v[i + 2 * k] += a;
-                        v[i + 2 * k + 1] += b;
-                    }
-                }
-            }
-            uint32_t o[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if constexpr (DT == kMxF32)
-                    o[k] = __float_as_uint(v[i + k]);
-                else
-                    o[k] = D::pack2(v[i + 2 * k], v[i + 2 * k + 1]);
-            }
-            *reinterpret_cast<uint4*>(y + i) = make_uint4(o[0], o[1], o[2], o[3]);
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-        if (col + i < p.N)
-            y[i] = D::pack(res ? v[i] + D::load(res + i) : v[i]);
-}
-
-__device__ __forceinline__ void mx_finish(const MxEpilogue& p, long long row, int col, const uint32_t (&acc)[32])
-{
-    if (row >= p.M || col >= p.N)
-        return;
-    float v[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        const float b = p.bias && col + i < p.N ? p.bias[col + i] : 0.0f;
-        const float t = fmaf(__uint_as_float(acc[i]), p.alpha, b);
-        v[i] = t >= 0.0f ? t : t * p.slope;
-    }
-    if (p.y_dtype == kMxF16)
-        mx_store_row<kMxF16>(p, row, col, v);
-    else if (p.y_dtype == kMxBf16)
-        mx_store_row<kMxBf16>(p, row, col, v);
-    else
-        mx_store_row<kMxF32>(p, row, col, v);
-}
 
 constexpr int kMxGemmThreads = 320;  // warp 0 copies, warp 1 MMA, warps 2..9 epilogue
 constexpr int kMxMaxStages = 8;
@@ -94,7 +30,7 @@ struct MxTile {
     static constexpr uint32_t kA = 128 * 128, kB = BN * 128;
     static constexpr uint32_t kSA = Mx<F>::kWords * 512, kSB = kBands * kSA;
     static constexpr uint32_t kStage = (kA + kB + kSA + kSB + 1023) / 1024 * 1024;
-    static constexpr int kStages = (227 * 1024 - 2048) / kStage < kMxMaxStages ? (227 * 1024 - 2048) / kStage : kMxMaxStages;
+    static constexpr int kStages = (227 * 1024 - 2048 - 8 * kMxTurnBytes) / kStage < kMxMaxStages ? (227 * 1024 - 2048 - 8 * kMxTurnBytes) / kStage : kMxMaxStages;
 };
 
 // Tiles in bands of 8 row tiles, so that the tiles in flight share operands.
@@ -117,7 +53,7 @@ __device__ __forceinline__ void mx_gemm(const MxGemmParams& p)
     MxShared* sh = reinterpret_cast<MxShared*>(base);
     uint8_t* stages = base + 1024;
     static_assert(sizeof(MxShared) <= 1024, "header");
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = threadIdx.x / 32;
     if (threadIdx.x == 0) {
         for (int s = 0; s < T::kStages; ++s) {
             mbar_init(&sh->full[s], 1);
@@ -244,6 +180,7 @@ __device__ __forceinline__ void mx_gemm(const MxGemmParams& p)
         __syncwarp();
     } else {
         const int quadrant = warp & 3, group = (warp - 2) / 4;
+        float4* turn = reinterpret_cast<float4*>(stages + T::kStages * T::kStage + (warp - 2) * kMxTurnBytes);
         uint32_t acc = 0, acc_phase = 0;
         for (int t = blockIdx.x; t < total; t += gridDim.x) {
             int mt, nt;
@@ -253,11 +190,8 @@ __device__ __forceinline__ void mx_gemm(const MxGemmParams& p)
                 break;
             tc_fence_after();
             for (int c = group * 32; c < BN; c += 64) {
-                uint32_t v[32];
-                tmem_ld32_nowait(tmem + acc * BN + c + (static_cast<uint32_t>(quadrant * 32) << 16), v);
-                tmem_wait_ld();
-                mx_finish(p.e, static_cast<long long>(mt) * 128 + quadrant * 32 + lane, nt * BN + c, v);
-                __syncwarp();
+                mx_empty(p.e, turn, tmem + acc * BN + c + (static_cast<uint32_t>(quadrant * 32) << 16),
+                         static_cast<long long>(mt) * 128 + quadrant * 32, nt * BN + c, [] {});
             }
             tc_fence_before();
             mbar_arrive(&sh->tmem_empty[acc]);

@@ -13,7 +13,7 @@
 //
 // Warps: 0 copies (both CTAs, completing on the even CTA's barriers), 1 MMA
 // (even CTA), 2..9 empty the accumulators.
-#include "mx.cuh"
+#include "mx_epilogue.cuh"
 
 namespace mlvc_b200 {
 
@@ -36,7 +36,7 @@ struct MxPairTile {
     static constexpr uint32_t kSA = Mx<F>::kWords * 512, kSB = 2 * kSA;
     static constexpr uint32_t kStage = (2 * kOperand + kSA + kSB + 1023) / 1024 * 1024;
     static constexpr int kStages =
-        (227 * 1024 - 2048) / kStage < kMxPairMaxStages ? (227 * 1024 - 2048) / kStage : kMxPairMaxStages;
+        (227 * 1024 - 2048 - 8 * kMxTurnBytes) / kStage < kMxPairMaxStages ? (227 * 1024 - 2048 - 8 * kMxTurnBytes) / kStage : kMxPairMaxStages;
     static constexpr uint32_t kTx = 2 * (2 * kOperand + kSA + kSB);
 };
 
@@ -177,6 +177,7 @@ __device__ __forceinline__ void mx_pair(const MxPairParams& p)
     } else {
         const int quadrant = warp & 3, group = (warp - 2) / 4;
         const uint32_t out = cluster_address(&sh->shared_out, 0);
+        float4* turn = reinterpret_cast<float4*>(stages + T::kStages * T::kStage + (warp - 2) * kMxTurnBytes);
         uint32_t tile = 0;
         for (int t = pair_id; t < total; t += pairs, ++tile) {
             int mt, nt;
@@ -185,22 +186,20 @@ __device__ __forceinline__ void mx_pair(const MxPairParams& p)
             if (!__all_sync(0xFFFFFFFFu, mbar_wait(&sh->sums, tile & 1u, &sh->abort_flag, kErrMxEpilogue)))
                 break;
             tc_fence_after();
-            const long long row = static_cast<long long>(mt) * 256 + rank * 128 + quadrant * 32 + lane;
+            const long long row = static_cast<long long>(mt) * 256 + rank * 128 + quadrant * 32;
             const int odd = tile & 1u;
             for (int c = 0; c < 4; ++c) {
                 // the shared columns 192..255 first
                 const int at = c == 0 ? 192 + 32 * group : (odd ? 256 : 0) + 96 * group + 32 * (c - 1);
-                uint32_t v[32];
-                tmem_ld32_nowait(tmem + at + (static_cast<uint32_t>(quadrant * 32) << 16), v);
-                tmem_wait_ld();
-                if (c == 0) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0)
-                        mbar_arrive_cluster(out);
-                }
-                mx_finish(p.e, row, nt * 256 + at - (odd ? 192 : 0), v);
-                __syncwarp();
+                mx_empty(p.e, turn, tmem + at + (static_cast<uint32_t>(quadrant * 32) << 16), row, nt * 256 + at - (odd ? 192 : 0),
+                         [&] {
+                             if (c == 0) {
+                                 tc_fence_before();
+                                 __syncwarp();
+                                 if (lane == 0)
+                                     mbar_arrive_cluster(out);
+                             }
+                         });
             }
         }
         __syncwarp();
