@@ -211,21 +211,21 @@ void Mx::launch(int index, unsigned grid, unsigned block, unsigned smem, unsigne
     check(cuLaunchKernelEx(&cfg, fn(index), args, nullptr), "cuLaunchKernelEx(mx)");
 }
 
-// Clusters of this many one-CTA-an-SM blocks that run at once.
-int Mx::clusters(int size)
+// Clusters of this many blocks that run at once, one or two blocks an SM.
+int Mx::clusters(int size, bool half_sm)
 {
-    int& known = clusters_[size];
+    int& known = clusters_[half_sm][size];
     if (!known) {
         CUlaunchAttribute attr{};
         attr.id = CU_LAUNCH_ATTRIBUTE_CLUSTER_DIMENSION;
         attr.value.clusterDim.x = size;
         attr.value.clusterDim.y = attr.value.clusterDim.z = 1;
         CUlaunchConfig cfg{};
-        cfg.gridDimX = size;
+        cfg.gridDimX = size * 1024;  // more than fit
         cfg.gridDimY = cfg.gridDimZ = 1;
         cfg.blockDimX = 320;
         cfg.blockDimY = cfg.blockDimZ = 1;
-        cfg.sharedMemBytes = kGemmSmem;
+        cfg.sharedMemBytes = half_sm ? 113 * 1024 : kGemmSmem;
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
         int n = 0;
@@ -485,28 +485,43 @@ bool Mx::few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream)
     MxRowsParams p{};
     p.k = panels_of(w.format, w.cols);
     const int64_t n_tiles = ceil_div(w.rows, 128);
-    // as many CTAs on k as there are SMs for at once: clusters take SMs of one
-    // group, so fewer of them fit than SMs divided by their size
-    p.splits = static_cast<int>(std::min<int64_t>(8, p.k.count));
-    while (p.splits > 1 && n_tiles > clusters(p.splits))
-        --p.splits;
-    const int64_t grid = n_tiles * p.splits;
     p.row_tile = static_cast<int>(ceil_div(rows, 8) * 8);
-    const size_t x_bytes = static_cast<size_t>(p.row_tile) * 128, most = ceil_div(p.k.count, p.splits);
-    const size_t scale_bytes = static_cast<size_t>(w.format == kNvFp4 ? 4 : w.format == kMxFp4 ? 2 : 1) * 512;
+    const size_t x_bytes = static_cast<size_t>(p.row_tile) * 128;
+    const int words = w.format == kNvFp4 ? 4 : w.format == kMxFp4 ? 2 : 1;
+    const size_t scale_bytes = static_cast<size_t>(words) * 512;
     const size_t stage = ceil_div(128 * 128 + scale_bytes + (a ? x_bytes + scale_bytes : 0), 1024) * 1024;
-    const size_t fixed = 2048 + (a ? 0 : most * x_bytes + ceil_div(most * scale_bytes, 1024) * 1024);
-    // two CTAs an SM where there are more than SMs, if that leaves a ring of four
+    int64_t most = 0;
+    auto fixed = [&](int splits) {
+        most = ceil_div(p.k.count, splits);
+        return 2048 + (splits > 1 ? ceil_div(splits * ceil_div(rows, splits) * 512, 1024) * 1024 : 0) +
+               (a ? 0 : most * x_bytes + ceil_div(most * scale_bytes, 1024) * 1024);
+    };
+    // as many CTAs on k as there is room for at once, each with two panels or
+    // more; two CTAs an SM (the waits of one are filled by the other) where that
+    // leaves a ring of four and no fewer CTAs; clusters take SMs of one group, so
+    // fewer of them fit than SMs divided by their size
     const size_t whole = kGemmSmem, half = 113 * 1024;
-    const size_t room = grid > sm_count_ && fixed + 4 * stage <= half ? half : whole;
-    if (fixed + std::min<size_t>(most, 3) * stage > room)
+    size_t room = 0;
+    const int widest = static_cast<int>(std::clamp<int64_t>(p.k.count / 2, 1, 8));
+    for (const bool half_sm : {true, false})
+        for (int splits = widest; splits >= 1; --splits)
+            if (splits > (room ? p.splits : 0) &&
+                fixed(splits) + std::min<size_t>(most, half_sm ? 4 : 3) * stage <= (half_sm ? half : whole) &&
+                (splits == 1 || n_tiles <= clusters(splits, half_sm))) {
+                room = half_sm ? half : whole;
+                p.splits = splits;
+                break;
+            }
+    if (!room)
         return false;
-    p.stages = static_cast<int>(std::min({most, (room - fixed) / stage, size_t{12}}));
-    size_t smem = fixed + p.stages * stage;
-    if (p.splits > 1)
-        smem = std::max(smem, fixed + static_cast<size_t>(p.row_tile) * 512);
+    const size_t used = fixed(p.splits);
+    p.stages = static_cast<int>(std::min<size_t>({static_cast<size_t>(most), (room - used) / stage, 12}));
+    // the ring holds the sums in the end
+    const size_t smem = used + std::max(p.stages * stage, static_cast<size_t>(rows) * 512);
     if (smem > whole)
         return false;
+    p.batch = std::max(1, std::min(4, p.stages >= most ? static_cast<int>(most) : p.stages / 2));
+    const int64_t grid = n_tiles * p.splits;
     const size_t pitch = pitch_of(w.format, w.cols);
     encode_rows(&p.map_w, w.data, pitch, w.rows, 128);
     p.scales_w = reinterpret_cast<const uint8_t*>(w.scales);
@@ -523,7 +538,7 @@ bool Mx::few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream)
         p.tensor_scale = x_scale;
         p.inv_six_scale = inverse_six(x_scale);
         const int64_t panel_chunks = rows * (w.format == kMxFp8 ? 8 : 16);
-        p.group = static_cast<int>(std::max({int64_t{1}, 1024 / panel_chunks, ceil_div(most, 32)}));
+        p.group = static_cast<int>(std::max({int64_t{1}, 512 / panel_chunks, ceil_div(most, 32)}));
     }
     p.e = epilogue_of(l, rows, x_scale);
     const int type = a ? 0 : l.x.dtype == kMxF16 ? 1 : l.x.dtype == kMxBf16 ? 2 : 3;
@@ -547,13 +562,13 @@ void Mx::pair(const MxLinear& l, const MxMatrix& a, CUstream stream)
     encode_scales(&p.map_sa, a.scales, p.k.k_tiles, ceil_div(a.rows, 128), words, 1);
     encode_scales(&p.map_sb, w.scales, p.k.k_tiles, ceil_div(w.rows, 128), words, 2);
     const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
-    launch(kPair + w.format, static_cast<unsigned>(2 * std::min<int64_t>(clusters(2), tiles)), 320, kGemmSmem, 2, &p, stream);
+    launch(kPair + w.format, static_cast<unsigned>(2 * std::min<int64_t>(clusters(2, false), tiles)), 320, kGemmSmem, 2, &p, stream);
 }
 
 void Mx::product(const MxLinear& l, const MxMatrix& a, CUstream stream)
 {
     ContextGuard guard(ctx_);
-    if (ceil_div(a.rows, 256) * ceil_div(l.w.rows, 256) >= 1) {
+    if (ceil_div(a.rows, 256) * ceil_div(l.w.rows, 256) >= 48) {
         pair(l, a, stream);
         return;
     }

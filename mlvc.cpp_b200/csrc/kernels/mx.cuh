@@ -433,12 +433,12 @@ __device__ __forceinline__ void umma_mx(uint32_t tmem_d, uint64_t adesc, uint64_
             : "memory");
 }
 
-// A scale tile (512 bytes of shared memory) into four TMEM columns, repeated
-// for each warp's 32 lanes.
-__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t saddr)
+// A scale tile (512 bytes of shared memory, by its descriptor: no swizzle,
+// 128 bytes between eights of rows) into four TMEM columns, repeated for each
+// warp's 32 lanes.
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc)
 {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(smem_desc(saddr, 16, 128, 0))
-                 : "memory");
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
 // ---- the same over a pair of CTAs (cta_group::2): one thread of the even CTA
@@ -472,10 +472,9 @@ __device__ __forceinline__ void umma_mx_pair(uint32_t tmem_d, uint64_t adesc, ui
             : "memory");
 }
 
-__device__ __forceinline__ void tmem_copy_scales_pair(uint32_t taddr, uint32_t saddr)
+__device__ __forceinline__ void tmem_copy_scales_pair(uint32_t taddr, uint64_t desc)
 {
-    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(smem_desc(saddr, 16, 128, 0))
-                 : "memory");
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
 // Arrives on `bar` in both CTAs when the MMAs issued so far are complete.

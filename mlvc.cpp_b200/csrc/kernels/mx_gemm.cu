@@ -128,6 +128,9 @@ __device__ __forceinline__ void mx_gemm(const MxGemmParams& p)
             issuer = true;
             constexpr uint32_t idesc = mx_idesc<F>(128, BN);
             const uint32_t tmem_sa = tmem + 2 * BN, tmem_sb = tmem_sa + 4 * kWords;
+            // descriptors differ by their start addresses (16-byte units) alone
+            const uint64_t a_desc = smem_desc(smem_u32(stages), 16, 1024, 2);
+            const uint64_t s_desc = smem_desc(smem_u32(stages) + T::kA + T::kB, 16, 128, 0);
             int stage = 0;
             uint32_t phase = 0, acc = 0, acc_phase = 0;
             bool ok = true;
@@ -146,22 +149,21 @@ __device__ __forceinline__ void mx_gemm(const MxGemmParams& p)
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t s = smem_u32(stages + stage * T::kStage);
+                    const uint64_t a = a_desc + stage * (T::kStage >> 4), sa = s_desc + stage * (T::kStage >> 4);
                     const bool last = k + 1 == p.k.count;
                     const int words = last ? p.k.last_words : kWords, steps = last ? p.k.last_steps : 4;
                     for (int w = 0; w < words; ++w) {
-                        tmem_copy_scales(tmem_sa + 4 * w, s + T::kA + T::kB + 512 * w);
+                        tmem_copy_scales(tmem_sa + 4 * w, sa + 32 * w);
 #pragma unroll
                         for (int b = 0; b < T::kBands; ++b)
-                            tmem_copy_scales(tmem_sb + 4 * (w * T::kBands + b), s + T::kA + T::kB + T::kSA * (1 + b) + 512 * w);
+                            tmem_copy_scales(tmem_sb + 4 * (w * T::kBands + b), sa + (T::kSA >> 4) * (1 + b) + 32 * w);
                     }
 #pragma unroll
                     for (int ks = 0; ks < 4; ++ks) {
                         if (ks >= steps)
                             break;
                         const uint32_t w = ks * kWords / 4, id = kWords == 4 ? 0 : kWords == 2 ? (ks & 1) * 2 : ks;
-                        umma_mx<F>(d, smem_desc(s + ks * 32, 16, 1024, 2), smem_desc(s + T::kA + ks * 32, 16, 1024, 2), idesc,
-                                   id, tmem_sa + 4 * w, tmem_sb + 4 * w * T::kBands + in_band, (k | ks) != 0);
+                        umma_mx<F>(d, a + 2 * ks, a + (T::kA >> 4) + 2 * ks, idesc, id, tmem_sa + 4 * w, tmem_sb + 4 * w * T::kBands + in_band, (k | ks) != 0);
                         ++issued;
                     }
                     umma_commit(&sh->empty[stage]);

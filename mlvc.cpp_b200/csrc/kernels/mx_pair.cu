@@ -126,6 +126,9 @@ __device__ __forceinline__ void mx_pair(const MxPairParams& p)
             issuer = true;
             constexpr uint32_t idesc = mx_idesc<F>(256, 256);
             const uint32_t tmem_sa = tmem + 448, tmem_sb = tmem_sa + 4 * kWords;
+            // descriptors differ by their start addresses (16-byte units) alone
+            const uint64_t a_desc = smem_desc(smem_u32(stages), 16, 1024, 2);
+            const uint64_t s_desc = smem_desc(smem_u32(stages) + 2 * T::kOperand, 16, 128, 0);
             int stage = 0;
             uint32_t phase = 0, tile = 0;
             bool ok = true;
@@ -141,25 +144,24 @@ __device__ __forceinline__ void mx_pair(const MxPairParams& p)
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t s = smem_u32(stages + stage * T::kStage), sa = s + 2 * T::kOperand, sb = sa + T::kSA;
+                    const uint64_t a = a_desc + stage * (T::kStage >> 4), b = a + (T::kOperand >> 4);
+                    const uint64_t sa = s_desc + stage * (T::kStage >> 4), sb = sa + (T::kSA >> 4);
                     const bool last = k + 1 == p.k.count;
                     const int words = last ? p.k.last_words : kWords, steps = last ? p.k.last_steps : 4;
 #pragma unroll
                     for (int w = 0; w < kWords; ++w) {
                         if (w >= words)
                             break;
-                        tmem_copy_scales_pair(tmem_sa + 4 * w, sa + 512 * w);
-                        tmem_copy_scales_pair(tmem_sb + 8 * w, sb + 512 * w);
-                        tmem_copy_scales_pair(tmem_sb + 8 * w + 4, sb + T::kSA + 512 * w);
+                        tmem_copy_scales_pair(tmem_sa + 4 * w, sa + 32 * w);
+                        tmem_copy_scales_pair(tmem_sb + 8 * w, sb + 32 * w);
+                        tmem_copy_scales_pair(tmem_sb + 8 * w + 4, sb + (T::kSA >> 4) + 32 * w);
                     }
 #pragma unroll
                     for (int ks = 0; ks < 4; ++ks) {
                         if (ks >= steps)
                             break;
                         const uint32_t w = ks * kWords / 4, id = kWords == 4 ? 0 : kWords == 2 ? (ks & 1) * 2 : ks;
-                        umma_mx_pair<F>(d, smem_desc(s + ks * 32, 16, 1024, 2),
-                                        smem_desc(s + T::kOperand + ks * 32, 16, 1024, 2), idesc, id, tmem_sa + 4 * w,
-                                        tmem_sb + 8 * w, (k | ks) != 0);
+                        umma_mx_pair<F>(d, a + 2 * ks, b + 2 * ks, idesc, id, tmem_sa + 4 * w, tmem_sb + 8 * w, (k | ks) != 0);
                         ++issued;
                     }
                     umma_commit_pair(&sh->empty[stage]);

@@ -99,7 +99,8 @@ struct MxRowsParams {
     int splits;                        // CTAs of a cluster, each with its share of the panels
     int row_tile;                      // rows rounded up to 8
     int stages;
-    // dense rows: quantised in groups of panels, about four chunks a thread each,
+    int batch;                         // panels whose scales go to TMEM at once
+    // dense rows: quantised in groups of panels, about two chunks a thread each,
     // so that the first products begin before the last rows are quantised
     int group;
     const void* x;

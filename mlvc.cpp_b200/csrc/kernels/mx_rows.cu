@@ -4,15 +4,20 @@
 // Reading the weights bounds these calls, so the roles of the operands are
 // swapped: 128 weight rows fill the tensor core's M, the few rows of x are its
 // N (a multiple of 8), and nothing is padded to 128 but what is in memory
-// anyway.  Where there are fewer weight tiles than SMs, the panels of k are
-// split over the CTAs of a cluster; their sums meet through distributed shared
-// memory, in rank order, so results do not depend on timing.
+// anyway.  Where there are fewer weight tiles than room for CTAs, the panels of
+// k are split over the CTAs of a cluster.  Each of them finishes a share of y's
+// rows: the others copy it their sums of those rows in one piece (bulk copies
+// through distributed shared memory, counted by the receiver's barrier), and it
+// adds them in rank order, so results do not depend on timing.
 //
 // Dense rows are quantised here, by every CTA for its share of k, into the
-// swizzled tiles that the tensor core reads: that work (16 values a lane) runs
-// while the first weight panels are on their way, and saves a launch and a
-// round trip of x through memory.  Rows quantised beforehand come by TMA beside
-// each weight panel.
+// swizzled tiles that the tensor core reads: that work (16 values a lane, the
+// next two chunks of each lane under way meanwhile) runs while the first weight
+// panels are on their way, and saves a launch and a round trip of x through
+// memory.  Rows quantised beforehand come by TMA beside each weight panel.
+//
+// Scales go to TMEM for a batch of panels at once: copies and MMAs wait for each
+// other, about 150 cycles a turn.
 //
 // Warps: 0 copies, 1 MMA and TMEM, 2..9 quantise and then finish the sums.
 #include "mx.cuh"
@@ -28,44 +33,38 @@ struct MxRowsShared {
     uint64_t full[kMxRowsMaxStages];
     uint64_t empty[kMxRowsMaxStages];
     uint64_t x_full[kMxRowsMaxGroups];
-    uint64_t sums;
+    uint64_t sums;       // this CTA's sums are complete, and tmem_base is there
+    uint64_t received;   // the other CTAs' sums of this CTA's rows of y
     uint64_t drain;
     uint32_t tmem_base;
     int abort_flag;
 };
 static_assert(sizeof(MxRowsShared) <= kMxRowsHeader, "header");
 
-__device__ __forceinline__ float4 load_cluster(uint32_t saddr, uint32_t rank)
+// Shared memory of this CTA to the same or another place of the cluster's.
+__device__ __forceinline__ void bulk_send(uint32_t to, const void* from, uint32_t bytes, uint32_t bar)
 {
-    float4 v;
-    asm volatile(
-        "{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\t"
-        "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
-        : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-        : "r"(saddr), "r"(rank));
-    return v;
+    asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to),
+                 "r"(smem_u32(from)), "r"(bytes), "r"(bar)
+                 : "memory");
 }
 
 // One result.
-__device__ __forceinline__ void mx_finish_one(const MxEpilogue& e, int m, int n, float sum, float bias)
+template <int DT>
+__device__ __forceinline__ void mx_finish_one(const MxEpilogue& e, int m, int n, float sum)
 {
-    const float t = fmaf(sum, e.alpha, bias);
+    using T = typename Dense<DT>::T;
+    const float t = fmaf(sum, e.alpha, e.bias ? e.bias[n] : 0.0f);
     float v = t >= 0.0f ? t : t * e.slope;
-    const long long at = m * e.y_stride + n, res = m * e.residual_stride + n;
-    if (e.y_dtype == kMxF16) {
-        if (e.residual)
-            v += __half2float(static_cast<const __half*>(e.residual)[res]);
-        static_cast<__half*>(e.y)[at] = __float2half_rn(v);
-    } else if (e.y_dtype == kMxBf16) {
-        if (e.residual)
-            v += __bfloat162float(static_cast<const __nv_bfloat16*>(e.residual)[res]);
-        static_cast<__nv_bfloat16*>(e.y)[at] = __float2bfloat16_rn(v);
-    } else {
-        if (e.residual)
-            v += static_cast<const float*>(e.residual)[res];
-        static_cast<float*>(e.y)[at] = v;
-    }
+    if (e.residual)
+        v += Dense<DT>::load(static_cast<const T*>(e.residual) + m * e.residual_stride + n);
+    static_cast<T*>(e.y)[m * e.y_stride + n] = Dense<DT>::pack(v);
 }
+
+template <int DT>
+struct MxType {
+    static constexpr int value = DT;
+};
 
 // DT < 0: x is already quantised.
 template <int F, int DT>
@@ -85,10 +84,14 @@ __device__ __forceinline__ void mx_rows(const MxRowsParams& p)
     const int panels = k1 - k0;
     const int M = p.e.M;
 
-    // shared memory: dense: x tiles and their scales of all panels, then the
-    // ring of weight panels; else the ring holds both operands
+    // shared memory: sums of this CTA's rows from all CTAs, then, dense: x tiles
+    // and their scales of all panels, then the ring of weight panels; else the
+    // ring holds both operands.  The ring holds this CTA's sums in the end.
     const uint32_t x_bytes = static_cast<uint32_t>(p.row_tile) * 128u;
-    uint8_t* x_tiles = base + kMxRowsHeader;
+    const int share = (M + p.splits - 1) / p.splits;  // rows of y that a CTA finishes
+    const int m0 = static_cast<int>(rank) * share, mine = max(0, min(share, M - m0));
+    uint8_t* parts = base + kMxRowsHeader;
+    uint8_t* x_tiles = parts + (p.splits > 1 ? (p.splits * share * 512 + 1023) / 1024 * 1024 : 0);
     const int most = (p.k.count + p.splits - 1) / p.splits;
     uint8_t* x_scales = x_tiles + (kDense ? most * x_bytes : 0);
     uint8_t* ring = x_scales + (kDense ? (most * kS + 1023) / 1024 * 1024 : 0);
@@ -103,24 +106,23 @@ __device__ __forceinline__ void mx_rows(const MxRowsParams& p)
         if constexpr (kDense)
             for (int g = 0; g * p.group < panels; ++g)
                 mbar_init(&sh->x_full[g], 256);
-        mbar_init(&sh->sums, 1);
+        mbar_init(&sh->sums, 2);
+        mbar_init(&sh->received, 1);
         mbar_init(&sh->drain, 1);
         sh->abort_flag = 0;
         fence_barrier_init();
+        if (p.splits > 1)
+            mbar_arrive_expect_tx(&sh->received, static_cast<uint32_t>((p.splits - 1) * mine) * 512u);
     }
-    // TMEM is taken once the kernel before has ended: one that allocates after
-    // it let this one start would otherwise wait for columns held here.  The
-    // columns hold the sums, then the scales of both operands.
-    const uint32_t cols_needed = p.row_tile + 8 * kWords;
-    const uint32_t tmem_cols = cols_needed <= 64 ? 64 : cols_needed <= 128 ? 128 : 256;
-    pdl_wait();
-    if (warp == 1)
-        tmem_alloc(&sh->tmem_base, tmem_cols);
-    tc_fence_before();
     __syncthreads();
-    tc_fence_after();
-    pdl_launch_dependents();
-    const uint32_t tmem = sh->tmem_base;
+    if (p.splits > 1)  // waited for before anything is sent
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    // Memory and TMEM are touched once the kernel before has ended: one that
+    // allocates TMEM after it let this one start would otherwise wait for columns
+    // held here.  The columns hold the sums, then a batch of both operands' scales.
+    pdl_wait();
+    const uint32_t cols_needed = p.row_tile + p.batch * 8 * kWords;
+    const uint32_t tmem_cols = cols_needed <= 64 ? 64 : cols_needed <= 128 ? 128 : 256;
     bool issuer = false;
     uint32_t issued = 0;
 
@@ -159,46 +161,70 @@ __device__ __forceinline__ void mx_rows(const MxRowsParams& p)
         }
         __syncwarp();
     } else if (warp == 1) {
+        tmem_alloc(&sh->tmem_base, tmem_cols);
+        pdl_launch_dependents();
+        __syncwarp();
         if (elect_one()) {
             issuer = true;
+            mbar_arrive(&sh->sums);  // tmem_base
+            const uint32_t tmem = sh->tmem_base;
             const uint32_t idesc = mx_idesc<F>(128, p.row_tile);
-            const uint32_t tmem_sw = tmem + p.row_tile, tmem_sx = tmem_sw + 4 * kWords;
+            const uint32_t scales = tmem + p.row_tile;  // of a batch: weights' and x's 4 columns a scale tile
+            // descriptors differ by their start addresses (16-byte units) alone
+            const uint64_t ring_desc = smem_desc(smem_u32(ring), 16, 1024, 2);
+            const uint64_t ring_scales = smem_desc(smem_u32(ring) + sw_at, 16, 128, 0);
+            const uint64_t x_tiles_desc = smem_desc(smem_u32(x_tiles), 16, 1024, 2);
+            const uint64_t x_scales_desc = smem_desc(smem_u32(x_scales), 16, 128, 0);
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
-            for (int k = k0, g = 0; ok && k < k1; ++k) {
-                if (kDense && k - k0 == g * p.group &&
-                    !mbar_wait(&sh->x_full[g++], 0, &sh->abort_flag, kErrMxMma)) {
-                    ok = false;
-                    break;
-                }
-                if (!mbar_wait(&sh->full[stage], phase, &sh->abort_flag, kErrMxMma)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t s = smem_u32(ring + stage * stage_bytes);
-                const uint32_t x = kDense ? smem_u32(x_tiles) + (k - k0) * x_bytes : s + x_at;
-                const uint32_t sx = kDense ? smem_u32(x_scales) + (k - k0) * kS : s + sx_at;
-                const bool last = k + 1 == p.k.count;
-                const int words = last ? p.k.last_words : kWords, steps = last ? p.k.last_steps : 4;
-                for (int w = 0; w < words; ++w) {
-                    tmem_copy_scales(tmem_sw + 4 * w, s + sw_at + 512 * w);
-                    tmem_copy_scales(tmem_sx + 4 * w, sx + 512 * w);
-                }
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks) {
-                    if (ks >= steps)
+            for (int k = k0, g = 0; ok && k < k1; k += p.batch) {
+                const int n = min(p.batch, k1 - k);
+                int at = stage;
+                uint32_t at_phase = phase;
+                for (int i = 0; ok && i < n; ++i) {
+                    if (kDense && k + i - k0 == g * p.group)
+                        ok = mbar_wait(&sh->x_full[g++], 0, &sh->abort_flag, kErrMxMma);
+                    if (!ok || !mbar_wait(&sh->full[at], at_phase, &sh->abort_flag, kErrMxMma)) {
+                        ok = false;
                         break;
-                    const uint32_t w = ks * kWords / 4, id = kWords == 4 ? 0 : kWords == 2 ? (ks & 1) * 2 : ks;
-                    umma_mx<F>(tmem, smem_desc(s + ks * 32, 16, 1024, 2), smem_desc(x + ks * 32, 16, 1024, 2), idesc, id,
-                               tmem_sw + 4 * w, tmem_sx + 4 * w, (k - k0) | ks);
-                    ++issued;
+                    }
+                    tc_fence_after();
+                    const uint64_t sw = ring_scales + at * (stage_bytes >> 4);
+                    const uint64_t sx = kDense ? x_scales_desc + (k + i - k0) * (kS >> 4) : sw + ((sx_at - sw_at) >> 4);
+                    const uint32_t to = scales + 8 * kWords * i;
+                    const int words = k + i + 1 == p.k.count ? p.k.last_words : kWords;
+#pragma unroll
+                    for (int w = 0; w < kWords; ++w) {
+                        if (w >= words)
+                            break;
+                        tmem_copy_scales(to + 8 * w, sw + 32 * w);
+                        tmem_copy_scales(to + 8 * w + 4, sx + 32 * w);
+                    }
+                    if (++at == p.stages) {
+                        at = 0;
+                        at_phase ^= 1u;
+                    }
                 }
-                umma_commit(&sh->empty[stage]);
-                if (++stage == p.stages) {
-                    stage = 0;
-                    phase ^= 1u;
+                for (int i = 0; ok && i < n; ++i) {
+                    const uint64_t w_desc = ring_desc + stage * (stage_bytes >> 4);
+                    const uint64_t x_desc = kDense ? x_tiles_desc + (k + i - k0) * (x_bytes >> 4) : w_desc + (x_at >> 4);
+                    const uint32_t from = scales + 8 * kWords * i;
+                    const int steps = k + i + 1 == p.k.count ? p.k.last_steps : 4;
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks) {
+                        if (ks >= steps)
+                            break;
+                        const uint32_t w = ks * kWords / 4, id = kWords == 4 ? 0 : kWords == 2 ? (ks & 1) * 2 : ks;
+                        umma_mx<F>(tmem, w_desc + 2 * ks, x_desc + 2 * ks, idesc, id, from + 8 * w, from + 8 * w + 4,
+                                   (k + i - k0) | ks);
+                        ++issued;
+                    }
+                    umma_commit(&sh->empty[stage]);
+                    if (++stage == p.stages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
                 }
             }
             if (ok)
@@ -208,30 +234,37 @@ __device__ __forceinline__ void mx_rows(const MxRowsParams& p)
     } else {
         const int t = threadIdx.x - 64;  // 0..255
         if constexpr (kDense) {
-            // a group of panels at a time, four chunks a thread under way at once
+            // A group of panels at a time, two chunks a thread, the next two
+            // under way.  The code is small on purpose: in calls this short it
+            // comes from memory as x does.
             constexpr int kChunks = Mx<F>::kPanelValues / 16;  // of a panel
-            constexpr int kBatch = 4;
-            for (int g = 0; g * p.group < panels; ++g) {
-                const int first = g * p.group;  // panel
-                const int row_chunks = min(p.group, panels - first) * kChunks, items = M * row_chunks;
-                for (int i0 = t; i0 < ((items + 31) & ~31); i0 += 256 * kBatch) {
-                    Raw<DT> x[kBatch];
+            constexpr int kBatch = 2;
+            const typename Dense<DT>::T* dense = static_cast<const typename Dense<DT>::T*>(p.x);
+            Raw<DT> now[kBatch];
+            // the chunks that were asked for: from i0 on in the group that begins at panel `first`
+            int first = 0, i0 = t, row_chunks = 0;
+            for (int next_first = 0, next = t;;) {
+                const int next_chunks = min(p.group, panels - next_first) * kChunks;
+                const bool more = next_first < panels;
+                Raw<DT> ahead[kBatch];
 #pragma unroll
-                    for (int b = 0; b < kBatch; ++b) {
-                        const int i = i0 + 256 * b, m = i / row_chunks, c = i - m * row_chunks;
-                        if (i < items)
-                            load_raw<DT>(static_cast<const typename Dense<DT>::T*>(p.x) + m * p.row_stride, p.col_stride,
-                                         ((k0 + first) * kChunks + c) * 16, p.cols, p.vec, x[b]);
-                        else
-                            x[b] = Raw<DT>{};
-                    }
+                for (int b = 0; b < kBatch; ++b) {
+                    const int i = next + 256 * b, m = i / max(next_chunks, 1), c = i - m * next_chunks;
+                    if (more && m < M)
+                        load_raw<DT>(dense + m * p.row_stride, p.col_stride, ((k0 + next_first) * kChunks + c) * 16, p.cols,
+                                     p.vec, ahead[b]);
+                    else
+                        ahead[b] = Raw<DT>{};
+                }
+                if (row_chunks) {
+                    const int items = M * row_chunks;
 #pragma unroll
                     for (int b = 0; b < kBatch; ++b) {
                         const int i = i0 + 256 * b, m = i / row_chunks, c = i - m * row_chunks;
                         if ((i & ~31) >= items)  // whole warps
                             break;
                         uint32_t codes[4], scale;
-                        quantise_chunk<F, DT>(x[b], p.tensor_scale, p.inv_six_scale, codes, scale);
+                        quantise_chunk<F, DT>(now[b], p.tensor_scale, p.inv_six_scale, codes, scale);
                         if (i >= items)
                             continue;
                         const int panel = first + c / kChunks, in = c % kChunks;
@@ -246,37 +279,87 @@ __device__ __forceinline__ void mx_rows(const MxRowsParams& p)
                             x_scales[panel * kS + (column >> 2) * 512 + (m & 31) * 16 + (m >> 5) * 4 + (column & 3)] =
                                 static_cast<uint8_t>(scale);
                     }
+                    if (next_first != first) {
+                        fence_proxy_async_smem();  // the tensor core reads through the async proxy
+                        mbar_arrive(&sh->x_full[first / p.group]);
+                    }
                 }
-                fence_proxy_async_smem();  // the tensor core reads through the async proxy
-                mbar_arrive(&sh->x_full[g]);
+                if (!more)
+                    break;
+                first = next_first;
+                i0 = next;
+                row_chunks = next_chunks;
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b)
+                    now[b] = ahead[b];
+                next += 256 * kBatch;
+                if ((next & ~31) >= M * next_chunks) {  // the warp has no more of this group
+                    next = t;
+                    next_first += p.group;
+                }
             }
         }
+        __syncwarp();
         // the warp's quadrant of the 128 weight rows, half of the columns (rows
-        // of x, 32 at a time)
+        // of x, 16 at a time)
         const int quadrant = warp & 3, group = (warp - 2) / 4, n = quadrant * 32 + lane;
+        if (p.splits > 1)
+            asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         const bool ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sh->sums, 0, &sh->abort_flag, kErrMxEpilogue));
         tc_fence_after();
+        float* sums = reinterpret_cast<float*>(ring);  // [row of x][128], once the weights are consumed
         if (ok) {
-            float* part = reinterpret_cast<float*>(ring);  // [row of x][128], once the weights are consumed
-            const float bias = p.e.bias && n0 + n < p.e.N ? p.e.bias[n0 + n] : 0.0f;
-            for (int c = group * 32; c < M; c += 64) {
-                uint32_t v[32];
-                const uint32_t at = tmem + c + (static_cast<uint32_t>(quadrant * 32) << 16);
-                tmem_ld32_nowait(at, v);
+            const uint32_t tmem = sh->tmem_base + (static_cast<uint32_t>(quadrant * 32) << 16);
+            for (int c = group * 16; c < M; c += 32) {
+                uint32_t v[16];
+                tmem_ld16_nowait(tmem + c, v);
                 tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    if (c + i >= M)
-                        break;
-                    if (p.splits > 1)
-                        part[(c + i) * 128 + n] = __uint_as_float(v[i]);
-                    else if (n0 + n < p.e.N)
-                        mx_finish_one(p.e, c + i, n0 + n, __uint_as_float(v[i]), bias);
-                }
+                for (int i = 0; i < 16; ++i)
+                    if (c + i < M)
+                        sums[(c + i) * 128 + n] = __uint_as_float(v[i]);
                 __syncwarp();
             }
         }
+        fence_proxy_async_smem();  // the bulk copies read through the async proxy
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        bool all = !sh->abort_flag;
+        if (p.splits > 1) {
+            // one thread for each other CTA; a CTA that gave up sends nothing
+            if (t < p.splits && t != static_cast<int>(rank) && all) {
+                const int first = t * share, rows = min(share, M - first);
+                if (rows > 0)
+                    bulk_send(cluster_address(parts + rank * share * 512, t), sums + first * 128,
+                              static_cast<uint32_t>(rows) * 512u, cluster_address(&sh->received, t));
+            }
+            all = mine > 0 && mbar_wait(&sh->received, 0, &sh->abort_flag, kErrMxEpilogue);
+        }
+        // a warp takes 32 columns of a row of y at a time
+        auto finish = [&](auto type) {
+#pragma unroll 1
+            for (int i = warp - 2; i < mine * 4; i += 8) {
+                const int j = i >> 2, c = (i & 3) * 32 + lane;
+                float sum = 0.0f;
+#pragma unroll 2
+                for (int r = 0; r < p.splits; ++r)
+                    sum += r == static_cast<int>(rank) ? sums[(m0 + j) * 128 + c]
+                                                       : reinterpret_cast<const float*>(parts)[(r * share + j) * 128 + c];
+                if (n0 + c < p.e.N)
+                    mx_finish_one<decltype(type)::value>(p.e, m0 + j, n0 + c, sum);
+            }
+        };
+        if (all) {
+            if (p.e.y_dtype == kMxF16)
+                finish(MxType<kMxF16>{});
+            else if (p.e.y_dtype == kMxBf16)
+                finish(MxType<kMxBf16>{});
+            else
+                finish(MxType<kMxF32>{});
+        }
+        __syncwarp();
     }
+    if (p.splits > 1 && warp < 2)
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (issuer && sh->abort_flag && issued) {  // MMAs in flight end before TMEM is freed
         umma_commit(&sh->drain);
         volatile int never = 0;
@@ -284,37 +367,11 @@ __device__ __forceinline__ void mx_rows(const MxRowsParams& p)
     }
     tc_fence_before();
     __syncthreads();
-    if (p.splits > 1) {
-        cluster_barrier();  // every CTA's part is written
-        if (warp >= 2) {
-            // a warp takes a row of x: four columns a lane, all parts under way at once
-            const uint32_t part = smem_u32(ring) + lane * 16;
-            for (int m = static_cast<int>(rank) + p.splits * (warp - 2); m < M; m += 8 * p.splits) {
-                float4 v[8];
-#pragma unroll
-                for (int r = 0; r < 8; ++r)
-                    if (r < p.splits)
-                        v[r] = load_cluster(part + m * 512, r);
-                float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-                for (int r = 0; r < 8; ++r)
-                    if (r < p.splits)
-                        sum = make_float4(sum.x + v[r].x, sum.y + v[r].y, sum.z + v[r].z, sum.w + v[r].w);
-                const float s[4] = {sum.x, sum.y, sum.z, sum.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int n = n0 + lane * 4 + i;
-                    if (n < p.e.N)
-                        mx_finish_one(p.e, m, n, s[i], p.e.bias ? p.e.bias[n] : 0.0f);
-                }
-            }
-        }
-        __syncwarp();
-        cluster_barrier();  // no CTA leaves while its part is being read
-    }
+    if (p.splits > 1)
+        cluster_barrier();  // no CTA leaves while its sums are being copied or others may reach it
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, tmem_cols);
+        tmem_dealloc(sh->tmem_base, tmem_cols);
     }
 }
 
