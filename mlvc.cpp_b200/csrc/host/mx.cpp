@@ -211,10 +211,10 @@ void Mx::launch(int index, unsigned grid, unsigned block, unsigned smem, unsigne
     check(cuLaunchKernelEx(&cfg, fn(index), args, nullptr), "cuLaunchKernelEx(mx)");
 }
 
-// Clusters of this many blocks that run at once, one or two blocks an SM.
-int Mx::clusters(int size, bool half_sm)
+// Clusters of this many blocks that run at once, one block an SM.
+int Mx::clusters(int size)
 {
-    int& known = clusters_[half_sm][size];
+    int& known = clusters_[size];
     if (!known) {
         CUlaunchAttribute attr{};
         attr.id = CU_LAUNCH_ATTRIBUTE_CLUSTER_DIMENSION;
@@ -225,7 +225,7 @@ int Mx::clusters(int size, bool half_sm)
         cfg.gridDimY = cfg.gridDimZ = 1;
         cfg.blockDimX = 320;
         cfg.blockDimY = cfg.blockDimZ = 1;
-        cfg.sharedMemBytes = half_sm ? 113 * 1024 : kGemmSmem;
+        cfg.sharedMemBytes = kGemmSmem;
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
         int n = 0;
@@ -479,7 +479,11 @@ bool Mx::few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream)
 {
     const MxMatrix& w = l.w;
     const int64_t rows = a ? a->rows : l.x.rows;
-    if (rows > kMxRowsMax)
+    // Measured against the tiles of 128 rows (nvfp4, 4096 x 4096: 32 rows 6.2 us
+    // to 7.9, 64 rows 7.2 to 7.9, 96 rows 8.5 to 8.0): from 64 rows on sending
+    // and adding up the parts costs more than the padding.  Rows of less than 8
+    // panels leave less to share (1024 x 1024: 32 rows 4.6 to 4.6, 64 rows 5.8 to 4.6).
+    if (rows > (w.cols <= 1024 && w.format != kMxFp8 ? kMxRowsMax / 2 : kMxRowsMax))
         return false;
     ContextGuard guard(ctx_);
     MxRowsParams p{};
@@ -496,23 +500,32 @@ bool Mx::few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream)
         return 2048 + (splits > 1 ? ceil_div(splits * ceil_div(rows, splits) * 512, 1024) * 1024 : 0) +
                (a ? 0 : most * x_bytes + ceil_div(most * scale_bytes, 1024) * 1024);
     };
-    // as many CTAs on k as there is room for at once, each with two panels or
-    // more; two CTAs an SM (the waits of one are filled by the other) where that
-    // leaves a ring of four and no fewer CTAs; clusters take SMs of one group, so
-    // fewer of them fit than SMs divided by their size
+    // As many CTAs on k as there are SMs for at once, each with two panels or
+    // more; clusters take SMs of one group, so fewer of them fit than SMs divided
+    // by their size.  Where that is one, two CTAs share an SM: in a cluster while
+    // two times as many still fit (14336 x 4096 nvfp4, 16 rows: 10.6 -> 9.6 us),
+    // each on a tile of its own beyond that.  More CTAs than that on k lose more
+    // by their parts than they win (4096 x 4096: 5.1 -> 7.1 us).
     const size_t whole = kGemmSmem, half = 113 * 1024;
-    size_t room = 0;
-    const int widest = static_cast<int>(std::clamp<int64_t>(p.k.count / 2, 1, 8));
-    for (const bool half_sm : {true, false})
-        for (int splits = widest; splits >= 1; --splits)
-            if (splits > (room ? p.splits : 0) &&
-                fixed(splits) + std::min<size_t>(most, half_sm ? 4 : 3) * stage <= (half_sm ? half : whole) &&
-                (splits == 1 || n_tiles <= clusters(splits, half_sm))) {
-                room = half_sm ? half : whole;
-                p.splits = splits;
-                break;
-            }
-    if (!room)
+    auto fits = [&](int splits, size_t room) { return fixed(splits) + std::min<size_t>(most, 3) * stage <= room; };
+    p.splits = static_cast<int>(std::clamp<int64_t>(p.k.count / 2, 1, 8));
+    while (p.splits > 1 && n_tiles > clusters(p.splits))
+        --p.splits;
+    size_t room = whole;
+    if (p.splits == 1) {
+        if (p.k.count >= 4 && n_tiles <= 2 * clusters(2) && fits(2, half)) {
+            p.splits = 2;
+            room = half;
+        } else if (n_tiles > sm_count_ && fits(1, half)) {
+            room = half;
+        }
+    }
+    if (!fits(p.splits, room))
+        return false;
+    // Every CTA quantises its share of dense rows again: more than four chunks a
+    // thread cost more than a kernel that does it once (4096 x 4096: 16 rows 6.7
+    // to 7.1 us, 32 rows 9.9 to 8.4)
+    if (!a && rows * most * (w.format == kMxFp8 ? 8 : 16) > 1024)
         return false;
     const size_t used = fixed(p.splits);
     p.stages = static_cast<int>(std::min<size_t>({static_cast<size_t>(most), (room - used) / stage, 12}));
@@ -562,13 +575,21 @@ void Mx::pair(const MxLinear& l, const MxMatrix& a, CUstream stream)
     encode_scales(&p.map_sa, a.scales, p.k.k_tiles, ceil_div(a.rows, 128), words, 1);
     encode_scales(&p.map_sb, w.scales, p.k.k_tiles, ceil_div(w.rows, 128), words, 2);
     const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
-    launch(kPair + w.format, static_cast<unsigned>(2 * std::min<int64_t>(clusters(2, false), tiles)), 320, kGemmSmem, 2, &p, stream);
+    launch(kPair + w.format, static_cast<unsigned>(2 * std::min<int64_t>(clusters(2), tiles)), 320, kGemmSmem, 2, &p, stream);
 }
 
 void Mx::product(const MxLinear& l, const MxMatrix& a, CUstream stream)
 {
     ContextGuard guard(ctx_);
-    if (ceil_div(a.rows, 256) * ceil_div(l.w.rows, 256) >= 48) {
+    // Tiles of 128 x 64, 128 x 128 or, by pairs of CTAs, 256 x 256: the least
+    // rounds over the SMs, each weighted with what it takes (nvfp4, k = 4096: 5.2,
+    // 6.1 and 8.7 us a round beside 3 us that every call takes).
+    const int64_t m128 = ceil_div(a.rows, 128), n64 = ceil_div(l.w.rows, 64), n128 = ceil_div(l.w.rows, 128);
+    const double t64 = 0.87 * static_cast<double>(ceil_div(m128 * n64, sm_count_));
+    const double t128 = static_cast<double>(ceil_div(m128 * n128, sm_count_));
+    const double t256 =
+        1.45 * static_cast<double>(ceil_div(ceil_div(a.rows, 256) * ceil_div(l.w.rows, 256), std::max(1, sm_count_ / 2)));
+    if (t256 <= t128 && t256 <= t64) {
         pair(l, a, stream);
         return;
     }
@@ -580,7 +601,7 @@ void Mx::product(const MxLinear& l, const MxMatrix& a, CUstream stream)
     p.k = panels_of(w.format, w.cols);
     p.e = epilogue_of(l, a.rows, a.tensor_scale);
     p.m_tiles = static_cast<int>(ceil_div(a.rows, 128));
-    const bool narrow = p.m_tiles * ceil_div(w.rows, 128) < sm_count_;
+    const bool narrow = t64 < t128;
     const int bn = narrow ? 64 : 128;
     p.n_tiles = static_cast<int>(ceil_div(w.rows, bn));
     if (static_cast<int64_t>(p.m_tiles) * p.n_tiles > 0x7FFFFFFF - 8 * p.n_tiles)

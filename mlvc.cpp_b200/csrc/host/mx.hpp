@@ -85,7 +85,7 @@ private:
     bool few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream);
     void product(const MxLinear& l, const MxMatrix& a, CUstream stream);
     void pair(const MxLinear& l, const MxMatrix& a, CUstream stream);
-    int clusters(int size, bool half_sm);
+    int clusters(int size);
     void launch(int index, unsigned grid, unsigned block, unsigned smem, unsigned cluster, void* params, CUstream stream);
     void require_device() const;
 
@@ -94,7 +94,7 @@ private:
     CUdeviceptr status_ = 0;
     int sm_count_ = 0;
     CUfunction functions_[64] = {};
-    int clusters_[2][9] = {};  // by size, 0: not asked yet
+    int clusters_[9] = {};  // by size, 0: not asked yet
 };
 
 }  // namespace mlvc_b200

@@ -87,9 +87,9 @@ struct MxPairParams {
     MxEpilogue e;
 };
 
-// Products of at most 128 rows (see mx_rows): weights are the tensor core's
-// first operand, rows its second.
-constexpr int kMxRowsMax = 128;
+// Products of few rows (see mx_rows): weights are the tensor core's first
+// operand, rows its second.
+constexpr int kMxRowsMax = 64;
 struct MxRowsParams {
     CUtensorMap map_w;                 // weights, boxes of 128 bytes x 128 rows
     CUtensorMap map_x;                 // quantised rows, boxes of 128 bytes x row_tile rows

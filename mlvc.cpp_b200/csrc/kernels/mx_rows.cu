@@ -1,4 +1,4 @@
-// Products of few rows (1 to 128) with quantised weights:
+// Products of few rows (1 to 64) with quantised weights:
 //     y[m, n] = leaky(alpha * sum_k x[m, k] w[n, k] + bias[n]) + residual[m, n]
 //
 // Reading the weights bounds these calls, so the roles of the operands are
@@ -334,18 +334,23 @@ __device__ __forceinline__ void mx_rows(const MxRowsParams& p)
             }
             all = mine > 0 && mbar_wait(&sh->received, 0, &sh->abort_flag, kErrMxEpilogue);
         }
-        // a warp takes 32 columns of a row of y at a time
+        // a warp takes a row of y, a lane every 32nd column of it
         auto finish = [&](auto type) {
 #pragma unroll 1
-            for (int i = warp - 2; i < mine * 4; i += 8) {
-                const int j = i >> 2, c = (i & 3) * 32 + lane;
-                float sum = 0.0f;
-#pragma unroll 2
-                for (int r = 0; r < p.splits; ++r)
-                    sum += r == static_cast<int>(rank) ? sums[(m0 + j) * 128 + c]
-                                                       : reinterpret_cast<const float*>(parts)[(r * share + j) * 128 + c];
-                if (n0 + c < p.e.N)
-                    mx_finish_one<decltype(type)::value>(p.e, m0 + j, n0 + c, sum);
+            for (int j = warp - 2; j < mine; j += 8) {
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+                for (int r = 0; r < p.splits; ++r) {
+                    const float* from = r == static_cast<int>(rank) ? sums + (m0 + j) * 128
+                                                                    : reinterpret_cast<const float*>(parts) + (r * share + j) * 128;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        sum[i] += from[32 * i + lane];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (n0 + 32 * i + lane < p.e.N)
+                        mx_finish_one<decltype(type)::value>(p.e, m0 + j, n0 + 32 * i + lane, sum[i]);
             }
         };
         if (all) {
@@ -375,8 +380,10 @@ __device__ __forceinline__ void mx_rows(const MxRowsParams& p)
     }
 }
 
+// Two CTAs an SM have to be asked for: without it a kernel that allocates TMEM
+// gets an SM to itself, whatever its registers and shared memory are.
 #define MLVC_MX_ROWS(NAME, F, DT)                                                                              \
-    extern "C" __global__ void __launch_bounds__(kMxRowsThreads) NAME(const __grid_constant__ MxRowsParams p) \
+    extern "C" __global__ void __launch_bounds__(kMxRowsThreads, 2) NAME(const __grid_constant__ MxRowsParams p) \
     {                                                                                                          \
         mx_rows<F, DT>(p);                                                                                     \
     }
