@@ -89,7 +89,7 @@ int wide(const MxDense& d)
 }
 
 // Order of functions_: the four conversions by type and format, then products.
-enum { kQuantise = 0, kDequantise = 9, kCacheWrite = 18, kCacheRead = 27, kGemm64 = 36, kGemm128 = 39, kRows = 42, kPair = 54, kFunctions = 57 };
+enum { kQuantise = 0, kDequantise = 9, kCacheWrite = 18, kCacheRead = 27, kGemm64 = 36, kGemm128 = 39, kRows = 42, kPair = 54, kTall = 57, kFunctions = 66 };
 
 int convert_index(int base, int dtype, int format) { return base + (dtype == kMxF16 ? 0 : dtype == kMxBf16 ? 3 : 6) + format; }
 
@@ -99,6 +99,8 @@ std::string function_name(int i)
     static const int types[3] = {kMxF16, kMxBf16, kMxF32};
     if (i < kGemm64)
         return std::string("mlvc_mx_") + conversions[i / 9] + "_" + kTypeNames[types[i % 9 / 3]] + "_" + kFormatNames[i % 3];
+    if (i >= kTall)
+        return std::string("mlvc_mx_tall_") + kTypeNames[types[(i - kTall) / 3]] + "_" + kFormatNames[i % 3];
     if (i >= kPair)
         return std::string("mlvc_mx_pair_") + kFormatNames[i % 3];
     if (i >= kRows)
@@ -405,7 +407,7 @@ void Mx::linear(const MxLinear& l, CUstream stream)
             product(l, l.a, stream);
         return;
     }
-    if (few_rows(l, nullptr, stream))
+    if (few_rows(l, nullptr, stream) || tall(l, stream))
         return;
     const MxLayout lay = mx_layout(w.format, rows, cols);
     const MxMatrix a{w.format, l.tensor_scale, rows, cols, l.workspace, l.workspace + (lay.data_bytes + 255) / 256 * 256};
@@ -454,7 +456,7 @@ MxEpilogue epilogue_of(const MxLinear& l, int64_t rows, float x_scale)
     auto aligned = [&](const MxDense& d) {
         return d.data % 16 == 0 && (d.rows <= 1 || static_cast<size_t>(d.row_stride) * size % 16 == 0);
     };
-    e.vec = aligned(l.y) && (!l.residual.data || aligned(l.residual));
+    e.vec = aligned(l.y) && (!l.residual.data || aligned(l.residual)) && l.bias % 16 == 0;
     e.alpha = x_scale * l.w.tensor_scale;
     e.slope = l.slope;
     return e;
@@ -557,6 +559,44 @@ bool Mx::few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream)
     const int type = a ? 0 : l.x.dtype == kMxF16 ? 1 : l.x.dtype == kMxBf16 ? 2 : 3;
     launch(kRows + 3 * type + w.format, static_cast<unsigned>(grid), 320, static_cast<unsigned>(smem),
            static_cast<unsigned>(p.splits), &p, stream);
+    return true;
+}
+
+bool Mx::tall(const MxLinear& l, CUstream stream)
+{
+    const MxMatrix& w = l.w;
+    MxTallParams p{};
+    p.k = panels_of(w.format, w.cols);
+    const int words = w.format == kNvFp4 ? 4 : w.format == kMxFp4 ? 2 : 1;
+    // Fewer rows leave the SMs one CTA with little to do at a time (256 -> 256
+    // nvfp4: 8192 rows 8.8 us to 7.7 of two kernels, 14336 rows 8.4 to 11, 32640
+    // rows 11.8 to 16.8)
+    if (p.k.k_tiles > kMxTallScaleTiles || l.x.rows < 96 * sm_count_)
+        return false;
+    p.n_tiles = static_cast<int>(ceil_div(w.rows, 64));
+    const size_t scale_bytes = static_cast<size_t>(p.k.k_tiles) * 512;
+    const size_t smem = 2048 + p.k.count * size_t{128 * 128} + 2 * (p.k.count * size_t{64 * 128} + ceil_div(scale_bytes, 1024) * 1024) +
+                        static_cast<size_t>(p.k.count) * words * 512 + 8 * size_t{4096};
+    // two CTAs an SM, or it is no faster (512 -> 128 mxfp8: 22 us to 20)
+    if (smem > 113 * 1024)
+        return false;
+    // as many rows a tile as let all SMs end together
+    const int64_t rounds = ceil_div(l.x.rows, static_cast<int64_t>(sm_count_) * 128);
+    p.tile_rows = static_cast<int>(std::min<int64_t>(128, ceil_div(ceil_div(l.x.rows, sm_count_ * rounds), 8) * 8));
+    ContextGuard guard(ctx_);
+    encode_rows(&p.map_w, w.data, pitch_of(w.format, w.cols), w.rows, 64);
+    p.scales_w = reinterpret_cast<const uint8_t*>(w.scales);
+    p.x = reinterpret_cast<const void*>(l.x.data);
+    p.row_stride = l.x.row_stride;
+    p.col_stride = l.x.col_stride;
+    p.cols = static_cast<int>(l.x.cols);
+    p.vec = wide(l.x);
+    p.tensor_scale = l.tensor_scale;
+    p.inv_six_scale = inverse_six(l.tensor_scale);
+    p.e = epilogue_of(l, l.x.rows, l.tensor_scale);
+    const int type = l.x.dtype == kMxF16 ? 0 : l.x.dtype == kMxBf16 ? 1 : 2;
+    launch(kTall + 3 * type + w.format, static_cast<unsigned>(ceil_div(l.x.rows, p.tile_rows)), 288, static_cast<unsigned>(smem), 1,
+           &p, stream);
     return true;
 }
 

@@ -83,6 +83,8 @@ private:
     // y from rows quantised in `a`, or (a null) from dense rows quantised by the
     // product's kernel itself; false: there is no such kernel for these sizes.
     bool few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream);
+    // y from dense rows and weights that fit in shared memory; false: they do not.
+    bool tall(const MxLinear& l, CUstream stream);
     void product(const MxLinear& l, const MxMatrix& a, CUstream stream);
     void pair(const MxLinear& l, const MxMatrix& a, CUstream stream);
     int clusters(int size);
@@ -93,7 +95,7 @@ private:
     CUmodule module_ = nullptr;
     CUdeviceptr status_ = 0;
     int sm_count_ = 0;
-    CUfunction functions_[64] = {};
+    CUfunction functions_[72] = {};
     int clusters_[9] = {};  // by size, 0: not asked yet
 };
 

@@ -292,29 +292,27 @@ __device__ __forceinline__ void quantise_chunk(const Raw<DT>& x, float tensor_sc
         const float w4[4] = {want, 0.0f, 0.0f, 0.0f};
         scale = finite ? e4m3x4(w4) & 0xFFu : 0x7Fu;
         const float r = scale_value<F>(scale) * tensor_scale;
-        if (scale - 1u < 0x7Du) {
-            // neither zero, NaN nor the largest: |v / r| stays below 8, so
-            // nothing overflows (r lies in [2^-99, 2^99]), and what underflows
-            // is far below the smallest code's half.  h is below 1 / r by a few
-            // of its last places, so l >= 0 and a zero keeps its sign.
-            float h;
-            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(h) : "f"(r));
-            h = __uint_as_float(__float_as_uint(h) - 2u);
-            const float l = fmaf(-r, h, 1.0f) * h;
-            const uint64_t hh = pair(h, h), ll = pair(l, l);
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                const uint64_t vv = pair(v[i], v[i + 1]);
-                split(fma2(vv, hh, mul2(vv, ll)), v[i], v[i + 1]);
-            }
-        } else if (scale == 0x7Eu) {
+        // h is below 1 / r by a few of its last places, so l >= 0 and a zero
+        // keeps its sign.  r lies in [2^-99, 2^99]; below the largest scale
+        // |v / r| stays below 8, and what underflows is far below the smallest
+        // code's half.
+        float h;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(h) : "f"(r));
+        h = __uint_as_float(__float_as_uint(h) - 2u);
+        float l = fmaf(-r, h, 1.0f) * h;
+        if (scale - 1u >= 0x7Du) {  // rare: zero, NaN, or the largest
+            if (scale != 0x7Eu)
+                h = l = 0.0f;
+            const float most = scale == 0x7Eu ? 8.0f * r : __uint_as_float(0x7F7FFFFFu);
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                v[i] = __fdiv_rn(v[i], r);
-        } else {
+                v[i] = finite ? fminf(fmaxf(v[i], -most), most) : 0.0f;
+        }
+        const uint64_t hh = pair(h, h), ll = pair(l, l);
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                v[i] = finite ? v[i] * 0.0f : 0.0f;  // zeros keep their sign
+        for (int i = 0; i < 16; i += 2) {
+            const uint64_t vv = pair(v[i], v[i + 1]);
+            split(fma2(vv, hh, mul2(vv, ll)), v[i], v[i + 1]);
         }
     } else {
         const int e = static_cast<int>(m >> 23) - Mx<F>::kExponentMax;

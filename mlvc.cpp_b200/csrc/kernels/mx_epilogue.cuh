@@ -16,108 +16,164 @@ namespace mlvc_b200 {
 
 constexpr int kMxTurnBytes = 4096;  // of a warp
 
-template <int DT>
-struct MxTurn {
-    static constexpr int kCols = DT == kMxF32 ? 4 : 8;  // a lane's columns: 16 bytes of y
-    static constexpr int kLanes = 32 / kCols;           // of a row
-    static constexpr int kRounds = kLanes;              // each of 32 / kLanes rows
-};
-
-// `after` is called once the sums are in registers.
-template <int DT, typename After>
-__device__ __forceinline__ void mx_empty_chunk(const MxEpilogue& e, float4* turn, uint32_t taddr, long long row0, int col0,
-                                               After&& after)
+__device__ __forceinline__ uint4 load16(const void* p)
 {
-    using D = Dense<DT>;
-    using T = typename D::T;
-    using S = MxTurn<DT>;
-    const int lane = threadIdx.x & 31;
-    const int col = col0 + (lane % S::kLanes) * S::kCols, sub = lane / S::kLanes;
-    const bool wide = e.vec && col + S::kCols <= e.N;
-    uint4 res[S::kRounds];
-    float bias[S::kCols];
-#pragma unroll
-    for (int i = 0; i < S::kRounds; ++i) {
-        res[i] = make_uint4(0, 0, 0, 0);
-        const long long row = row0 + sub + i * S::kCols;
-        if (e.residual && wide && row < e.M)
-            res[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(e.residual) + row * e.residual_stride + col);
-    }
-#pragma unroll
-    for (int k = 0; k < S::kCols; ++k)
-        bias[k] = e.bias && wide ? e.bias[col + k] : 0.0f;
-
-    uint32_t v[32];
-    tmem_ld32_nowait(taddr, v);
-    tmem_wait_ld();
-    after();
-#pragma unroll
-    for (int q = 0; q < 8; ++q)
-        turn[lane * 8 + (q ^ (lane & 7))] = make_float4(__uint_as_float(v[4 * q]), __uint_as_float(v[4 * q + 1]),
-                                                        __uint_as_float(v[4 * q + 2]), __uint_as_float(v[4 * q + 3]));
-    __syncwarp();
-    auto finish = [&](float sum, float b) {
-        const float t = fmaf(sum, e.alpha, b);
-        return t >= 0.0f ? t : t * e.slope;
-    };
-    if (__all_sync(0xFFFFFFFFu, wide)) {
-#pragma unroll
-        for (int i = 0; i < S::kRounds; ++i) {
-            const int r = sub + i * S::kCols;
-            const int q = (lane % S::kLanes) * (S::kCols / 4);
-            float f[S::kCols];
-#pragma unroll
-            for (int k = 0; k < S::kCols; k += 4) {
-                const float4 s = turn[r * 8 + ((q + k / 4) ^ (r & 7))];
-                f[k] = finish(s.x, bias[k]);
-                f[k + 1] = finish(s.y, bias[k + 1]);
-                f[k + 2] = finish(s.z, bias[k + 2]);
-                f[k + 3] = finish(s.w, bias[k + 3]);
-            }
-            const uint32_t u[4] = {res[i].x, res[i].y, res[i].z, res[i].w};
-            uint32_t o[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if constexpr (DT == kMxF32) {
-                    o[k] = __float_as_uint(f[k] + __uint_as_float(u[k]));
-                } else {
-                    float a, b;
-                    D::unpack(u[k], a, b);
-                    o[k] = D::pack2(f[2 * k] + a, f[2 * k + 1] + b);
-                }
-            }
-            if (row0 + r < e.M)
-                *reinterpret_cast<uint4*>(static_cast<T*>(e.y) + (row0 + r) * e.y_stride + col) =
-                    make_uint4(o[0], o[1], o[2], o[3]);
-        }
-    } else if (col0 + lane < e.N) {
-        // off 16-byte boundaries or at the last columns: a lane takes a column
-        const float b = e.bias ? e.bias[col0 + lane] : 0.0f;
-        const float* sums = reinterpret_cast<const float*>(turn);
-        const int rows = static_cast<int>(min(e.M - row0, 32ll));
-        T* y = static_cast<T*>(e.y) + row0 * e.y_stride + col0 + lane;
-        const T* from = static_cast<const T*>(e.residual) + row0 * e.residual_stride + col0 + lane;
-#pragma unroll 8
-        for (int r = 0; r < rows; ++r) {
-            float f = finish(sums[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)], b);
-            if (e.residual)
-                f += D::load(from + r * e.residual_stride);
-            y[r * e.y_stride] = D::pack(f);
-        }
-    }
-    __syncwarp();
+    uint4 v;
+    asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ void store16(void* p, const uint4& v)
+{
+    asm volatile("st.global.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-template <typename After>
-__device__ __forceinline__ void mx_empty(const MxEpilogue& e, float4* turn, uint32_t taddr, long long row0, int col0,
-                                         After&& after)
+// A lane's part of 32 rows of y: a piece of 16 bytes (kCols columns) of each
+// kCols-th row.  Warps work alone here, so what a chunk waits for one after the
+// other is what it takes: addresses are made once for the rows, and all that a
+// chunk reads is asked for before any of it is used.
+template <int DT>
+struct MxOut {
+    using D = Dense<DT>;
+    using T = typename D::T;
+    static constexpr int kCols = DT == kMxF32 ? 4 : 8;
+    static constexpr int kLanes = 32 / kCols;  // of a row
+    static constexpr int kRounds = kLanes;     // each of kCols rows
+
+    struct Asked {  // what a chunk needs from memory
+        uint4 res[kRounds];
+        float bias[kCols];
+    };
+
+    T* y;
+    const T* res;
+    long long y_step, res_step;  // bytes
+    uint32_t there;              // bit i: the row of round i exists
+    long long row0;
+    int rows;
+
+    // Rows row0 .. row0 + 32, none from `end` on.
+    __device__ __forceinline__ void set_rows(const MxEpilogue& e, long long first, long long end)
+    {
+        const int sub = (threadIdx.x & 31) / kLanes;
+        row0 = first;
+        rows = static_cast<int>(max(min(end - first, 32ll), 0ll));
+        y = static_cast<T*>(e.y) + (first + sub) * e.y_stride;
+        res = static_cast<const T*>(e.residual) + (first + sub) * e.residual_stride;
+        y_step = e.y_stride * (kCols * static_cast<long long>(sizeof(T)));
+        res_step = e.residual_stride * (kCols * static_cast<long long>(sizeof(T)));
+        there = 0;
+#pragma unroll
+        for (int i = 0; i < kRounds; ++i)
+            there |= (sub + i * kCols < rows ? 1u : 0u) << i;
+    }
+
+    __device__ __forceinline__ void ask(const MxEpilogue& e, int col0, Asked& a) const
+    {
+        const int col = col0 + (threadIdx.x & 31) % kLanes * kCols;
+        const bool wide = e.vec && col + kCols <= e.N;
+        const uint8_t* from = reinterpret_cast<const uint8_t*>(res + col);
+#pragma unroll
+        for (int i = 0; i < kRounds; ++i, from += res_step)
+            a.res[i] = e.residual && wide && (there >> i & 1u) ? load16(from) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int k = 0; k < kCols; k += 4) {
+            const uint4 b = e.bias && wide ? load16(e.bias + col + k) : make_uint4(0, 0, 0, 0);
+            a.bias[k] = __uint_as_float(b.x);
+            a.bias[k + 1] = __uint_as_float(b.y);
+            a.bias[k + 2] = __uint_as_float(b.z);
+            a.bias[k + 3] = __uint_as_float(b.w);
+        }
+    }
+
+    // The chunk at `taddr` to columns col0 ...; `after` is called once the sums
+    // are in registers.
+    template <typename After>
+    __device__ __forceinline__ void empty(const MxEpilogue& e, const Asked& a, float4* turn, uint32_t taddr, int col0,
+                                          After&& after) const
+    {
+        const int lane = threadIdx.x & 31;
+        const int col = col0 + lane % kLanes * kCols, sub = lane / kLanes;
+        uint32_t v[32];
+        tmem_ld32_nowait(taddr, v);
+        tmem_wait_ld();
+        after();
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            turn[lane * 8 + (q ^ (lane & 7))] = make_float4(__uint_as_float(v[4 * q]), __uint_as_float(v[4 * q + 1]),
+                                                            __uint_as_float(v[4 * q + 2]), __uint_as_float(v[4 * q + 3]));
+        __syncwarp();
+        auto finish = [&](float sum, float b) {
+            const float t = fmaf(sum, e.alpha, b);
+            return t >= 0.0f ? t : t * e.slope;
+        };
+        if (__all_sync(0xFFFFFFFFu, e.vec && col + kCols <= e.N)) {
+            float f[kRounds][kCols];
+#pragma unroll
+            for (int i = 0; i < kRounds; ++i) {
+                const int r = sub + i * kCols, q = lane % kLanes * (kCols / 4);
+#pragma unroll
+                for (int k = 0; k < kCols; k += 4) {
+                    const float4 s = turn[r * 8 + ((q + k / 4) ^ (r & 7))];
+                    f[i][k] = s.x;
+                    f[i][k + 1] = s.y;
+                    f[i][k + 2] = s.z;
+                    f[i][k + 3] = s.w;
+                }
+            }
+            uint8_t* to = reinterpret_cast<uint8_t*>(y + col);
+#pragma unroll
+            for (int i = 0; i < kRounds; ++i, to += y_step) {
+#pragma unroll
+                for (int k = 0; k < kCols; ++k)
+                    f[i][k] = finish(f[i][k], a.bias[k]);
+                const uint32_t u[4] = {a.res[i].x, a.res[i].y, a.res[i].z, a.res[i].w};
+                uint32_t o[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if constexpr (DT == kMxF32) {
+                        o[k] = __float_as_uint(f[i][k] + __uint_as_float(u[k]));
+                    } else {
+                        float r0, r1;
+                        D::unpack(u[k], r0, r1);
+                        o[k] = D::pack2(f[i][2 * k] + r0, f[i][2 * k + 1] + r1);
+                    }
+                }
+                if (there >> i & 1u)
+                    store16(to, make_uint4(o[0], o[1], o[2], o[3]));
+            }
+        } else if (col0 + lane < e.N) {
+            // off 16-byte boundaries or at the last columns: a lane takes a column
+            const float b = e.bias ? e.bias[col0 + lane] : 0.0f;
+            const float* sums = reinterpret_cast<const float*>(turn);
+            T* to = static_cast<T*>(e.y) + row0 * e.y_stride + col0 + lane;
+            const T* from = static_cast<const T*>(e.residual) + row0 * e.residual_stride + col0 + lane;
+#pragma unroll 8
+            for (int r = 0; r < rows; ++r) {
+                float g = finish(sums[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)], b);
+                if (e.residual)
+                    g += D::load(from + r * e.residual_stride);
+                to[r * e.y_stride] = D::pack(g);
+            }
+        }
+        __syncwarp();
+    }
+};
+
+template <int DT>
+struct MxType {
+    static constexpr int value = DT;
+};
+
+// fn(MxType<DT>) of y's type.
+template <typename Fn>
+__device__ __forceinline__ void mx_by_type(int y_dtype, Fn&& fn)
 {
-    if (e.y_dtype == kMxF16)
-        mx_empty_chunk<kMxF16>(e, turn, taddr, row0, col0, after);
-    else if (e.y_dtype == kMxBf16)
-        mx_empty_chunk<kMxBf16>(e, turn, taddr, row0, col0, after);
+    if (y_dtype == kMxF16)
+        fn(MxType<kMxF16>{});
+    else if (y_dtype == kMxBf16)
+        fn(MxType<kMxBf16>{});
     else
-        mx_empty_chunk<kMxF32>(e, turn, taddr, row0, col0, after);
+        fn(MxType<kMxF32>{});
 }
 
 }  // namespace mlvc_b200

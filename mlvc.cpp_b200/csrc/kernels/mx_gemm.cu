@@ -183,23 +183,32 @@ __device__ __forceinline__ void mx_gemm(const MxGemmParams& p)
     } else {
         const int quadrant = warp & 3, group = (warp - 2) / 4;
         float4* turn = reinterpret_cast<float4*>(stages + T::kStages * T::kStage + (warp - 2) * kMxTurnBytes);
-        uint32_t acc = 0, acc_phase = 0;
-        for (int t = blockIdx.x; t < total; t += gridDim.x) {
-            int mt, nt;
-            mx_tile_at(p.m_tiles, p.n_tiles, t, mt, nt);
-            // the whole warp goes on or none of it: the TMEM loads are collective
-            if (!__all_sync(0xFFFFFFFFu, mbar_wait(&sh->tmem_full[acc], acc_phase, &sh->abort_flag, kErrMxEpilogue)))
-                break;
-            tc_fence_after();
-            for (int c = group * 32; c < BN; c += 64) {
-                mx_empty(p.e, turn, tmem + acc * BN + c + (static_cast<uint32_t>(quadrant * 32) << 16),
-                         static_cast<long long>(mt) * 128 + quadrant * 32, nt * BN + c, [] {});
+        mx_by_type(p.e.y_dtype, [&](auto type) {
+            using Out = MxOut<decltype(type)::value>;
+            Out out;
+            uint32_t acc = 0, acc_phase = 0;
+            for (int t = blockIdx.x; t < total; t += gridDim.x) {
+                int mt, nt;
+                mx_tile_at(p.m_tiles, p.n_tiles, t, mt, nt);
+                out.set_rows(p.e, static_cast<long long>(mt) * 128 + quadrant * 32, p.e.M);
+                typename Out::Asked asked;
+                out.ask(p.e, nt * BN + group * 32, asked);
+                // the whole warp goes on or none of it: the TMEM loads are collective
+                if (!__all_sync(0xFFFFFFFFu, mbar_wait(&sh->tmem_full[acc], acc_phase, &sh->abort_flag, kErrMxEpilogue)))
+                    break;
+                tc_fence_after();
+                for (int c = group * 32; c < BN; c += 64) {
+                    if (c >= 64)
+                        out.ask(p.e, nt * BN + c, asked);
+                    out.empty(p.e, asked, turn, tmem + acc * BN + c + (static_cast<uint32_t>(quadrant * 32) << 16), nt * BN + c,
+                              [] {});
+                }
+                tc_fence_before();
+                mbar_arrive(&sh->tmem_empty[acc]);
+                acc ^= 1u;
+                acc_phase ^= acc == 0;
             }
-            tc_fence_before();
-            mbar_arrive(&sh->tmem_empty[acc]);
-            acc ^= 1u;
-            acc_phase ^= acc == 0;
-        }
+        });
         __syncwarp();
     }
     if (issuer && sh->abort_flag && issued) {  // MMAs in flight end before TMEM is freed

@@ -9,3 +9,4 @@ extern "C" __device__ unsigned long long mlvc_b200_wait_limit_ns = mlvc_b200::kW
 #include "mx_gemm.cu"
 #include "mx_pair.cu"
 #include "mx_rows.cu"
+#include "mx_tall.cu"

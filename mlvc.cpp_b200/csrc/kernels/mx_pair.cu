@@ -180,30 +180,38 @@ __device__ __forceinline__ void mx_pair(const MxPairParams& p)
         const int quadrant = warp & 3, group = (warp - 2) / 4;
         const uint32_t out = cluster_address(&sh->shared_out, 0);
         float4* turn = reinterpret_cast<float4*>(stages + T::kStages * T::kStage + (warp - 2) * kMxTurnBytes);
-        uint32_t tile = 0;
-        for (int t = pair_id; t < total; t += pairs, ++tile) {
-            int mt, nt;
-            mx_tile_at(p.m_tiles, p.n_tiles, t, mt, nt);
-            // the whole warp goes on or none of it: the TMEM loads are collective
-            if (!__all_sync(0xFFFFFFFFu, mbar_wait(&sh->sums, tile & 1u, &sh->abort_flag, kErrMxEpilogue)))
-                break;
-            tc_fence_after();
-            const long long row = static_cast<long long>(mt) * 256 + rank * 128 + quadrant * 32;
-            const int odd = tile & 1u;
-            for (int c = 0; c < 4; ++c) {
-                // the shared columns 192..255 first
-                const int at = c == 0 ? 192 + 32 * group : (odd ? 256 : 0) + 96 * group + 32 * (c - 1);
-                mx_empty(p.e, turn, tmem + at + (static_cast<uint32_t>(quadrant * 32) << 16), row, nt * 256 + at - (odd ? 192 : 0),
-                         [&] {
-                             if (c == 0) {
-                                 tc_fence_before();
-                                 __syncwarp();
-                                 if (lane == 0)
-                                     mbar_arrive_cluster(out);
-                             }
-                         });
+        mx_by_type(p.e.y_dtype, [&](auto type) {
+            using Out = MxOut<decltype(type)::value>;
+            Out rows;
+            uint32_t tile = 0;
+            for (int t = pair_id; t < total; t += pairs, ++tile) {
+                int mt, nt;
+                mx_tile_at(p.m_tiles, p.n_tiles, t, mt, nt);
+                const bool odd = tile & 1u;
+                const int col0 = nt * 256 - (odd ? 192 : 0);  // of TMEM column 0
+                rows.set_rows(p.e, static_cast<long long>(mt) * 256 + rank * 128 + quadrant * 32, p.e.M);
+                typename Out::Asked asked;
+                rows.ask(p.e, col0 + 192 + 32 * group, asked);
+                // the whole warp goes on or none of it: the TMEM loads are collective
+                if (!__all_sync(0xFFFFFFFFu, mbar_wait(&sh->sums, tile & 1u, &sh->abort_flag, kErrMxEpilogue)))
+                    break;
+                tc_fence_after();
+                for (int c = 0; c < 4; ++c) {
+                    // the shared columns 192..255 first
+                    const int at = c == 0 ? 192 + 32 * group : (odd ? 256 : 0) + 96 * group + 32 * (c - 1);
+                    if (c)
+                        rows.ask(p.e, col0 + at, asked);
+                    rows.empty(p.e, asked, turn, tmem + at + (static_cast<uint32_t>(quadrant * 32) << 16), col0 + at, [&] {
+                        if (c == 0) {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0)
+                                mbar_arrive_cluster(out);
+                        }
+                    });
+                }
             }
-        }
+        });
         __syncwarp();
     }
     if (issuer && sh->abort_flag && issued) {  // MMAs in flight end before TMEM is freed

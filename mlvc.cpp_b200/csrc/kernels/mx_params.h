@@ -54,7 +54,7 @@ struct MxEpilogue {
     void* y;
     long long y_stride;
     int y_dtype;
-    int vec;                           // y and residual rows begin on 16-byte boundaries
+    int vec;                           // rows of y and residual, and bias, begin on 16-byte boundaries
     float alpha, slope;
 };
 
@@ -86,6 +86,21 @@ struct MxPairParams {
     int m_tiles, n_tiles;
     MxEpilogue e;
 };
+
+// Many dense rows with few values each (see mx_tall).
+struct MxTallParams {
+    CUtensorMap map_w;                 // weights, boxes of 128 bytes x 64 rows
+    const uint8_t* scales_w;
+    MxPanels k;
+    int n_tiles;                       // of 64 columns
+    int tile_rows;                     // of a CTA, at most 128
+    const void* x;
+    long long row_stride, col_stride;
+    int cols, vec;
+    float tensor_scale, inv_six_scale;
+    MxEpilogue e;
+};
+constexpr int kMxTallScaleTiles = 16;   // of a row at most: their TMEM columns
 
 // Products of few rows (see mx_rows): weights are the tensor core's first
 // operand, rows its second.

@@ -20,7 +20,7 @@
 // other, about 150 cycles a turn.
 //
 // Warps: 0 copies, 1 MMA and TMEM, 2..9 quantise and then finish the sums.
-#include "mx.cuh"
+#include "mx_epilogue.cuh"
 
 namespace mlvc_b200 {
 
@@ -60,11 +60,6 @@ __device__ __forceinline__ void mx_finish_one(const MxEpilogue& e, int m, int n,
         v += Dense<DT>::load(static_cast<const T*>(e.residual) + m * e.residual_stride + n);
     static_cast<T*>(e.y)[m * e.y_stride + n] = Dense<DT>::pack(v);
 }
-
-template <int DT>
-struct MxType {
-    static constexpr int value = DT;
-};
 
 // DT < 0: x is already quantised.
 template <int F, int DT>
@@ -353,14 +348,8 @@ __device__ __forceinline__ void mx_rows(const MxRowsParams& p)
                         mx_finish_one<decltype(type)::value>(p.e, m0 + j, n0 + 32 * i + lane, sum[i]);
             }
         };
-        if (all) {
-            if (p.e.y_dtype == kMxF16)
-                finish(MxType<kMxF16>{});
-            else if (p.e.y_dtype == kMxBf16)
-                finish(MxType<kMxBf16>{});
-            else
-                finish(MxType<kMxF32>{});
-        }
+        if (all)
+            mx_by_type(p.e.y_dtype, finish);
         __syncwarp();
     }
     if (p.splits > 1 && warp < 2)

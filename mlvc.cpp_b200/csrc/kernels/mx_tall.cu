@@ -1,0 +1,233 @@
+// Many dense rows with few values each: the codec's 1x1 convolutions, whose rows
+// are the pixels of a plane.
+//     y = leaky(quantise(x) . w^T + bias) + residual
+//
+// Memory bounds these calls: x, the residual and y, each once; the products of
+// one or two panels are nothing beside them.  So one kernel does all of it, in
+// CTAs that are small enough for two to share an SM, each a step further or
+// behind the other: eight warps load up to 128 rows and quantise them into the
+// swizzled panels and scale tiles that the tensor core reads; then a ninth issues
+// the products of 64 columns after another into two accumulators in turn, and
+// the eight empty them.  (With warps that only quantise, multiply or empty, one
+// CTA an SM, the 240 x 136 x 256 plane took 18.5 us: too few warps at each of
+// the steps.)
+#include "mx_epilogue.cuh"
+
+namespace mlvc_b200 {
+
+constexpr int kMxTallThreads = 288;
+constexpr int kMxTallWorkers = 256;
+
+struct MxTallShared {
+    uint64_t weights[2];
+    uint64_t rows;        // quantised
+    uint64_t sums[2], emptied[2];
+    uint64_t drain;
+    uint32_t tmem_base;
+    int abort_flag;
+};
+
+template <int F, int DT>
+__device__ __forceinline__ void mx_tall(const MxTallParams& p)
+{
+    constexpr int kWords = Mx<F>::kWords;
+    constexpr uint32_t kPanel = 128 * 128, kWeights = 64 * 128;  // of a panel
+    constexpr uint32_t kTmemCols = 256;  // 64 sums twice, then x's scales and the weights'
+    static_assert(128 + 2 * 4 * kMxTallScaleTiles <= kTmemCols, "TMEM");
+    extern __shared__ __align__(1024) uint8_t smem_dyn[];
+    uint8_t* base = align_smem_1024(smem_dyn);
+    MxTallShared* sh = reinterpret_cast<MxTallShared*>(base);
+    const int warp = threadIdx.x / 32, t = threadIdx.x;
+    const int panels = p.k.count;
+    const uint32_t scale_bytes = static_cast<uint32_t>(p.k.k_tiles) * 512u;  // of 128 rows
+    const uint32_t w_bytes = panels * kWeights, w_stage = w_bytes + (scale_bytes + 1023) / 1024 * 1024;
+    uint8_t* a_tiles = base + 1024;
+    uint8_t* w_stages = a_tiles + panels * kPanel;  // weights and their scales of 64 columns, two in turn
+    uint8_t* a_scales = w_stages + 2 * w_stage;
+    float4* turn = reinterpret_cast<float4*>(a_scales + panels * kWords * 512) + warp * (kMxTurnBytes / 16);
+    if (t == 0) {
+        mbar_init(&sh->weights[0], 1);
+        mbar_init(&sh->weights[1], 1);
+        mbar_init(&sh->rows, kMxTallWorkers);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh->sums[i], 1);
+            mbar_init(&sh->emptied[i], kMxTallWorkers);
+        }
+        mbar_init(&sh->drain, 1);
+        sh->abort_flag = 0;
+        fence_barrier_init();
+    }
+    pdl_wait();
+    // TMEM is taken once the kernel before has ended (see mx_gemm)
+    if (warp == 8)
+        tmem_alloc(&sh->tmem_base, kTmemCols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    pdl_launch_dependents();
+    const uint32_t tmem = sh->tmem_base;
+    const long long first = static_cast<long long>(blockIdx.x) * p.tile_rows;
+    const int rows = static_cast<int>(min(static_cast<long long>(p.tile_rows), p.e.M - first));
+
+    if (warp == 8) {
+        if (elect_one()) {
+            uint32_t issued = 0;
+            int loaded = 0;
+            auto load_weights = [&] {  // the next 64 columns'
+                const int n = loaded++;
+                uint8_t* s = w_stages + (n & 1) * w_stage;
+                mbar_arrive_expect_tx(&sh->weights[n & 1], w_bytes + scale_bytes);
+                for (int k = 0; k < panels; ++k)
+                    tma_load_2d(s + k * kWeights, &p.map_w, &sh->weights[n & 1], k * 128, n * 64);
+                bulk_load(s + w_bytes, p.scales_w + static_cast<long long>(n / 2) * scale_bytes, scale_bytes, &sh->weights[n & 1]);
+            };
+            load_weights();
+            if (p.n_tiles > 1)
+                load_weights();
+            constexpr uint32_t idesc = mx_idesc<F>(128, 64);
+            const uint32_t tmem_sa = tmem + 128, tmem_sb = tmem_sa + 4 * kMxTallScaleTiles;
+            const uint64_t a = smem_desc(smem_u32(a_tiles), 16, 1024, 2), sa = smem_desc(smem_u32(a_scales), 16, 128, 0);
+            bool ok = mbar_wait(&sh->rows, 0, &sh->abort_flag, kErrMxMma);
+            for (int n = 0; ok && n < p.n_tiles; ++n) {
+                const uint32_t phase = (n >> 1) & 1u;
+                ok = mbar_wait(&sh->weights[n & 1], phase, &sh->abort_flag, kErrMxMma) &&
+                     mbar_wait(&sh->emptied[n & 1], phase ^ 1u, &sh->abort_flag, kErrMxMma);
+                if (!ok)
+                    break;
+                tc_fence_after();
+                const uint32_t s = smem_u32(w_stages) + (n & 1) * w_stage, sums = tmem + 64 * (n & 1);
+                const uint64_t b = smem_desc(s, 16, 1024, 2), sw = smem_desc(s + w_bytes, 16, 128, 0);
+                const uint32_t in_band = (n & 1) * 2;  // 64 weights are half of a scale tile's rows
+                for (int w = 0; w < p.k.k_tiles; ++w) {
+                    if (n == 0)
+                        tmem_copy_scales(tmem_sa + 4 * w, sa + 32 * w);
+                    tmem_copy_scales(tmem_sb + 4 * w, sw + 32 * w);
+                }
+                for (int k = 0; k < panels; ++k) {
+                    const int steps = k + 1 == panels ? p.k.last_steps : 4;
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks) {
+                        if (ks >= steps)
+                            break;
+                        const uint32_t w = k * kWords + ks * kWords / 4, id = kWords == 4 ? 0 : kWords == 2 ? (ks & 1) * 2 : ks;
+                        umma_mx<F>(sums, a + k * (kPanel >> 4) + 2 * ks, b + k * (kWeights >> 4) + 2 * ks, idesc, id,
+                                   tmem_sa + 4 * w, tmem_sb + 4 * w + in_band, (k | ks) != 0);
+                        ++issued;
+                    }
+                }
+                umma_commit(&sh->sums[n & 1]);
+                // the weights before these have been used once their sums are complete
+                if (n && loaded < p.n_tiles) {
+                    ok = mbar_wait(&sh->sums[(n - 1) & 1], ((n - 1) >> 1) & 1u, &sh->abort_flag, kErrMxMma);
+                    if (ok)
+                        load_weights();
+                }
+            }
+            if (sh->abort_flag) {  // nothing may land or run after this CTA has gone
+                volatile int never = 0;
+                for (int n = max(loaded - 2, 0); n < loaded; ++n)
+                    mbar_wait(&sh->weights[n & 1], (n >> 1) & 1u, &never, kErrMxProducer);
+                if (issued) {
+                    umma_commit(&sh->drain);
+                    mbar_wait(&sh->drain, 0, &never, kErrMxMma);
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        // x: the chunks that the products read, four of a thread (FP32: two) under way
+        // at once
+        {
+            constexpr int kChunks = Mx<F>::kPanelValues / 16;  // of a panel
+            constexpr int kBatch = DT == kMxF32 ? 2 : 4;
+            const int row_chunks = (panels - 1) * kChunks + p.k.last_steps * (kChunks / 4);
+            const int items = rows * row_chunks;
+            const typename Dense<DT>::T* dense = static_cast<const typename Dense<DT>::T*>(p.x) + first * p.row_stride;
+            const int step_m = kMxTallWorkers / row_chunks, step_c = kMxTallWorkers - step_m * row_chunks;
+            int m = t / row_chunks, c = t - m * row_chunks;
+#pragma unroll 1
+            for (int i0 = t; i0 < ((items + 31) & ~31); i0 += kMxTallWorkers * kBatch) {
+                Raw<DT> x[kBatch];
+                int at_m[kBatch], at_c[kBatch];
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b) {
+                    at_m[b] = m;
+                    at_c[b] = c;
+                    if (m < rows)
+                        load_raw<DT>(dense + m * p.row_stride, p.col_stride, c * 16, p.cols, p.vec, x[b]);
+                    else
+                        x[b] = Raw<DT>{};
+                    m += step_m;
+                    c += step_c;
+                    if (c >= row_chunks) {
+                        c -= row_chunks;
+                        ++m;
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b) {
+                    uint32_t codes[4], scale;
+                    quantise_chunk<F, DT>(x[b], p.tensor_scale, p.inv_six_scale, codes, scale);
+                    if (at_m[b] < rows) {
+                        const int panel = at_c[b] / kChunks, in = at_c[b] % kChunks, r = at_m[b];
+                        const int byte = in * Mx<F>::kChunkBytes;
+                        uint8_t* to = a_tiles + panel * kPanel + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15);
+                        if constexpr (Mx<F>::kIs8)
+                            *reinterpret_cast<uint4*>(to) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+                        else
+                            *reinterpret_cast<uint2*>(to) = make_uint2(codes[0], codes[1]);
+                        const int column = Mx<F>::kIsNv ? in : in >> 1;
+                        if (Mx<F>::kIsNv || !(in & 1))
+                            a_scales[(panel * kWords + (column >> 2)) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (column & 3)] =
+                                static_cast<uint8_t>(scale);
+                    }
+                }
+            }
+        }
+        fence_proxy_async_smem();  // the tensor core reads through the async proxy
+        mbar_arrive(&sh->rows);
+        __syncwarp();
+        const int quadrant = warp & 3, group = warp / 4;
+        mx_by_type(p.e.y_dtype, [&](auto type) {
+            using Out = MxOut<decltype(type)::value>;
+            Out out;
+            out.set_rows(p.e, first + quadrant * 32, first + rows);
+#pragma unroll 1
+            for (int n = 0; n < p.n_tiles; ++n) {
+                const int col0 = n * 64 + group * 32;
+                typename Out::Asked asked;
+                out.ask(p.e, col0, asked);
+                // the whole warp goes on or none of it: the TMEM loads are collective
+                if (!__all_sync(0xFFFFFFFFu, mbar_wait(&sh->sums[n & 1], (n >> 1) & 1u, &sh->abort_flag, kErrMxEpilogue)))
+                    break;
+                tc_fence_after();
+                out.empty(p.e, asked, turn, tmem + 64 * (n & 1) + group * 32 + (static_cast<uint32_t>(quadrant * 32) << 16), col0, [&] {
+                    tc_fence_before();
+                    mbar_arrive(&sh->emptied[n & 1]);
+                });
+            }
+        });
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kTmemCols);
+    }
+}
+
+// Two CTAs an SM have to be asked for (see mx_rows).
+#define MLVC_MX_TALL(NAME, F, DT)                                                                              \
+    extern "C" __global__ void __launch_bounds__(kMxTallThreads, 2) NAME(const __grid_constant__ MxTallParams p) \
+    {                                                                                                          \
+        mx_tall<F, DT>(p);                                                                                     \
+    }
+#define MLVC_MX_TALL_ALL(FN, F)                      \
+    MLVC_MX_TALL(mlvc_mx_tall_f16_##FN, F, kMxF16)   \
+    MLVC_MX_TALL(mlvc_mx_tall_bf16_##FN, F, kMxBf16) \
+    MLVC_MX_TALL(mlvc_mx_tall_f32_##FN, F, kMxF32)
+MLVC_MX_TALL_ALL(mxfp4, kMxFp4)
+MLVC_MX_TALL_ALL(nvfp4, kNvFp4)
+MLVC_MX_TALL_ALL(mxfp8, kMxFp8)
+
+}  // namespace mlvc_b200

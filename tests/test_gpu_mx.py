@@ -205,6 +205,52 @@ def test_linear(be, fmt, shape):
     assert torch.equal(y, z)
 
 
+LARGE = [  # rows, inputs, outputs: enough rows and outputs for the wider tiles
+    (600, 520, 3000), (2500, 300, 2600), (2305, 1025, 2563), (14300, 200, 70), (14500, 64, 257), (32640, 256, 256),
+    (19000, 100, 64),
+]
+
+
+@pytest.mark.parametrize("shape", LARGE)
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_linear_large(be, fmt, shape):
+    m, k, n = shape
+    rng = np.random.default_rng(m + n)
+    names = list(DTYPES)
+    dtype, out = names[(m + k) % 3], names[(m + n) % 3]
+    x, w = rows(rng, m, k, dtype, 0.1).cuda(), rows(rng, n, k, "f32", 0.1).cuda()
+    bias = torch.from_numpy(rng.standard_normal(n).astype(np.float32)).cuda()
+    residual = rows(rng, m, n, out).cuda()
+    gx, gw = scale_of(fmt), scale_of(fmt) / 4 if fmt == "nvfp4" else 1.0
+    layer = MxLinear(be, quantised(be, w, fmt, gw), bias=bias, slope=0.25, tensor_scale=gx)
+    y = torch.full((m, n), float("nan"), dtype=DTYPES[out], device="cuda")
+    layer(x, y, residual=residual, workspace=alloc(layer.workspace_bytes(m)), stream=0)
+    check_linear(y, x, w, fmt, gx, gw, out, bias, 0.25, residual)
+    z = torch.full((m, n), float("nan"), dtype=DTYPES[out], device="cuda")
+    layer(quantised(be, x, fmt, gx), z, residual=residual, stream=0)
+    check_linear(z, x, w, fmt, gx, gw, out, bias, 0.25, residual)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_linear_large_strides(be, fmt):
+    """Many rows, as parts of wider matrices, on and off wide boundaries; nothing
+    beside y is written."""
+    rng = np.random.default_rng(8)
+    m, k, n = 14400, 96, 72
+    g = scale_of(fmt)
+    w = rows(rng, n, k, "f32", 0.1).cuda()
+    layer = MxLinear(be, quantised(be, w, fmt), tensor_scale=g)
+    xs = rows(rng, m, 150, "bf16", 0.1).cuda()
+    for at, y_at in ((0, 0), (32, 16), (3, 5)):
+        x = xs[:, at:at + k]
+        base = torch.full((m + 1, 160), 3.0, dtype=torch.bfloat16, device="cuda")
+        y = base[:m, y_at:y_at + n]
+        layer(x, y, workspace=alloc(layer.workspace_bytes(m)), stream=0)
+        check_linear(y, x, w, fmt, g, g, "bf16")
+        y.fill_(3.0)
+        assert bool((base == 3.0).all())
+
+
 @pytest.mark.parametrize("rows_", [1, 5, 20, 64, 150, 700])
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_linear_strides(be, fmt, rows_):
