@@ -151,6 +151,7 @@ class Backend:
         if debug_tensors:
             _check(lib().mlvc_b200_set_debug_tensors(self._h, 1))
         self._in, self._out = [], []
+        self._calls = mx.Calls()
 
     def close(self):
         if self._h:
@@ -268,30 +269,41 @@ class Backend:
         _check(lib().mlvc_b200_integer_values_device(self._h, values_ptr, count, symbols_ptr, out_of_range_ptr))
 
     # ------------------------------------------------------ microscaled
-    def _mx(self, fn, *args, stream):
-        _check(fn(self._h, *args, self.stream or 0 if stream is None else stream))
-
     def mx_quantise(self, x, out, stream=None):
         """Quantises the dense matrix x into the MxMatrix `out` of its shape."""
-        self._mx(lib().mlvc_b200_mx_quantise, ctypes.byref(mx._fill(mx.Matrix(), x)), ctypes.byref(out.c), stream=stream)
+        c = self._calls
+        mx._fill(c.matrix, x)
+        if _lib.mlvc_b200_mx_quantise(self._h, c.matrix_ref, out.ref, self.stream or 0 if stream is None else stream):
+            _check(-1)
 
     def mx_dequantise(self, m, y, stream=None):
         """Reads the MxMatrix m back into the dense matrix y of its shape."""
-        self._mx(lib().mlvc_b200_mx_dequantise, ctypes.byref(m.c), ctypes.byref(mx._fill(mx.Matrix(), y)), stream=stream)
+        c = self._calls
+        mx._fill(c.matrix, y)
+        if _lib.mlvc_b200_mx_dequantise(self._h, m.ref, c.matrix_ref, self.stream or 0 if stream is None else stream):
+            _check(-1)
 
     def mx_cache_write(self, cache, x, pages, offsets, starts=None, stream=None):
         """Quantises the packed rows of several sequences into their places:
         rows offsets[s] .. offsets[s + 1] of x become positions starts[s] ... of
         sequence s, whose pages are pages[s] (device int32 arrays [sequences,
         pages], [sequences + 1], [sequences]; starts None: all zero)."""
-        self._mx(lib().mlvc_b200_mx_cache_write, ctypes.byref(cache.c), ctypes.byref(mx._fill(mx.Matrix(), x)),
-                 ctypes.byref(mx.rows_of(pages, offsets, starts)), stream=stream)
+        c = self._calls
+        mx._fill(c.matrix, x)
+        mx._fill_rows(c.rows, pages, offsets, starts)
+        if _lib.mlvc_b200_mx_cache_write(self._h, cache.ref, c.matrix_ref, c.rows_ref,
+                                         self.stream or 0 if stream is None else stream):
+            _check(-1)
 
     def mx_cache_read(self, cache, y, pages, offsets, starts=None, stream=None):
         """Reads packed rows back into the dense matrix y, addressed as in
         mx_cache_write; rows that have no place are zeros."""
-        self._mx(lib().mlvc_b200_mx_cache_read, ctypes.byref(cache.c), ctypes.byref(mx._fill(mx.Matrix(), y)),
-                 ctypes.byref(mx.rows_of(pages, offsets, starts)), stream=stream)
+        c = self._calls
+        mx._fill(c.matrix, y)
+        mx._fill_rows(c.rows, pages, offsets, starts)
+        if _lib.mlvc_b200_mx_cache_read(self._h, cache.ref, c.matrix_ref, c.rows_ref,
+                                        self.stream or 0 if stream is None else stream):
+            _check(-1)
 
     # ----------------------------------------------------------- slots
     def configure_slots(self, n):

@@ -22,6 +22,7 @@ non-finite values and cache rows without a place hold here too:
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import NamedTuple
 
 FORMATS = {"mxfp4": 0, "nvfp4": 1, "mxfp8": 2}
@@ -74,13 +75,16 @@ EXPORTS = {
 
 
 def _code(dtype):
-    code = _dtype_codes.get(dtype)
+    code = _DTYPES.get(str(dtype).rsplit(".", 1)[-1])
     if code is None:
-        code = _DTYPES.get(str(dtype).rsplit(".", 1)[-1])
-        if code is None:
-            raise RuntimeError(f"mlvc-b200: a dense matrix is float16, bfloat16 or float32, not {dtype}")
-        _dtype_codes[dtype] = code
+        raise RuntimeError(f"mlvc-b200: a dense matrix is float16, bfloat16 or float32, not {dtype}")
+    _dtype_codes[dtype] = code
     return code
+
+
+# A Matrix at once: a call on few rows takes little longer than its description.
+_pack_matrix = struct.Struct("=Qiiqqqq").pack_into
+_pack_rows = struct.Struct("=QqQQq").pack_into
 
 
 def _fill(m, t):
@@ -88,11 +92,10 @@ def _fill(m, t):
     shape = t.shape
     if len(shape) != 2:
         raise RuntimeError(f"mlvc-b200: a dense matrix has two dimensions, not {len(shape)}")
-    m.data = t.data_ptr()
-    m.dtype = _code(t.dtype)
-    m.rows, m.cols = shape
-    m.row_stride, m.col_stride = t.stride()
-    return m
+    code = _dtype_codes.get(t.dtype)
+    if code is None:
+        code = _code(t.dtype)
+    _pack_matrix(m, 0, t.data_ptr(), code, 0, *shape, *t.stride())
 
 
 def _format(name):
@@ -101,13 +104,17 @@ def _format(name):
     return FORMATS[name]
 
 
+_int32 = set()  # dtype objects known to be int32
+
+
 def _ints(t, what, dims):
-    """Address of a contiguous int32 device array (None: 0)."""
-    if t is None:
-        return 0
-    if str(t.dtype).rsplit(".", 1)[-1] != "int32" or len(t.shape) != dims or not t.is_contiguous():
+    """Shape of a contiguous int32 device array."""
+    shape = t.shape
+    if t.dtype not in _int32 and str(t.dtype).rsplit(".", 1)[-1] == "int32":
+        _int32.add(t.dtype)
+    if t.dtype not in _int32 or len(shape) != dims or not t.is_contiguous():
         raise RuntimeError(f"mlvc-b200: {what} must be a contiguous int32 array of {dims} dimension(s)")
-    return t.data_ptr()
+    return shape
 
 
 def _room(buffer, need, what):
@@ -124,22 +131,23 @@ class MxLayout(NamedTuple):
 
 def _layout(fn, *args):
     from . import _check, lib
-    out = [ctypes.c_size_t() for _ in range(3)]
-    _check(getattr(lib(), fn)(*args, *[ctypes.byref(o) for o in out]))
-    return MxLayout(*(o.value for o in out))
+    a, b, c = ctypes.c_size_t(), ctypes.c_size_t(), ctypes.c_size_t()
+    _check(getattr(lib(), fn)(*args, ctypes.byref(a), ctypes.byref(b), ctypes.byref(c)))
+    return MxLayout(a.value, b.value, c.value)
 
 
 class MxMatrix:
     """A quantised matrix [rows, cols] in the caller's buffers `data` and
     `scales` (objects with data_ptr(), at least layout()'s bytes each)."""
 
-    def __init__(self, format, rows, cols, data, scales, tensor_scale=1.0):
-        lay = self.layout(format, rows, cols)
+    def __init__(self, format, rows, cols, data, scales, tensor_scale=1.0, lay=None):
+        lay = lay or self.layout(format, rows, cols)
         _room(data, lay.data_bytes, "a quantised matrix's data")
         _room(scales, lay.scale_bytes, "a quantised matrix's scales")
         self.format, self.rows, self.cols, self.tensor_scale = format, int(rows), int(cols), float(tensor_scale)
         self.data, self.scales = data, scales
         self.c = MxMatrixC(_format(format), tensor_scale, rows, cols, data.data_ptr(), scales.data_ptr())
+        self.ref = ctypes.byref(self.c)
 
     @staticmethod
     def layout(format, rows, cols):
@@ -149,7 +157,7 @@ class MxMatrix:
     def allocate(cls, format, rows, cols, alloc, tensor_scale=1.0):
         """With buffers from alloc(bytes)."""
         lay = cls.layout(format, rows, cols)
-        return cls(format, rows, cols, alloc(lay.data_bytes), alloc(lay.scale_bytes), tensor_scale)
+        return cls(format, rows, cols, alloc(lay.data_bytes), alloc(lay.scale_bytes), tensor_scale, lay)
 
 
 class MxCache:
@@ -157,13 +165,14 @@ class MxCache:
     caller's buffers: of the features, keys or values of many sequences, whose
     pages a table names."""
 
-    def __init__(self, format, pages, page_rows, cols, data, scales, tensor_scale=1.0):
-        lay = self.layout(format, pages, page_rows, cols)
+    def __init__(self, format, pages, page_rows, cols, data, scales, tensor_scale=1.0, lay=None):
+        lay = lay or self.layout(format, pages, page_rows, cols)
         _room(data, lay.data_bytes, "a cache's data")
         _room(scales, lay.scale_bytes, "a cache's scales")
         self.format, self.pages, self.page_rows, self.cols = format, int(pages), int(page_rows), int(cols)
         self.tensor_scale, self.data, self.scales = float(tensor_scale), data, scales
         self.c = MxCacheC(_format(format), tensor_scale, pages, page_rows, cols, data.data_ptr(), scales.data_ptr())
+        self.ref = ctypes.byref(self.c)
 
     @staticmethod
     def layout(format, pages, page_rows, cols):
@@ -173,19 +182,26 @@ class MxCache:
     def allocate(cls, format, pages, page_rows, cols, alloc, tensor_scale=1.0):
         """With buffers from alloc(bytes)."""
         lay = cls.layout(format, pages, page_rows, cols)
-        return cls(format, pages, page_rows, cols, alloc(lay.data_bytes), alloc(lay.scale_bytes), tensor_scale)
+        return cls(format, pages, page_rows, cols, alloc(lay.data_bytes), alloc(lay.scale_bytes), tensor_scale, lay)
 
 
-def rows_of(pages, offsets, starts):
-    """The C description of where packed rows lie (see mlvc_b200_mx_rows)."""
-    r = MxRows()
-    r.pages = _ints(pages, "the page table", 2)
-    r.offsets = _ints(offsets, "offsets", 1)
-    r.starts = _ints(starts, "starts", 1)
-    r.sequences, r.pages_per_sequence = pages.shape
-    if offsets.shape[0] != r.sequences + 1 or (starts is not None and starts.shape[0] != r.sequences):
+def _fill_rows(r, pages, offsets, starts):
+    """Describes where packed rows lie (see mlvc_b200_mx_rows) in the structure `r`."""
+    sequences, per_sequence = _ints(pages, "the page table", 2)
+    if _ints(offsets, "offsets", 1)[0] != sequences + 1 or (starts is not None and
+                                                            _ints(starts, "starts", 1)[0] != sequences):
         raise RuntimeError("mlvc-b200: offsets has one entry more than there are sequences, starts as many")
-    return r
+    _pack_rows(r, 0, pages.data_ptr(), per_sequence, offsets.data_ptr(), 0 if starts is None else starts.data_ptr(),
+               sequences)
+
+
+class Calls:
+    """A backend's descriptions of the operands of a call, filled anew by each
+    (calls on one backend come from one host thread at a time)."""
+
+    def __init__(self):
+        self.matrix, self.rows = Matrix(), MxRows()
+        self.matrix_ref, self.rows_ref = ctypes.byref(self.matrix), ctypes.byref(self.rows)
 
 
 class MxLinear:
@@ -197,7 +213,7 @@ class MxLinear:
 
     def __init__(self, backend, weight, bias=None, slope=1.0, tensor_scale=1.0):
         from . import _check, lib
-        if bias is not None and (_code(bias.dtype) != 3 or tuple(bias.shape) != (weight.rows,) or
+        if bias is not None and (not str(bias.dtype).endswith("float32") or tuple(bias.shape) != (weight.rows,) or
                                  not bias.is_contiguous()):
             raise RuntimeError("mlvc-b200: bias must be a contiguous float32 vector, one value for each output")
         self._keep = (weight, bias)
@@ -207,7 +223,7 @@ class MxLinear:
         a.w = weight.c
         a.bias = bias.data_ptr() if bias is not None else 0
         a.slope, a.tensor_scale = slope, tensor_scale
-        self._x, self._y, self._residual = a.x, a.y, a.residual  # views
+        self._x, self._a, self._y, self._residual = a.x, a.a, a.y, a.residual  # views
         self._ref = ctypes.byref(a)
 
     def workspace_bytes(self, rows):
@@ -225,17 +241,18 @@ class MxLinear:
             a.a = x.c
             self._x.data = 0
         else:
-            a.a.data = 0
+            if self._a.data:
+                self._a.data = 0
             _fill(self._x, x)
         _fill(self._y, y)
-        if residual is None:
-            self._residual.data = 0
-        else:
+        if residual is not None:
             _fill(self._residual, residual)
-        if workspace is None:
-            a.workspace = a.workspace_bytes = 0
-        else:
+        elif self._residual.data:
+            self._residual.data = 0
+        if workspace is not None:
             a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.nbytes
+        elif a.workspace:
+            a.workspace = a.workspace_bytes = 0
         if self._call(self._backend._h, self._ref, self._backend.stream or 0 if stream is None else stream):
             self._check(-1)
         return y
