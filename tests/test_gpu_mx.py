@@ -451,3 +451,19 @@ def test_refusals_leave_the_backend_usable(be):
     with pytest.raises(RuntimeError, match="workspace must hold"):
         MxLinear(be, m)(x, torch.ones(4, 5, device="cuda"), stream=0)
     check_held(quantised(be, x, "mxfp4"), x, "mxfp4")
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_feature_streams_example(fmt):
+    """Read, two layers, write, frame after frame: no further from 32 bits than
+    the formats are.  E2M1: half the widest step is a sixth of a block's largest
+    value, which is about 2.5 times the root mean square of normal values, so
+    0.42 of it at most, and less after the sums over many values; E4M3: a
+    sixteenth of the value itself, twice, plus what saturates."""
+    import sys
+    from pathlib import Path
+    sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "examples"))
+    import mx_feature_streams
+    error, weights, ms = mx_feature_streams.run(fmt, streams=2, height=9, width=17, channels=96, hidden=160, frames=2, page_rows=16)
+    worst = {"mxfp4": 0.5, "nvfp4": 0.5, "mxfp8": 0.15}[fmt]
+    assert 0 < weights < worst and 0 < error < worst and ms > 0
