@@ -80,16 +80,19 @@ int64_t k_tiles_of(int format, int64_t cols) { return ceil_div(ceil_div(cols, bl
 // 1 / (6 g), rounded once.
 float inverse_six(float tensor_scale) { return static_cast<float>(1.0 / (6.0 * tensor_scale)); }
 
-// Rows are contiguous and every chunk of 16 values begins on a 32-byte
-// boundary, so that a lane moves its chunk with one (FP32: two) accesses.
+// Rows are contiguous and every chunk of 16 values begins on a 32-byte (1) or a
+// 16-byte (2) boundary, so that a lane moves its chunk as a whole; else 0.
 int wide(const MxDense& d)
 {
-    const uint64_t stride = static_cast<uint64_t>(d.row_stride) * elem_size(d.dtype);
-    return d.data % 32 == 0 && (d.rows <= 1 || stride % 32 == 0) && (d.col_stride == 1 || d.cols == 1);
+    const uint64_t at = d.data | (d.rows > 1 ? static_cast<uint64_t>(d.row_stride) * elem_size(d.dtype) : 0);
+    if (d.col_stride != 1 && d.cols > 1)
+        return 0;
+    return at % 32 == 0 ? 1 : at % 16 == 0 ? 2 : 0;
 }
 
-// Order of functions_: the four conversions by type and format, then products.
-enum { kQuantise = 0, kDequantise = 9, kCacheWrite = 18, kCacheRead = 27, kGemm64 = 36, kGemm128 = 39, kRows = 42, kPair = 54, kTall = 57, kFunctions = 66 };
+// Order of functions_: the four conversions by type and format, products, and
+// the conversions of rows that are not wide.
+enum { kQuantise = 0, kDequantise = 9, kCacheWrite = 18, kCacheRead = 27, kGemm64 = 36, kGemm128 = 39, kRows = 42, kPair = 54, kTall = 57, kAny = 66, kFunctions = 102 };
 
 int convert_index(int base, int dtype, int format) { return base + (dtype == kMxF16 ? 0 : dtype == kMxBf16 ? 3 : 6) + format; }
 
@@ -97,6 +100,8 @@ std::string function_name(int i)
 {
     static const char* const conversions[4] = {"quantise", "dequantise", "cache_write", "cache_read"};
     static const int types[3] = {kMxF16, kMxBf16, kMxF32};
+    if (i >= kAny)
+        return function_name(i - kAny) + "_any";
     if (i < kGemm64)
         return std::string("mlvc_mx_") + conversions[i / 9] + "_" + kTypeNames[types[i % 9 / 3]] + "_" + kFormatNames[i % 3];
     if (i >= kTall)
@@ -170,7 +175,7 @@ CUfunction Mx::fn(int index)
         const std::string name = function_name(index);
         CUfunction got = nullptr;
         check(cuModuleGetFunction(&got, module_, name.c_str()), name.c_str());
-        if (index >= kGemm64)
+        if (index >= kGemm64 && index < kAny)
             check(cuFuncSetAttribute(got, CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES, kGemmSmem), name.c_str());
         f = got;
     }
@@ -264,15 +269,17 @@ void Mx::convert(const MxDense& d, int format, float tensor_scale, uint64_t data
             p.segments = segments;
         }
     }
-    // up to four groups of rows a warp (FP32: two, they are twice the bytes),
+    // up to four groups of rows a warp (FP32 and rows off 32-byte boundaries: two),
     // fewer where that leaves SMs without work; the cache's kernels name a
     // warp's rows with its lanes, so 32 rows at most
     const int group_rows = 32 >> p.lane_bits;
-    p.steps = std::min(d.dtype == kMxF32 ? 2 : 4, 1 << p.lane_bits);
+    p.vec = wide(d);
+    const bool is_wide = p.vec == 1;
+    p.steps = std::min(d.dtype == kMxF32 || !is_wide ? 2 : 4, 1 << p.lane_bits);
     while (p.steps > 1 && ceil_div(d.rows, 4 * group_rows * p.steps) * p.segments < 2 * sm_count_)
         p.steps /= 2;
     const int64_t grid = ceil_div(d.rows, 4 * group_rows * p.steps) * p.segments;
-    p.vec = wide(d);
+    p.turned = !p.vec && (d.col_stride == 1 || d.cols == 1);
     p.data = reinterpret_cast<uint8_t*>(data);
     p.scales = reinterpret_cast<uint8_t*>(scales);
     p.pitch = static_cast<long long>(pitch_of(format, d.cols));
@@ -290,7 +297,7 @@ void Mx::convert(const MxDense& d, int format, float tensor_scale, uint64_t data
         p.page_count = static_cast<int>(cache->pages);
     }
     const int base = cache ? (read ? kCacheRead : kCacheWrite) : (read ? kDequantise : kQuantise);
-    const int index = convert_index(base, d.dtype, format);
+    const int index = convert_index(base, d.dtype, format) + (is_wide ? 0 : kAny);
     if (grid > 0x7FFFFFFF)
         refuse("too many rows for one call");
     launch(index, static_cast<unsigned>(grid), 128, 0, 1, &p, stream);
@@ -526,8 +533,9 @@ bool Mx::few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream)
         return false;
     // Every CTA quantises its share of dense rows again: more than four chunks a
     // thread cost more than a kernel that does it once (4096 x 4096: 16 rows 6.7
-    // to 7.1 us, 32 rows 9.9 to 8.4)
-    if (!a && rows * most * (w.format == kMxFp8 ? 8 : 16) > 1024)
+    // to 7.1 us, 32 rows 9.9 to 8.4), and more than one where rows begin off
+    // 16-byte boundaries and are read value by value (16 rows of 4095: 10.9)
+    if (!a && rows * most * (w.format == kMxFp8 ? 8 : 16) > (wide(l.x) ? 1024 : 256))
         return false;
     const size_t used = fixed(p.splits);
     p.stages = static_cast<int>(std::min<size_t>({static_cast<size_t>(most), (room - used) / stage, 12}));
@@ -571,7 +579,7 @@ bool Mx::tall(const MxLinear& l, CUstream stream)
     // Fewer rows leave the SMs one CTA with little to do at a time (256 -> 256
     // nvfp4: 8192 rows 8.8 us to 7.7 of two kernels, 14336 rows 8.4 to 11, 32640
     // rows 11.8 to 16.8)
-    if (p.k.k_tiles > kMxTallScaleTiles || l.x.rows < 96 * sm_count_)
+    if (p.k.k_tiles > kMxTallScaleTiles || l.x.rows < 96 * sm_count_ || !wide(l.x))
         return false;
     p.n_tiles = static_cast<int>(ceil_div(w.rows, 64));
     const size_t scale_bytes = static_cast<size_t>(p.k.k_tiles) * 512;

@@ -95,7 +95,7 @@ private:
     CUmodule module_ = nullptr;
     CUdeviceptr status_ = 0;
     int sm_count_ = 0;
-    CUfunction functions_[72] = {};
+    CUfunction functions_[112] = {};
     int clusters_[9] = {};  // by size, 0: not asked yet
 };
 

@@ -58,19 +58,30 @@ struct Dense<kMxF32> {
     static __device__ __forceinline__ T pack(float v) { return v; }
 };
 
-// 32-byte accesses: one per lane covers a chunk of 16-bit values, so a warp
-// touches whole sectors only.
-__device__ __forceinline__ void load32(const void* p, uint32_t (&w)[8])
+// 32 bytes of a lane, a chunk of 16-bit values: one access, or two where rows
+// begin on 16-byte boundaries only (kVec16; kVec32 otherwise, 0: value by value).
+constexpr int kVec32 = 1, kVec16 = 2;
+__device__ __forceinline__ void load32(const void* p, uint32_t (&w)[8], int vec)
 {
-    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
-                 : "l"(p));
+    if (vec == kVec32)
+        asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                     : "l"(p));
+    else
+        asm volatile("ld.global.v4.b32 {%0,%1,%2,%3}, [%8];\n\tld.global.v4.b32 {%4,%5,%6,%7}, [%8 + 16];"
+                     : "=&r"(w[0]), "=&r"(w[1]), "=&r"(w[2]), "=&r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                     : "l"(p));
 }
-__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8])
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8], int vec)
 {
-    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                 : "memory");
+    if (vec == kVec32)
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                     "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                     : "memory");
+    else
+        asm volatile("st.global.v4.b32 [%0], {%1,%2,%3,%4};\n\tst.global.v4.b32 [%0 + 16], {%5,%6,%7,%8};" ::"l"(p),
+                     "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                     : "memory");
 }
 
 // A chunk of a dense row as it lies in memory: 16 values.
@@ -80,8 +91,8 @@ struct Raw {
     uint32_t w[kWords];
 };
 
-// The chunk from column `col`; columns from `cols` on read as 0.  `vec`: the
-// row is contiguous and begins on a 32-byte boundary.
+// The chunk from column `col`; columns from `cols` on read as 0.  `vec`, where
+// the row is contiguous: kVec32 or kVec16.
 template <int DT>
 __device__ __forceinline__ void load_raw(const typename Dense<DT>::T* p, long long col_stride, int col, int cols, int vec,
                                          Raw<DT>& x)
@@ -89,7 +100,7 @@ __device__ __forceinline__ void load_raw(const typename Dense<DT>::T* p, long lo
     if (vec && col + 16 <= cols) {
 #pragma unroll
         for (int i = 0; i < Raw<DT>::kWords; i += 8)
-            load32(reinterpret_cast<const uint32_t*>(p + col) + i, reinterpret_cast<uint32_t(&)[8]>(x.w[i]));
+            load32(reinterpret_cast<const uint32_t*>(p + col) + i, reinterpret_cast<uint32_t(&)[8]>(x.w[i]), vec);
         return;
     }
     if constexpr (DT == kMxF32) {
@@ -159,27 +170,31 @@ __device__ __forceinline__ uint32_t largest_raw(const Raw<DT>& x)
 }
 
 template <int DT>
+__device__ __forceinline__ Raw<DT> pack_raw(const float (&v)[16])
+{
+    Raw<DT> x;
+    if constexpr (DT == kMxF32) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            x.w[i] = __float_as_uint(v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            x.w[i] = Dense<DT>::pack2(v[2 * i], v[2 * i + 1]);
+    }
+    return x;
+}
+
+template <int DT>
 __device__ __forceinline__ void store_chunk(typename Dense<DT>::T* p, long long col_stride, int col, int cols, int vec,
                                             const float (&v)[16])
 {
     using D = Dense<DT>;
     if (vec && col + 16 <= cols) {
-        uint32_t w[8];
-        if constexpr (DT == kMxF32) {
-            uint32_t u[8];
+        const Raw<DT> x = pack_raw<DT>(v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                w[i] = __float_as_uint(v[i]);
-                u[i] = __float_as_uint(v[8 + i]);
-            }
-            store32(p + col, w);
-            store32(p + col + 8, u);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                w[i] = D::pack2(v[2 * i], v[2 * i + 1]);
-            store32(p + col, w);
-        }
+        for (int i = 0; i < Raw<DT>::kWords; i += 8)
+            store32(reinterpret_cast<uint32_t*>(p + col) + i, reinterpret_cast<const uint32_t(&)[8]>(x.w[i]), vec);
         return;
     }
 #pragma unroll

@@ -50,11 +50,133 @@ __device__ __forceinline__ long long cache_slots(const MxConvertParams& p, long 
                           (position - static_cast<long long>(place) * p.page_rows);
 }
 
+// ---- contiguous rows that begin anywhere: lanes of a row take consecutive words
+// and turn them into chunks through shared memory (a word of padding after each
+// chunk keeps the lanes on different banks).  16-bit rows that begin in the
+// middle of a word are shifted by half a word on the way; every word that is
+// touched holds a value of the row.  Element by element the 32 lanes would touch
+// 32 sectors for 2 bytes each: 8192 x 4099 bf16 and back took 228 us.
+template <int DT>
+struct Turn {
+    static constexpr int kWords = Raw<DT>::kWords;         // of a chunk
+    static constexpr int kBuffer = 32 * (kWords + 1) + 16;  // of a warp: a word more for each row
+    static constexpr bool k16 = DT != kMxF32;
+
+    // of the lane's row, from the segment's first column on
+    uint32_t* buffer;
+    int in, lanes;  // lane of the row's `lanes`
+    int columns;    // that exist from there on
+    int half;       // the segment begins in the middle of a word
+
+    __device__ __forceinline__ Turn(uint32_t* warp_buffer, const void* segment, int lane_bits, int columns_left)
+    {
+        const int lane = threadIdx.x & 31;
+        lanes = 1 << lane_bits;
+        in = lane & (lanes - 1);
+        buffer = warp_buffer + (lane >> lane_bits) * (lanes * (kWords + 1) + 1);
+        columns = columns_left;
+        half = k16 ? static_cast<int>(reinterpret_cast<uintptr_t>(segment) >> 1 & 1) : 0;
+    }
+
+    // Values of word q: its first one's column and how many words it may use.
+    __device__ __forceinline__ bool some(int q) const
+    {
+        return k16 ? 2 * q - half < columns && 2 * q - half + 1 >= 0 : q < columns;
+    }
+
+    // Word q of the row, 0 if no column of it exists.
+    __device__ __forceinline__ uint32_t word(const void* segment, int q, bool there) const
+    {
+        const uint32_t* from = reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(segment) - 2 * half);
+        return there && some(q) ? from[q] : 0u;
+    }
+
+    // Asks for the lane's words of the row.
+    __device__ __forceinline__ void ask(const void* segment, bool there, Raw<DT>& x, uint32_t& last) const
+    {
+#pragma unroll
+        for (int j = 0; j < kWords; ++j)
+            x.w[j] = word(segment, j * lanes + in, there);
+        last = half && in == 0 ? word(segment, kWords * lanes, there) : 0u;
+    }
+
+    // Words into the lane's chunk; by the whole warp.
+    __device__ __forceinline__ void turn(Raw<DT>& x, uint32_t last) const
+    {
+#pragma unroll
+        for (int j = 0; j < kWords; ++j) {
+            const int q = j * lanes + in;
+            buffer[q + q / kWords] = x.w[j];
+        }
+        if (half && in == 0)
+            buffer[kWords * lanes + lanes] = last;
+        __syncwarp();
+        uint32_t r[kWords + 1];
+#pragma unroll
+        for (int i = 0; i < kWords; ++i)
+            r[i] = buffer[in * (kWords + 1) + i];
+        r[kWords] = half ? buffer[(in + 1) * (kWords + 1)] : 0u;
+        const int left = columns - in * 16;
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            x.w[i] = k16 ? __funnelshift_r(r[i], r[i + 1], 16 * half) : r[i];
+            const int per = 16 / kWords;  // values of a word
+            if (per * i + per > left)     // columns past the last one are zeros
+                x.w[i] = k16 && per * i < left ? x.w[i] & 0xFFFFu : 0u;
+        }
+        __syncwarp();
+    }
+
+    // The lane's chunk to the row; by the whole warp.
+    __device__ __forceinline__ void store(void* segment, bool there, const Raw<DT>& x) const
+    {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i)
+            buffer[in * (kWords + 1) + i] = x.w[i];
+        __syncwarp();
+        uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(segment) - 2 * half);
+#pragma unroll
+        for (int j = 0; j < kWords; ++j)
+            put(to, j * lanes + in, there);
+        if (half && in == 0)
+            put(to, kWords * lanes, there);
+        __syncwarp();
+    }
+
+    __device__ __forceinline__ void put(uint32_t* to, int q, bool there) const
+    {
+        if (!there || !some(q))
+            return;
+        const uint32_t now = q < kWords * lanes ? buffer[q + q / kWords] : 0u;
+        if constexpr (!k16) {
+            to[q] = now;
+        } else {
+            uint32_t v = now;
+            if (half)
+                v = __funnelshift_r(q ? buffer[q - 1 + (q - 1) / kWords] : 0u, now, 16);
+            const int first = 2 * q - half;
+            uint16_t* each = reinterpret_cast<uint16_t*>(to + q);
+            const bool low = first >= 0, high = first + 1 < columns && q < kWords * lanes;
+            if (low && high)
+                to[q] = v;
+            else if (low)
+                each[0] = static_cast<uint16_t>(v);
+            else if (high)
+                each[1] = static_cast<uint16_t>(v >> 16);
+        }
+    }
+};
+
 // A warp takes `steps` groups of 32 / lanes rows, `lanes` chunks wide; a lane's
 // chunk column is the same in all of them.  The warp's rows are a power of two
 // at a multiple of it, at most 32, so they share a band of the scale tiles and
 // each group's scales lie 16 bytes a row further on.
-template <int DT, int F, bool kCache, bool kRead>
+//
+// kWide: rows begin on 32-byte boundaries and are contiguous, so that a lane
+// moves its chunk with one access.  The other kernels take two (16-byte
+// boundaries, p.vec), turn the chunk (p.turned) or, where columns are apart, go
+// value by value.
+template <int DT, int F, bool kCache, bool kRead, bool kWide>
 __device__ __forceinline__ void mx_convert(const MxConvertParams& p)
 {
     using T = typename Dense<DT>::T;
@@ -71,22 +193,38 @@ __device__ __forceinline__ void mx_convert(const MxConvertParams& p)
     const int in_group = lane >> p.lane_bits;
     const long long row = row0 + in_group;
     const int column = Mx<F>::kIsNv ? chunk : chunk >> 1;
-    constexpr int kSteps = DT == kMxF32 ? 2 : 4;
+    constexpr int kSteps = DT == kMxF32 || !kWide ? 2 : 4;
     // rows of the lane that exist, none past the last column
     const int left = chunk < p.chunks ? static_cast<int>(min(p.rows - row0, 32ll)) - in_group : 0;
     const int count = min(p.steps, (left + (1 << group_bits) - 1) >> group_bits);
 
     T* dense = static_cast<T*>(p.dense) + row * p.row_stride;
     const long long dense_step = p.row_stride << group_bits;
+    __shared__ uint32_t turns[kWide ? 1 : kMxThreads / 32][kWide ? 1 : Turn<DT>::kBuffer];
+    const bool turned = !kWide && p.turned;
+    const int segment = (chunk - (lane & (lanes - 1))) * 16;  // first column of the lane's row here
     Raw<DT> x[kRead ? 1 : kSteps];
     if constexpr (!kRead) {
         const T* from = dense;
+        if (turned) {
+            uint32_t last[kSteps];
 #pragma unroll
-        for (int u = 0; u < kSteps; ++u, from += dense_step)
-            if (u < count)
-                load_raw<DT>(from, p.col_stride, chunk * 16, p.cols, p.vec, x[u]);
-            else
-                x[u] = Raw<DT>{};
+            for (int u = 0; u < kSteps; ++u, from += dense_step)
+                Turn<DT>(turns[warp], from + segment, p.lane_bits, p.cols - segment)
+                    .ask(from + segment, u < p.steps && row + (u << group_bits) < p.rows, x[u], last[u]);
+            from = dense;
+#pragma unroll
+            for (int u = 0; u < kSteps; ++u, from += dense_step)
+                if (u < p.steps)
+                    Turn<DT>(turns[warp], from + segment, p.lane_bits, p.cols - segment).turn(x[u], last[u]);
+        } else {
+#pragma unroll
+            for (int u = 0; u < kSteps; ++u, from += dense_step)
+                if (u < count)
+                    load_raw<DT>(from, p.col_stride, chunk * 16, p.cols, kWide ? kVec32 : p.vec, x[u]);
+                else
+                    x[u] = Raw<DT>{};
+        }
     }
     uint8_t* data[kSteps];   // the lane's chunk in the quantised form, null: none
     uint8_t* scale_[kSteps];
@@ -127,12 +265,17 @@ __device__ __forceinline__ void mx_convert(const MxConvertParams& p)
             }
         }
 #pragma unroll
-        for (int u = 0; u < kSteps; ++u, dense += dense_step)
-            if (u < count) {
-                float v[16];
-                read_chunk<F>(codes[u], scale[u], p.tensor_scale, v);
-                store_chunk<DT>(dense, p.col_stride, chunk * 16, p.cols, p.vec, v);
-            }
+        for (int u = 0; u < kSteps; ++u, dense += dense_step) {
+            if (u >= p.steps)
+                break;
+            float v[16];
+            read_chunk<F>(codes[u], scale[u], p.tensor_scale, v);
+            if (turned)
+                Turn<DT>(turns[warp], dense + segment, p.lane_bits, p.cols - segment)
+                    .store(dense + segment, row + (u << group_bits) < p.rows, pack_raw<DT>(v));
+            else if (u < count)
+                store_chunk<DT>(dense, p.col_stride, chunk * 16, p.cols, kWide ? kVec32 : p.vec, v);
+        }
     } else {
         // the product reads whole words: the rest of the last scale tile is zero
         const bool pads = !kCache && chunk == p.chunks - 1 && (column & 3) != 3;
@@ -156,18 +299,21 @@ __device__ __forceinline__ void mx_convert(const MxConvertParams& p)
     }
 }
 
-#define MLVC_MX_CONVERT(NAME, BOUNDS, DT, F, CACHE, READ)                                    \
+#define MLVC_MX_CONVERT(NAME, BOUNDS, DT, F, CACHE, READ, WIDE)                               \
     extern "C" __global__ void __launch_bounds__ BOUNDS NAME(const __grid_constant__ MxConvertParams p) \
     {                                                                                        \
-        mx_convert<DT, F, CACHE, READ>(p);                                                   \
+        mx_convert<DT, F, CACHE, READ, WIDE>(p);                                             \
     }
-// Quantising is bound by 64 registers a thread, eight CTAs an SM; reading back
+// Quantising is bound to 64 registers a thread, eight CTAs an SM; reading back
 // needs fewer of itself, and is slower when the compiler is told so.
-#define MLVC_MX_CONVERT_ALL(T, DT, FN, F)                                                     \
-    MLVC_MX_CONVERT(mlvc_mx_quantise_##T##_##FN, (kMxThreads, 8), DT, F, false, false)        \
-    MLVC_MX_CONVERT(mlvc_mx_dequantise_##T##_##FN, (kMxThreads), DT, F, false, true)          \
-    MLVC_MX_CONVERT(mlvc_mx_cache_write_##T##_##FN, (kMxThreads, 8), DT, F, true, false)      \
-    MLVC_MX_CONVERT(mlvc_mx_cache_read_##T##_##FN, (kMxThreads), DT, F, true, true)
+#define MLVC_MX_CONVERT_WIDE(T, DT, FN, F, SUFFIX, WIDE)                                                   \
+    MLVC_MX_CONVERT(mlvc_mx_quantise_##T##_##FN##SUFFIX, (kMxThreads, 8), DT, F, false, false, WIDE)       \
+    MLVC_MX_CONVERT(mlvc_mx_dequantise_##T##_##FN##SUFFIX, (kMxThreads), DT, F, false, true, WIDE)         \
+    MLVC_MX_CONVERT(mlvc_mx_cache_write_##T##_##FN##SUFFIX, (kMxThreads, 8), DT, F, true, false, WIDE)     \
+    MLVC_MX_CONVERT(mlvc_mx_cache_read_##T##_##FN##SUFFIX, (kMxThreads), DT, F, true, true, WIDE)
+#define MLVC_MX_CONVERT_ALL(T, DT, FN, F)           \
+    MLVC_MX_CONVERT_WIDE(T, DT, FN, F, , true)      \
+    MLVC_MX_CONVERT_WIDE(T, DT, FN, F, _any, false)
 
 MLVC_MX_CONVERT_ALL(f16, kMxF16, mxfp4, kMxFp4)
 MLVC_MX_CONVERT_ALL(f16, kMxF16, nvfp4, kNvFp4)

@@ -40,6 +40,8 @@ struct MxOut {
     static constexpr int kRounds = kLanes;     // each of kCols rows
 
     struct Asked {  // what a chunk needs from memory
+        // residual: the lane's pieces, or, off 16-byte boundaries, 32 rows' values
+        // of one column (16-bit: two a word)
         uint4 res[kRounds];
         float bias[kCols];
     };
@@ -50,6 +52,20 @@ struct MxOut {
     uint32_t there;              // bit i: the row of round i exists
     long long row0;
     int rows;
+
+    // The value at p, 0 where it is not there: no branch and no conversion, so
+    // that many can be under way.
+    static __device__ __forceinline__ uint32_t bits(const T* p, bool there)
+    {
+        uint32_t v;
+        if constexpr (DT == kMxF32)
+            asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.b32 %0, [%1];\n\t}"
+                         : "=&r"(v) : "l"(p), "r"(static_cast<int>(there)) : "memory");
+        else
+            asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.u16 %0, [%1];\n\t}"
+                         : "=&r"(v) : "l"(p), "r"(static_cast<int>(there)) : "memory");
+        return v;
+    }
 
     // Rows row0 .. row0 + 32, none from `end` on.
     __device__ __forceinline__ void set_rows(const MxEpilogue& e, long long first, long long end)
@@ -71,10 +87,27 @@ struct MxOut {
     {
         const int col = col0 + (threadIdx.x & 31) % kLanes * kCols;
         const bool wide = e.vec && col + kCols <= e.N;
-        const uint8_t* from = reinterpret_cast<const uint8_t*>(res + col);
+        if (__all_sync(0xFFFFFFFFu, wide)) {
+            const uint8_t* from = reinterpret_cast<const uint8_t*>(res + col);
 #pragma unroll
-        for (int i = 0; i < kRounds; ++i, from += res_step)
-            a.res[i] = e.residual && wide && (there >> i & 1u) ? load16(from) : make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < kRounds; ++i, from += res_step)
+                a.res[i] = e.residual && (there >> i & 1u) ? load16(from) : make_uint4(0, 0, 0, 0);
+        } else {
+            const int lane = threadIdx.x & 31;
+            const T* from = static_cast<const T*>(e.residual) + row0 * e.residual_stride + col0 + lane;
+            const int n = e.residual && col0 + lane < e.N ? rows : 0;
+            uint32_t* w = reinterpret_cast<uint32_t*>(a.res);
+            uint32_t each[32];  // all under way before two become one
+#pragma unroll
+            for (int r = 0; r < 32; ++r, from += e.residual_stride)
+                each[r] = bits(from, r < n);
+#pragma unroll
+            for (int r = 0; r < 32; ++r)
+                if constexpr (DT == kMxF32)
+                    w[r] = each[r];
+                else if (r & 1)
+                    w[r / 2] = each[r - 1] | each[r] << 16;
+        }
 #pragma unroll
         for (int k = 0; k < kCols; k += 4) {
             const uint4 b = e.bias && wide ? load16(e.bias + col + k) : make_uint4(0, 0, 0, 0);
@@ -145,14 +178,20 @@ struct MxOut {
             // off 16-byte boundaries or at the last columns: a lane takes a column
             const float b = e.bias ? e.bias[col0 + lane] : 0.0f;
             const float* sums = reinterpret_cast<const float*>(turn);
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(a.res);
             T* to = static_cast<T*>(e.y) + row0 * e.y_stride + col0 + lane;
-            const T* from = static_cast<const T*>(e.residual) + row0 * e.residual_stride + col0 + lane;
-#pragma unroll 8
-            for (int r = 0; r < rows; ++r) {
+#pragma unroll
+            for (int r = 0; r < 32; ++r, to += e.y_stride) {
                 float g = finish(sums[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)], b);
-                if (e.residual)
-                    g += D::load(from + r * e.residual_stride);
-                to[r * e.y_stride] = D::pack(g);
+                if constexpr (DT == kMxF32) {
+                    g += __uint_as_float(w[r]);
+                } else {
+                    float lo, hi;
+                    D::unpack(w[r / 2], lo, hi);
+                    g += r & 1 ? hi : lo;
+                }
+                if (r < rows)
+                    *to = D::pack(g);
             }
         }
         __syncwarp();

@@ -31,7 +31,8 @@ struct MxConvertParams {
     int lane_bits;                     // a warp is 2^lane_bits chunks wide
     int segments;                      // of that width in a row
     int steps;                         // groups of 32 / 2^lane_bits rows of a warp
-    int vec;                           // dense rows begin on 32-byte boundaries and are contiguous
+    int vec;                           // dense rows are contiguous and begin on 32-byte (1) or 16-byte (2) boundaries
+    int turned;                        // they are contiguous and begin elsewhere
     uint8_t* data;
     uint8_t* scales;
     long long pitch;                   // bytes of a quantised row
