@@ -484,21 +484,36 @@ void encode_scales(CUtensorMap* map, uint64_t scales, int k_tiles, int64_t bands
 }
 }  // namespace
 
+namespace {
+// Tiles of 128 x 64, 128 x 128 or, by pairs of CTAs, 256 x 256: rounds over the
+// SMs, each weighted with what it takes (nvfp4, k = 4096: 5.2, 6.1 and 8.7 us a
+// round beside 3 us that every call takes).
+struct Rounds {
+    double t64, t128, t256;
+};
+
+Rounds rounds_of(int64_t rows, int64_t outputs, int sms)
+{
+    const int64_t m128 = ceil_div(rows, 128), m256 = ceil_div(rows, 256);
+    return {0.87 * static_cast<double>(ceil_div(m128 * ceil_div(outputs, 64), sms)),
+            static_cast<double>(ceil_div(m128 * ceil_div(outputs, 128), sms)),
+            1.45 * static_cast<double>(ceil_div(m256 * ceil_div(outputs, 256), std::max(1, sms / 2)))};
+}
+}  // namespace
+
 bool Mx::few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream)
 {
     const MxMatrix& w = l.w;
     const int64_t rows = a ? a->rows : l.x.rows;
-    // Measured against the tiles of 128 rows (nvfp4, 4096 x 4096: 32 rows 6.2 us
-    // to 7.9, 64 rows 7.2 to 7.9, 96 rows 8.5 to 8.0): from 64 rows on sending
-    // and adding up the parts costs more than the padding.  Rows of less than 8
-    // panels leave less to share (1024 x 1024: 32 rows 4.6 to 4.6, 64 rows 5.8 to 4.6).
-    if (rows > (w.cols <= 1024 && w.format != kMxFp8 ? kMxRowsMax / 2 : kMxRowsMax))
-        return false;
     ContextGuard guard(ctx_);
     MxRowsParams p{};
     p.k = panels_of(w.format, w.cols);
-    const int64_t n_tiles = ceil_div(w.rows, 128);
-    p.row_tile = static_cast<int>(ceil_div(rows, 8) * 8);
+    const int64_t row_units = ceil_div(rows, kMxRowsMax), unit_rows = std::min<int64_t>(rows, kMxRowsMax);
+    if (row_units > sm_count_ || (!a && row_units > 1))
+        return false;
+    const int64_t tiles = ceil_div(w.rows, 128) * row_units;
+    p.n_tiles = static_cast<int>(ceil_div(w.rows, 128));
+    p.row_tile = static_cast<int>(ceil_div(unit_rows, 8) * 8);
     const size_t x_bytes = static_cast<size_t>(p.row_tile) * 128;
     const int words = w.format == kNvFp4 ? 4 : w.format == kMxFp4 ? 2 : 1;
     const size_t scale_bytes = static_cast<size_t>(words) * 512;
@@ -506,7 +521,7 @@ bool Mx::few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream)
     int64_t most = 0;
     auto fixed = [&](int splits) {
         most = ceil_div(p.k.count, splits);
-        return 2048 + (splits > 1 ? ceil_div(splits * ceil_div(rows, splits) * 512, 1024) * 1024 : 0) +
+        return 2048 + (splits > 1 ? ceil_div(splits * ceil_div(unit_rows, splits) * 512, 1024) * 1024 : 0) +
                (a ? 0 : most * x_bytes + ceil_div(most * scale_bytes, 1024) * 1024);
     };
     // As many CTAs on k as there are SMs for at once, each with two panels or
@@ -518,18 +533,28 @@ bool Mx::few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream)
     const size_t whole = kGemmSmem, half = 113 * 1024;
     auto fits = [&](int splits, size_t room) { return fixed(splits) + std::min<size_t>(most, 3) * stage <= room; };
     p.splits = static_cast<int>(std::clamp<int64_t>(p.k.count / 2, 1, 8));
-    while (p.splits > 1 && n_tiles > clusters(p.splits))
+    while (p.splits > 1 && tiles > clusters(p.splits))
         --p.splits;
     size_t room = whole;
     if (p.splits == 1) {
-        if (p.k.count >= 4 && n_tiles <= 2 * clusters(2) && fits(2, half)) {
+        if (p.k.count >= 4 && tiles <= 2 * clusters(2) && fits(2, half)) {
             p.splits = 2;
             room = half;
-        } else if (n_tiles > sm_count_ && fits(1, half)) {
+        } else if (tiles > sm_count_ && fits(1, half)) {
             room = half;
         }
     }
     if (!fits(p.splits, room))
+        return false;
+    // Measured beside the tiles of 128 rows: here 3.4 us, 0.3 a panel of a CTA's
+    // share and 2.6 for sending and adding up 64 rows; there 3.2 us and 0.38 a panel
+    // and round.  nvfp4: 4096 x 4096, 64 rows 7.2 to 7.5, 128 rows 9.1 to 7.7;
+    // 7168 -> 2048, 96 rows 8.0 to 10.8; 8192 -> 128, 512 rows 6.4 to 11.6.
+    const Rounds r = rounds_of(rows, w.rows, sm_count_);
+    const double here = 3.4 + 0.3 * static_cast<double>(most * ceil_div(tiles * p.splits, sm_count_)) +
+                        2.6 * static_cast<double>(unit_rows) / kMxRowsMax;
+    const double there = 3.2 + 0.38 * static_cast<double>(p.k.count) * std::min({r.t64, r.t128, r.t256});
+    if (rows > 16 && (here > (row_units > 1 ? 0.9 : 1.0) * there || (row_units > 1 && p.splits == 1)))
         return false;
     // Every CTA quantises its share of dense rows again: more than four chunks a
     // thread cost more than a kernel that does it once (4096 x 4096: 16 rows 6.7
@@ -540,11 +565,11 @@ bool Mx::few_rows(const MxLinear& l, const MxMatrix* a, CUstream stream)
     const size_t used = fixed(p.splits);
     p.stages = static_cast<int>(std::min<size_t>({static_cast<size_t>(most), (room - used) / stage, 12}));
     // the ring holds the sums in the end
-    const size_t smem = used + std::max(p.stages * stage, static_cast<size_t>(rows) * 512);
+    const size_t smem = used + std::max(p.stages * stage, static_cast<size_t>(unit_rows) * 512);
     if (smem > whole)
         return false;
     p.batch = std::max(1, std::min(4, p.stages >= most ? static_cast<int>(most) : p.stages / 2));
-    const int64_t grid = n_tiles * p.splits;
+    const int64_t grid = tiles * p.splits;
     const size_t pitch = pitch_of(w.format, w.cols);
     encode_rows(&p.map_w, w.data, pitch, w.rows, 128);
     p.scales_w = reinterpret_cast<const uint8_t*>(w.scales);
@@ -629,15 +654,8 @@ void Mx::pair(const MxLinear& l, const MxMatrix& a, CUstream stream)
 void Mx::product(const MxLinear& l, const MxMatrix& a, CUstream stream)
 {
     ContextGuard guard(ctx_);
-    // Tiles of 128 x 64, 128 x 128 or, by pairs of CTAs, 256 x 256: the least
-    // rounds over the SMs, each weighted with what it takes (nvfp4, k = 4096: 5.2,
-    // 6.1 and 8.7 us a round beside 3 us that every call takes).
-    const int64_t m128 = ceil_div(a.rows, 128), n64 = ceil_div(l.w.rows, 64), n128 = ceil_div(l.w.rows, 128);
-    const double t64 = 0.87 * static_cast<double>(ceil_div(m128 * n64, sm_count_));
-    const double t128 = static_cast<double>(ceil_div(m128 * n128, sm_count_));
-    const double t256 =
-        1.45 * static_cast<double>(ceil_div(ceil_div(a.rows, 256) * ceil_div(l.w.rows, 256), std::max(1, sm_count_ / 2)));
-    if (t256 <= t128 && t256 <= t64) {
+    const Rounds r = rounds_of(a.rows, l.w.rows, sm_count_);
+    if (r.t256 <= r.t128 && r.t256 <= r.t64) {
         pair(l, a, stream);
         return;
     }
@@ -649,7 +667,7 @@ void Mx::product(const MxLinear& l, const MxMatrix& a, CUstream stream)
     p.k = panels_of(w.format, w.cols);
     p.e = epilogue_of(l, a.rows, a.tensor_scale);
     p.m_tiles = static_cast<int>(ceil_div(a.rows, 128));
-    const bool narrow = t64 < t128;
+    const bool narrow = r.t64 < r.t128;
     const int bn = narrow ? 64 : 128;
     p.n_tiles = static_cast<int>(ceil_div(w.rows, bn));
     if (static_cast<int64_t>(p.m_tiles) * p.n_tiles > 0x7FFFFFFF - 8 * p.n_tiles)

@@ -105,15 +105,16 @@ constexpr int kMxTallScaleTiles = 16;   // of a row at most: their TMEM columns
 
 // Products of few rows (see mx_rows): weights are the tensor core's first
 // operand, rows its second.
-constexpr int kMxRowsMax = 64;
+constexpr int kMxRowsMax = 64;         // of a CTA
 struct MxRowsParams {
     CUtensorMap map_w;                 // weights, boxes of 128 bytes x 128 rows
     CUtensorMap map_x;                 // quantised rows, boxes of 128 bytes x row_tile rows
     const uint8_t* scales_w;
     const uint8_t* scales_x;
     MxPanels k;
+    int n_tiles;                       // of 128 weights
     int splits;                        // CTAs of a cluster, each with its share of the panels
-    int row_tile;                      // rows rounded up to 8
+    int row_tile;                      // rows of a CTA rounded up to 8
     int stages;
     int batch;                         // panels whose scales go to TMEM at once
     // dense rows: quantised in groups of panels, about two chunks a thread each,

@@ -1,4 +1,4 @@
-// Products of few rows (1 to 64) with quantised weights:
+// Products of few rows with quantised weights, 64 rows at a time:
 //     y[m, n] = leaky(alpha * sum_k x[m, k] w[n, k] + bias[n]) + residual[m, n]
 //
 // Reading the weights bounds these calls, so the roles of the operands are
@@ -51,7 +51,7 @@ __device__ __forceinline__ void bulk_send(uint32_t to, const void* from, uint32_
 
 // One result.
 template <int DT>
-__device__ __forceinline__ void mx_finish_one(const MxEpilogue& e, int m, int n, float sum)
+__device__ __forceinline__ void mx_finish_one(const MxEpilogue& e, long long m, int n, float sum)
 {
     using T = typename Dense<DT>::T;
     const float t = fmaf(sum, e.alpha, e.bias ? e.bias[n] : 0.0f);
@@ -73,11 +73,13 @@ __device__ __forceinline__ void mx_rows(const MxRowsParams& p)
     MxRowsShared* sh = reinterpret_cast<MxRowsShared*>(base);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t rank = blockIdx.x % p.splits;
-    const int n0 = blockIdx.x / p.splits * 128;
+    const int unit = blockIdx.x / p.splits, row_unit = unit / p.n_tiles;
+    const int n0 = (unit - row_unit * p.n_tiles) * 128;
+    const int base_m = row_unit * kMxRowsMax;  // first row
     const int k0 = static_cast<int>(static_cast<long long>(p.k.count) * rank / p.splits);
     const int k1 = static_cast<int>(static_cast<long long>(p.k.count) * (rank + 1) / p.splits);
     const int panels = k1 - k0;
-    const int M = p.e.M;
+    const int M = min(p.e.M - base_m, kMxRowsMax);
 
     // shared memory: sums of this CTA's rows from all CTAs, then, dense: x tiles
     // and their scales of all panels, then the ring of weight panels; else the
@@ -137,8 +139,9 @@ __device__ __forceinline__ void mx_rows(const MxRowsParams& p)
                 tma_load_2d(s, &p.map_w, bar, k * 128, n0);
                 bulk_load(s + sw_at, p.scales_w + (static_cast<long long>(n0 / 128) * p.k.k_tiles + word) * 512, sbytes, bar);
                 if constexpr (!kDense) {
-                    tma_load_2d(s + x_at, &p.map_x, bar, k * 128, 0);
-                    bulk_load(s + sx_at, p.scales_x + word * 512, sbytes, bar);
+                    tma_load_2d(s + x_at, &p.map_x, bar, k * 128, base_m);
+                    bulk_load(s + sx_at, p.scales_x + (static_cast<long long>(base_m / 128) * p.k.k_tiles + word) * 512, sbytes,
+                              bar);
                 }
                 armed |= 1u << stage;
                 parity = (parity & ~(1u << stage)) | (phase << stage);
@@ -164,6 +167,7 @@ __device__ __forceinline__ void mx_rows(const MxRowsParams& p)
             mbar_arrive(&sh->sums);  // tmem_base
             const uint32_t tmem = sh->tmem_base;
             const uint32_t idesc = mx_idesc<F>(128, p.row_tile);
+            const uint32_t in_band = base_m % 128 / 32;  // columns: these rows are half of a scale tile's
             const uint32_t scales = tmem + p.row_tile;  // of a batch: weights' and x's 4 columns a scale tile
             // descriptors differ by their start addresses (16-byte units) alone
             const uint64_t ring_desc = smem_desc(smem_u32(ring), 16, 1024, 2);
@@ -211,7 +215,7 @@ __device__ __forceinline__ void mx_rows(const MxRowsParams& p)
                         if (ks >= steps)
                             break;
                         const uint32_t w = ks * kWords / 4, id = kWords == 4 ? 0 : kWords == 2 ? (ks & 1) * 2 : ks;
-                        umma_mx<F>(tmem, w_desc + 2 * ks, x_desc + 2 * ks, idesc, id, from + 8 * w, from + 8 * w + 4,
+                        umma_mx<F>(tmem, w_desc + 2 * ks, x_desc + 2 * ks, idesc, id, from + 8 * w, from + 8 * w + 4 + in_band,
                                    (k + i - k0) | ks);
                         ++issued;
                     }
@@ -345,7 +349,7 @@ __device__ __forceinline__ void mx_rows(const MxRowsParams& p)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (n0 + 32 * i + lane < p.e.N)
-                        mx_finish_one<decltype(type)::value>(p.e, m0 + j, n0 + 32 * i + lane, sum[i]);
+                        mx_finish_one<decltype(type)::value>(p.e, base_m + m0 + j, n0 + 32 * i + lane, sum[i]);
             }
         };
         if (all)
