@@ -269,7 +269,8 @@ int mlvc_b200_read_tensor(mlvc_b200_backend* backend, const char* name, void* ds
  *   0 mxfp4  codes E2M1, blocks of 32, scales powers of two (E8M0)
  *   1 nvfp4  codes E2M1, blocks of 16, scales E4M3, one float per tensor
  *   2 mxfp8  codes E4M3, blocks of 32, scales powers of two (E8M0)
- * tensor_scale is 1 except for nvfp4.  A block that holds an infinity or a NaN
+ * tensor_scale is 1 except for nvfp4, where it and the product of two lie in
+ * [2^-90, 2^90] and [2^-126, 2^128).  A block that holds an infinity or a NaN
  * reads back as NaN, and so does every product with it.
  *
  * All pointers are device addresses on the backend's device and all work is

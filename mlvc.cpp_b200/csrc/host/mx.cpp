@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <numeric>
 #include <stdexcept>
 #include <string>
 
@@ -43,6 +44,16 @@ void check_size(int64_t rows, int64_t cols)
 
 size_t elem_size(int dtype) { return dtype == kMxF32 ? 4 : 2; }
 
+// Two elements at one address: i * row_stride = j * col_stride for rows i and
+// columns j apart, the nearest of which are col_stride / gcd and row_stride / gcd.
+bool overlaps(const MxDense& d)
+{
+    if (d.rows <= 1 || d.cols <= 1)
+        return (d.rows > 1 && d.row_stride < 1) || (d.cols > 1 && d.col_stride < 1);
+    const int64_t g = std::gcd(d.row_stride, d.col_stride);
+    return g == 0 || (d.col_stride / g < d.rows && d.row_stride / g < d.cols);
+}
+
 void check_dense(const MxDense& d, const char* what, bool output)
 {
     if (d.dtype != kMxF16 && d.dtype != kMxBf16 && d.dtype != kMxF32)
@@ -54,7 +65,7 @@ void check_dense(const MxDense& d, const char* what, bool output)
         refuse(std::string(what) + ": null or misaligned device pointer");
     if (d.row_stride < 0 || d.col_stride < 0)
         refuse(std::string(what) + ": negative stride");
-    if (output && ((d.rows > 1 && d.row_stride < 1) || (d.cols > 1 && d.col_stride < 1)))
+    if (output && overlaps(d))
         refuse(std::string(what) + ": an output's elements must not overlap");
     const int64_t limit = int64_t{1} << 60;
     if (d.row_stride > limit / std::max<int64_t>(d.rows, 1) || d.col_stride > limit / d.cols)
@@ -393,6 +404,11 @@ void Mx::linear(const MxLinear& l, CUstream stream)
         if (l.residual.cols > 1 && l.residual.col_stride != 1)
             refuse("the residual's columns must be contiguous");
     }
+    const float alpha = (dense ? l.tensor_scale : l.a.tensor_scale) * w.tensor_scale;
+    if (alpha < 0x1p-126f || !std::isfinite(alpha))
+        refuse("the product of the tensor scales must lie in [2^-126, 2^128)");
+    if (ceil_div(rows, 128) > 0x7FFFFFFF / ceil_div(w.rows, 64) - 8)
+        refuse("too many output tiles for one call");
     if (l.bias % 4)
         refuse("bias: misaligned device pointer");
     if (!std::isfinite(l.slope))
@@ -670,8 +686,6 @@ void Mx::product(const MxLinear& l, const MxMatrix& a, CUstream stream)
     const bool narrow = r.t64 < r.t128;
     const int bn = narrow ? 64 : 128;
     p.n_tiles = static_cast<int>(ceil_div(w.rows, bn));
-    if (static_cast<int64_t>(p.m_tiles) * p.n_tiles > 0x7FFFFFFF - 8 * p.n_tiles)
-        refuse("too many output tiles for one call");
     encode_rows(&p.map_a, a.data, pitch, a.rows, 128);
     encode_rows(&p.map_b, w.data, pitch, w.rows, bn);
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>(sm_count_, static_cast<int64_t>(p.m_tiles) * p.n_tiles));

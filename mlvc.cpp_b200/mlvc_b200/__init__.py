@@ -152,6 +152,7 @@ class Backend:
             _check(lib().mlvc_b200_set_debug_tensors(self._h, 1))
         self._in, self._out = [], []
         self._calls = mx.Calls()
+        self._device = device_id if plan_only_for is None else None  # operands' device
 
     def close(self):
         if self._h:
@@ -272,14 +273,18 @@ class Backend:
     def mx_quantise(self, x, out, stream=None):
         """Quantises the dense matrix x into the MxMatrix `out` of its shape."""
         c = self._calls
-        mx._fill(c.matrix, x)
+        if out.device != self._device:
+            mx._check_device(out.device, self._device, "the quantised matrix")
+        mx._fill(c.matrix, x, self._device)
         if _lib.mlvc_b200_mx_quantise(self._h, c.matrix_ref, out.ref, self.stream or 0 if stream is None else stream):
             _check(-1)
 
     def mx_dequantise(self, m, y, stream=None):
         """Reads the MxMatrix m back into the dense matrix y of its shape."""
         c = self._calls
-        mx._fill(c.matrix, y)
+        if m.device != self._device:
+            mx._check_device(m.device, self._device, "the quantised matrix")
+        mx._fill(c.matrix, y, self._device)
         if _lib.mlvc_b200_mx_dequantise(self._h, m.ref, c.matrix_ref, self.stream or 0 if stream is None else stream):
             _check(-1)
 
@@ -289,8 +294,10 @@ class Backend:
         sequence s, whose pages are pages[s] (device int32 arrays [sequences,
         pages], [sequences + 1], [sequences]; starts None: all zero)."""
         c = self._calls
-        mx._fill(c.matrix, x)
-        mx._fill_rows(c.rows, pages, offsets, starts)
+        if cache.device != self._device:
+            mx._check_device(cache.device, self._device, "the cache")
+        mx._fill(c.matrix, x, self._device)
+        mx._fill_rows(c.rows, pages, offsets, starts, self._device)
         if _lib.mlvc_b200_mx_cache_write(self._h, cache.ref, c.matrix_ref, c.rows_ref,
                                          self.stream or 0 if stream is None else stream):
             _check(-1)
@@ -299,8 +306,10 @@ class Backend:
         """Reads packed rows back into the dense matrix y, addressed as in
         mx_cache_write; rows that have no place are zeros."""
         c = self._calls
-        mx._fill(c.matrix, y)
-        mx._fill_rows(c.rows, pages, offsets, starts)
+        if cache.device != self._device:
+            mx._check_device(cache.device, self._device, "the cache")
+        mx._fill(c.matrix, y, self._device)
+        mx._fill_rows(c.rows, pages, offsets, starts, self._device)
         if _lib.mlvc_b200_mx_cache_read(self._h, cache.ref, c.matrix_ref, c.rows_ref,
                                         self.stream or 0 if stream is None else stream):
             _check(-1)

@@ -87,7 +87,30 @@ _pack_matrix = struct.Struct("=Qiiqqqq").pack_into
 _pack_rows = struct.Struct("=QqQQq").pack_into
 
 
-def _fill(m, t):
+def _device(t):
+    """Index of the device that holds `t`, -1: the host; None: `t` does not say."""
+    get = getattr(t, "get_device", None)
+    return None if get is None else get()
+
+
+def _check_device(at, device, what):
+    """`device`: a backend's, None where it only plans.  A kernel that is given
+    another memory's address faults."""
+    if device is not None and at is not None and at != device:
+        raise RuntimeError(f"mlvc-b200: {what} is on {'the host' if at < 0 else f'device {at}'}, the backend on "
+                           f"device {device}")
+
+
+def _elsewhere(t, device):
+    """Whether `t` is known to be on another device (inlined in _fill, once a
+    dense operand: calls on few rows are as long as the host takes for them)."""
+    try:
+        return t.get_device() != device
+    except AttributeError:
+        return False
+
+
+def _fill(m, t, device):
     """Describes the matrix `t` in the structure `m`."""
     shape = t.shape
     if len(shape) != 2:
@@ -95,6 +118,12 @@ def _fill(m, t):
     code = _dtype_codes.get(t.dtype)
     if code is None:
         code = _code(t.dtype)
+    if device is not None:
+        try:
+            if t.get_device() != device:
+                _check_device(t.get_device(), device, "a dense matrix")
+        except AttributeError:
+            pass
     _pack_matrix(m, 0, t.data_ptr(), code, 0, *shape, *t.stride())
 
 
@@ -107,13 +136,15 @@ def _format(name):
 _int32 = set()  # dtype objects known to be int32
 
 
-def _ints(t, what, dims):
+def _ints(t, what, dims, device):
     """Shape of a contiguous int32 device array."""
     shape = t.shape
     if t.dtype not in _int32 and str(t.dtype).rsplit(".", 1)[-1] == "int32":
         _int32.add(t.dtype)
     if t.dtype not in _int32 or len(shape) != dims or not t.is_contiguous():
         raise RuntimeError(f"mlvc-b200: {what} must be a contiguous int32 array of {dims} dimension(s)")
+    if device is not None and _elsewhere(t, device):
+        _check_device(t.get_device(), device, what)
     return shape
 
 
@@ -121,6 +152,13 @@ def _room(buffer, need, what):
     have = buffer.nbytes if hasattr(buffer, "nbytes") else need
     if have < need:
         raise RuntimeError(f"mlvc-b200: {what} needs {need} bytes and has {have}")
+
+
+def _held_device(data, scales):
+    at = _device(data)
+    if _device(scales) != at:
+        raise RuntimeError("mlvc-b200: data and scales are on different devices")
+    return at
 
 
 class MxLayout(NamedTuple):
@@ -146,6 +184,7 @@ class MxMatrix:
         _room(scales, lay.scale_bytes, "a quantised matrix's scales")
         self.format, self.rows, self.cols, self.tensor_scale = format, int(rows), int(cols), float(tensor_scale)
         self.data, self.scales = data, scales
+        self.device = _held_device(data, scales)
         self.c = MxMatrixC(_format(format), tensor_scale, rows, cols, data.data_ptr(), scales.data_ptr())
         self.ref = ctypes.byref(self.c)
 
@@ -171,6 +210,7 @@ class MxCache:
         _room(scales, lay.scale_bytes, "a cache's scales")
         self.format, self.pages, self.page_rows, self.cols = format, int(pages), int(page_rows), int(cols)
         self.tensor_scale, self.data, self.scales = float(tensor_scale), data, scales
+        self.device = _held_device(data, scales)
         self.c = MxCacheC(_format(format), tensor_scale, pages, page_rows, cols, data.data_ptr(), scales.data_ptr())
         self.ref = ctypes.byref(self.c)
 
@@ -185,11 +225,11 @@ class MxCache:
         return cls(format, pages, page_rows, cols, alloc(lay.data_bytes), alloc(lay.scale_bytes), tensor_scale, lay)
 
 
-def _fill_rows(r, pages, offsets, starts):
+def _fill_rows(r, pages, offsets, starts, device):
     """Describes where packed rows lie (see mlvc_b200_mx_rows) in the structure `r`."""
-    sequences, per_sequence = _ints(pages, "the page table", 2)
-    if _ints(offsets, "offsets", 1)[0] != sequences + 1 or (starts is not None and
-                                                            _ints(starts, "starts", 1)[0] != sequences):
+    sequences, per_sequence = _ints(pages, "the page table", 2, device)
+    if _ints(offsets, "offsets", 1, device)[0] != sequences + 1 or (
+            starts is not None and _ints(starts, "starts", 1, device)[0] != sequences):
         raise RuntimeError("mlvc-b200: offsets has one entry more than there are sequences, starts as many")
     _pack_rows(r, 0, pages.data_ptr(), per_sequence, offsets.data_ptr(), 0 if starts is None else starts.data_ptr(),
                sequences)
@@ -216,6 +256,9 @@ class MxLinear:
         if bias is not None and (not str(bias.dtype).endswith("float32") or tuple(bias.shape) != (weight.rows,) or
                                  not bias.is_contiguous()):
             raise RuntimeError("mlvc-b200: bias must be a contiguous float32 vector, one value for each output")
+        _check_device(weight.device, backend._device, "the weight")
+        if bias is not None:
+            _check_device(_device(bias), backend._device, "bias")
         self._keep = (weight, bias)
         self._check, self._lib = _check, lib()
         self._call, self._backend = self._lib.mlvc_b200_mx_linear, backend
@@ -236,20 +279,24 @@ class MxLinear:
         """x: dense [rows, inputs], or an MxMatrix of the weight's format; y and
         residual: dense [rows, outputs] of one type.  Dense x needs a workspace
         (256-byte boundary) that nothing else uses until the call's work is done."""
-        a = self._args
+        a, device = self._args, self._backend._device
         if isinstance(x, MxMatrix):
+            if x.device != device:
+                _check_device(x.device, device, "x")
             a.a = x.c
             self._x.data = 0
         else:
             if self._a.data:
                 self._a.data = 0
-            _fill(self._x, x)
-        _fill(self._y, y)
+            _fill(self._x, x, device)
+        _fill(self._y, y, device)
         if residual is not None:
-            _fill(self._residual, residual)
+            _fill(self._residual, residual, device)
         elif self._residual.data:
             self._residual.data = 0
         if workspace is not None:
+            if device is not None and _elsewhere(workspace, device):
+                _check_device(workspace.get_device(), device, "the workspace")
             a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.nbytes
         elif a.workspace:
             a.workspace = a.workspace_bytes = 0

@@ -172,6 +172,49 @@ def test_cache_refusals(be):
                 call(cache, a["x"], a["pages"], a["offsets"], starts=a["starts"])
 
 
+def test_outputs_that_overlap_are_refused(be):
+    """Against the addresses of all elements."""
+    for rows in (1, 2, 3, 5):
+        for cols in (1, 2, 3, 4):
+            for row_stride in range(0, 9):
+                for col_stride in range(0, 9):
+                    y = torch.zeros(64).as_strided((rows, cols), (row_stride, col_stride))
+                    distinct = len({i * row_stride + j * col_stride for i in range(rows) for j in range(cols)})
+                    with pytest.raises(RuntimeError, match="planning-only" if distinct == rows * cols else "must not overlap"):
+                        be.mx_dequantise(held("mxfp8", rows, cols), y)
+
+
+@pytest.mark.parametrize("gx, gw, ok", [(2.0**90, 2.0**-90, True), (2.0**-63, 2.0**-63, True), (2.0**-63, 2.0**-64, False),
+                                        (2.0**64, 2.0**63, True), (2.0**64, 2.0**64, False)])
+def test_products_of_tensor_scales_that_leave_floats_are_refused(be, gx, gw, ok):
+    layer = mx.MxLinear(be, held("nvfp4", 8, 64, gw), tensor_scale=gx)
+    match = "planning-only" if ok else "product of the tensor scales"
+    with pytest.raises(RuntimeError, match=match):
+        layer(dense(4, 64), dense(4, 8), workspace=aligned(4096))
+    with pytest.raises(RuntimeError, match=match):
+        layer(held("nvfp4", 4, 64, gx), dense(4, 8))
+
+
+def test_operands_on_the_host_are_refused():
+    """As a backend with a device does, before the library is called."""
+    be = Backend(plan_only_for=(148, 232448))
+    m, cache = held("mxfp4", 4, 64), mx.MxCache.allocate("nvfp4", 4, 8, 64, aligned)
+    layer = mx.MxLinear(be, held("mxfp4", 8, 64))
+    ints = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    be._device = 0
+    m_there = held("mxfp4", 4, 64)
+    m_there.device = 0
+    for call in (lambda: be.mx_quantise(dense(4, 64), m), lambda: be.mx_quantise(dense(4, 64), m_there),
+                 lambda: be.mx_dequantise(m, dense(4, 64)), lambda: be.mx_dequantise(m_there, dense(4, 64)),
+                 lambda: be.mx_cache_write(cache, dense(4, 64), ints(2, 3), ints(3)),
+                 lambda: be.mx_cache_read(cache, dense(4, 64), ints(2, 3), ints(3)),
+                 lambda: mx._fill_rows(mx.MxRows(), ints(2, 3), ints(3), None, 0),
+                 lambda: layer(dense(4, 64), dense(4, 8), workspace=aligned(4096)), lambda: layer(m, dense(4, 8)),
+                 lambda: mx.MxLinear(be, held("mxfp4", 8, 64))):
+        with pytest.raises(RuntimeError, match="is on the host, the backend on device 0"):
+            call()
+
+
 def test_null_arguments_are_errors():
     lib = mlvc_b200.lib()
     assert lib.mlvc_b200_mx_quantise(None, None, None, 0) == -1
