@@ -2,6 +2,14 @@
 //     y[m, n] = leaky(alpha * sum_k a[m, k] b[n, k] + bias[n]) + residual[m, n]
 // with a and b quantised along k, alpha the product of their tensor scales,
 // sums in 32 bits in tensor memory and one rounding to y's type.
+//
+// These are the tiles of calls that have too few for 256 x 256 ones by pairs
+// (mx_pair.cu) and too many for splitting k (mx_rows.cu): 300 x 4096 x 4096
+// nvfp4 takes 12 us with its quantising.  Operands are what bounds them: a panel
+// of 256 values brings 32 KB (128 x 128) or 24 KB (128 x 64) to an SM for products of
+// 256 or 128 cycles, and takes 0.38 us or 0.33 (700 and 600 cycles); beside it 3 us for
+// the first panel's way and the last results'.  So 128 x 64 wins only where it
+// leaves fewer SMs idle in the last round.
 #include "mx_epilogue.cuh"
 
 namespace mlvc_b200 {
