@@ -15,10 +15,11 @@
 // nvfp4: 221 us at full clock, 5.0 PFLOP/s, and 250 at the 1.46 GHz that remain);
 // at full clock the scales' copies, which the tensor core does not overlap with
 // products: a panel takes 600 cycles of mxfp4 and 700 of nvfp4, 512 of them
-// products; then the ends of tiles, about 2700 cycles each, and the last round's
-// idle pairs.  4096 x 14336 x 4096 mxfp4: 94 us, 5.1 PFLOP/s.  (Copies one tile
-// ahead, between the products: 353 us where a group before each panel took 307;
-// scales stored to TMEM from registers: 538.)
+// products; then the ends of tiles, about 2700 cycles each.  Where half of the pairs
+// would have no tile in the last round, all take halves of its tiles (a half takes
+// 0.8 of a tile's time: its operands come no faster).  4096 x 14336 x 4096 mxfp4:
+// 92 us, 5.2 PFLOP/s.  (Copies one tile ahead, between the products: 353 us where a
+// group before each panel took 307; scales stored to TMEM from registers: 538.)
 //
 // Warps: 0 copies (both CTAs, completing on the even CTA's barriers), 1 MMA
 // (even CTA), 2..9 empty the accumulators.
@@ -49,6 +50,19 @@ struct MxPairTile {
     static constexpr uint32_t kTx = 2 * (2 * kOperand + kSA + kSB);
 };
 
+// Tile `t` of a call: where it begins in tiles of 128 columns, and whether it is
+// half as wide.
+struct MxPairAt {
+    int mt, nt;
+    bool half;
+    __device__ __forceinline__ MxPairAt(const MxPairParams& p, int t)
+    {
+        half = t >= p.full;
+        mx_tile_at(p.m_tiles, p.n_tiles, half ? p.full + (t - p.full) / 2 : t, mt, nt);
+        nt = 2 * nt + (half ? (t - p.full) & 1 : 0);
+    }
+};
+
 template <int F>
 __device__ __forceinline__ void mx_pair(const MxPairParams& p)
 {
@@ -76,6 +90,7 @@ __device__ __forceinline__ void mx_pair(const MxPairParams& p)
     if (warp == 0 && elect_one()) {
         tma_prefetch_desc(&p.map_a);
         tma_prefetch_desc(&p.map_b);
+        tma_prefetch_desc(&p.map_b_half);
         tma_prefetch_desc(&p.map_sa);
         tma_prefetch_desc(&p.map_sb);
     }
@@ -89,7 +104,7 @@ __device__ __forceinline__ void mx_pair(const MxPairParams& p)
     tc_fence_after();
     pdl_launch_dependents();
     const uint32_t tmem = sh->tmem_base;
-    const int total = p.m_tiles * p.n_tiles;
+    const int total = p.total;
     bool issuer = false;
     uint32_t issued = 0;
 
@@ -99,8 +114,7 @@ __device__ __forceinline__ void mx_pair(const MxPairParams& p)
             int stage = 0;
             uint32_t phase = 0;
             for (int t = pair_id; t < total && !sh->abort_flag; t += pairs) {
-                int mt, nt;
-                mx_tile_at(p.m_tiles, p.n_tiles, t, mt, nt);
+                const MxPairAt at(p, t);
                 for (int k = 0; k < p.k.count; ++k) {
                     if (!mbar_wait(&sh->empty[stage], phase ^ 1u, &sh->abort_flag, kErrMxProducer))
                         break;
@@ -108,14 +122,17 @@ __device__ __forceinline__ void mx_pair(const MxPairParams& p)
                     const uint32_t bar = cluster_address(&sh->full[stage], 0);
                     // every box counts in full, rows and tiles outside are zeros
                     if (rank == 0) {
-                        mbar_arrive_expect_tx(&sh->full[stage], T::kTx);
+                        mbar_arrive_expect_tx(&sh->full[stage], at.half ? T::kTx - T::kOperand : T::kTx);
                         armed |= 1u << stage;
                         parity = (parity & ~(1u << stage)) | (phase << stage);
                     }
-                    tma_load_2d_pair(s, &p.map_a, bar, k * 128, mt * 256 + rank * 128);
-                    tma_load_2d_pair(s + T::kOperand, &p.map_b, bar, k * 128, nt * 256 + rank * 128);
-                    tma_load_3d_pair(s + 2 * T::kOperand, &p.map_sa, bar, 0, k * kWords, mt * 2 + rank);
-                    tma_load_3d_pair(s + 2 * T::kOperand + T::kSA, &p.map_sb, bar, 0, k * kWords, nt * 2);
+                    tma_load_2d_pair(s, &p.map_a, bar, k * 128, at.mt * 256 + rank * 128);
+                    if (at.half)
+                        tma_load_2d_pair(s + T::kOperand, &p.map_b_half, bar, k * 128, at.nt * 128 + rank * 64);
+                    else
+                        tma_load_2d_pair(s + T::kOperand, &p.map_b, bar, k * 128, at.nt * 128 + rank * 128);
+                    tma_load_3d_pair(s + 2 * T::kOperand, &p.map_sa, bar, 0, k * kWords, at.mt * 2 + rank);
+                    tma_load_3d_pair(s + 2 * T::kOperand + T::kSA, &p.map_sb, bar, 0, k * kWords, at.nt);
                     if (++stage == T::kStages) {
                         stage = 0;
                         phase ^= 1u;
@@ -133,7 +150,6 @@ __device__ __forceinline__ void mx_pair(const MxPairParams& p)
     } else if (warp == 1) {
         if (rank == 0 && elect_one()) {
             issuer = true;
-            constexpr uint32_t idesc = mx_idesc<F>(256, 256);
             const uint32_t tmem_sa = tmem + 448, tmem_sb = tmem_sa + 4 * kWords;
             // descriptors differ by their start addresses (16-byte units) alone
             const uint64_t a_desc = smem_desc(smem_u32(stages), 16, 1024, 2);
@@ -147,6 +163,8 @@ __device__ __forceinline__ void mx_pair(const MxPairParams& p)
                     break;
                 tc_fence_after();
                 const uint32_t d = tmem + (tile & 1u) * 192;
+                const bool half = t >= p.full;
+                const uint32_t idesc = half ? mx_idesc<F>(256, 128) : mx_idesc<F>(256, 256);
                 for (int k = 0; k < p.k.count; ++k) {
                     if (!mbar_wait(&sh->full[stage], phase, &sh->abort_flag, kErrMxMma)) {
                         ok = false;
@@ -163,7 +181,8 @@ __device__ __forceinline__ void mx_pair(const MxPairParams& p)
                             break;
                         tmem_copy_scales_pair(tmem_sa + 4 * w, sa + 32 * w);
                         tmem_copy_scales_pair(tmem_sb + 8 * w, sb + 32 * w);
-                        tmem_copy_scales_pair(tmem_sb + 8 * w + 4, sb + (T::kSA >> 4) + 32 * w);
+                        if (!half)
+                            tmem_copy_scales_pair(tmem_sb + 8 * w + 4, sb + (T::kSA >> 4) + 32 * w);
                     }
 #pragma unroll
                     for (int ks = 0; ks < 4; ++ks) {
@@ -194,20 +213,25 @@ __device__ __forceinline__ void mx_pair(const MxPairParams& p)
             Out rows;
             uint32_t tile = 0;
             for (int t = pair_id; t < total; t += pairs, ++tile) {
-                int mt, nt;
-                mx_tile_at(p.m_tiles, p.n_tiles, t, mt, nt);
+                const MxPairAt tile_at(p, t);
                 const bool odd = tile & 1u;
-                const int col0 = nt * 256 - (odd ? 192 : 0);  // of TMEM column 0
-                rows.set_rows(p.e, static_cast<long long>(mt) * 256 + rank * 128 + quadrant * 32, p.e.M);
+                const int first = odd ? 192 : 0, col0 = tile_at.nt * 128 - first;  // of TMEM column 0
+                rows.set_rows(p.e, static_cast<long long>(tile_at.mt) * 256 + rank * 128 + quadrant * 32, p.e.M);
+                // the shared columns 192..255 first; a half is the last tile of its CTAs
+                const int chunks = tile_at.half ? 2 : 4;
+                auto chunk_at = [&](int c) {
+                    return tile_at.half ? first + 64 * group + 32 * c
+                           : c == 0     ? 192 + 32 * group
+                                        : (odd ? 256 : 0) + 96 * group + 32 * (c - 1);
+                };
                 typename Out::Asked asked;
-                rows.ask(p.e, col0 + 192 + 32 * group, asked);
+                rows.ask(p.e, col0 + chunk_at(0), asked);
                 // the whole warp goes on or none of it: the TMEM loads are collective
                 if (!__all_sync(0xFFFFFFFFu, mbar_wait(&sh->sums, tile & 1u, &sh->abort_flag, kErrMxEpilogue)))
                     break;
                 tc_fence_after();
-                for (int c = 0; c < 4; ++c) {
-                    // the shared columns 192..255 first
-                    const int at = c == 0 ? 192 + 32 * group : (odd ? 256 : 0) + 96 * group + 32 * (c - 1);
+                for (int c = 0; c < chunks; ++c) {
+                    const int at = chunk_at(c);
                     if (c)
                         rows.ask(p.e, col0 + at, asked);
                     rows.empty(p.e, asked, turn, tmem + at + (static_cast<uint32_t>(quadrant * 32) << 16), col0 + at, [&] {

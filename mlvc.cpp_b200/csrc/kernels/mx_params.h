@@ -79,12 +79,14 @@ struct MxGemmParams {
 
 // Products in 256 x 256 tiles by pairs of CTAs (see mx_pair).
 struct MxPairParams {
-    CUtensorMap map_a, map_b;          // bytes [rows, pitch], boxes of 128 bytes x 128 rows, 128-byte swizzle
+    // bytes [rows, pitch], boxes of 128 bytes x 128 rows (map_b_half: 64), 128-byte swizzle
+    CUtensorMap map_a, map_b, map_b_half;
     // scale tiles as 16-bit values [bands, tiles of a band, 256]; boxes of a
     // panel's tiles, one band of A and two of B
     CUtensorMap map_sa, map_sb;
     MxPanels k;
     int m_tiles, n_tiles;
+    int full, total;                   // tiles of 256 x 256; those and the halves (256 x 128) of the others
     MxEpilogue e;
 };
 

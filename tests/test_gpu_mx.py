@@ -231,6 +231,14 @@ def test_linear_large(be, fmt, shape):
     check_linear(z, x, w, fmt, gx, gw, out, bias, 0.25, residual)
 
 
+@pytest.mark.parametrize("shape", [(3300, 130, 3200), (3300, 520, 3335), (2560, 96, 2432)])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_linear_last_round(be, fmt, shape):
+    """169, 182 and 100 tiles of 256 x 256: a last round of narrower ones after one
+    or two, some wholly past the last output."""
+    test_linear_large(be, fmt, shape)
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_linear_large_strides(be, fmt):
     """Many rows, as parts of wider matrices, on and off wide boundaries; nothing
