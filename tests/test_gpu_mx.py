@@ -239,6 +239,53 @@ def test_linear_last_round(be, fmt, shape):
     test_linear_large(be, fmt, shape)
 
 
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("shape", [(24, 4096, 4096), (48, 1000, 14336), (300, 2048, 4096), (200, 640, 1000), (2500, 300, 2600)])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_linear_right_after_its_weights(be, fmt, shape, captured):
+    """Weights quantised into one buffer and used at once, several times over: no
+    copy of a call's weights may begin before they are there, and none of its rows
+    before the call before has read the workspace."""
+    m, k, n = shape
+    gen = torch.Generator("cuda").manual_seed(m)
+    ws = [torch.randn(n, k, device="cuda", generator=gen).bfloat16() for _ in range(4)]
+    xs = [torch.randn(m, k, device="cuda", generator=gen).bfloat16() for _ in range(4)]
+    weight = MxMatrix.allocate(fmt, n, k, alloc)
+    layer = MxLinear(be, weight)
+    work = alloc(layer.workspace_bytes(m))
+    want = []
+    for x, w in zip(xs, ws):
+        apart = MxLinear(be, quantised(be, w, fmt, 1.0))
+        y = torch.empty(m, n, device="cuda")
+        torch.cuda.synchronize()
+        apart(quantised(be, x, fmt, 1.0), y, stream=0)
+        torch.cuda.synchronize()
+        want.append(y)
+    got = [torch.zeros(m, n, device="cuda") for _ in ws]
+    side = torch.cuda.Stream()
+
+    def calls():
+        stream = torch.cuda.current_stream().cuda_stream
+        for x, w, y in zip(xs, ws, got):
+            be.mx_quantise(w, weight, stream=stream)
+            layer(x, y, workspace=work, stream=stream)
+
+    torch.cuda.synchronize()
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            calls()
+        for _ in range(5):
+            graph.replay()
+    else:
+        with torch.cuda.stream(side):
+            for _ in range(5):
+                calls()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_linear_large_strides(be, fmt):
     """Many rows, as parts of wider matrices, on and off wide boundaries; nothing
