@@ -11,9 +11,11 @@
 4. nvcc compiles csrc/noalloc/*.cu (host and device code, CUDA runtime API)
    into an object linked with the static CUDA runtime, so the library still
    has no link-time dependency on libcudart or libcuda.
+5. g++ compiles csrc/python/calls.cpp, the package's extension for calls on
+   microscaled operands, for the interpreter that runs this.
 
-Outputs: mlvc.cpp_b200/lib/libmlvc_b200.so (git-ignored, travels with the
-repository snapshot to the GPU machine).  Usage: python mlvc.cpp_b200/build.py
+Outputs: mlvc.cpp_b200/lib/libmlvc_b200.so and mlvc.cpp_b200/mlvc_b200/_calls.so
+(git-ignored, travel with the repository snapshot to the GPU machine).  Usage: python mlvc.cpp_b200/build.py
 """
 
 from __future__ import annotations
@@ -22,6 +24,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -30,6 +33,7 @@ ROOT = HERE.parent
 CUDA = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
 BUILD = HERE / "_build"
 LIB = HERE / "lib" / "libmlvc_b200.so"
+CALLS = HERE / "mlvc_b200" / "_calls.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -48,9 +52,9 @@ def sources():
 
 
 def up_to_date():
-    if not LIB.exists():
+    if not LIB.exists() or not CALLS.exists():
         return False
-    t = LIB.stat().st_mtime
+    t = min(LIB.stat().st_mtime, CALLS.stat().st_mtime)
     return all(p.stat().st_mtime <= t for p in sources())
 
 
@@ -95,6 +99,10 @@ def build(force=False, verbose=False):
           f"-L{CUDA / 'lib64'}", "-lcudart_static", "-lrt", "-lpthread",
           "-ldl", "-o", str(tmp)])
     os.replace(tmp, LIB)
+    tmp = CALLS.with_suffix(".so.tmp")
+    _run([cxx, "-std=c++20", "-O2", "-fPIC", "-shared", "-Wall", f"-I{ROOT / 'include'}",
+          f"-I{sysconfig.get_paths()['include']}", str(HERE / "csrc" / "python" / "calls.cpp"), "-o", str(tmp)])
+    os.replace(tmp, CALLS)
     if verbose:
         print(out)
     return LIB

@@ -123,6 +123,7 @@ def lib():
             f = getattr(l, name)
             f.argtypes = args
             f.restype = res
+        mx.connect(l)
         _lib = l
     return _lib
 
@@ -151,7 +152,6 @@ class Backend:
         if debug_tensors:
             _check(lib().mlvc_b200_set_debug_tensors(self._h, 1))
         self._in, self._out = [], []
-        self._calls = mx.Calls()
         self._device = device_id if plan_only_for is None else None  # operands' device
 
     def close(self):
@@ -272,47 +272,33 @@ class Backend:
     # ------------------------------------------------------ microscaled
     def mx_quantise(self, x, out, stream=None):
         """Quantises the dense matrix x into the MxMatrix `out` of its shape."""
-        c = self._calls
         if out.device != self._device:
             mx._check_device(out.device, self._device, "the quantised matrix")
-        mx._fill(c.matrix, x, self._device)
-        if _lib.mlvc_b200_mx_quantise(self._h, c.matrix_ref, out.ref, self.stream or 0 if stream is None else stream):
-            _check(-1)
+        mx.calls.convert(False, self._h.value, x, out.address, self.stream or 0 if stream is None else stream, self._device)
 
     def mx_dequantise(self, m, y, stream=None):
         """Reads the MxMatrix m back into the dense matrix y of its shape."""
-        c = self._calls
         if m.device != self._device:
             mx._check_device(m.device, self._device, "the quantised matrix")
-        mx._fill(c.matrix, y, self._device)
-        if _lib.mlvc_b200_mx_dequantise(self._h, m.ref, c.matrix_ref, self.stream or 0 if stream is None else stream):
-            _check(-1)
+        mx.calls.convert(True, self._h.value, y, m.address, self.stream or 0 if stream is None else stream, self._device)
 
     def mx_cache_write(self, cache, x, pages, offsets, starts=None, stream=None):
         """Quantises the packed rows of several sequences into their places:
         rows offsets[s] .. offsets[s + 1] of x become positions starts[s] ... of
         sequence s, whose pages are pages[s] (device int32 arrays [sequences,
         pages], [sequences + 1], [sequences]; starts None: all zero)."""
-        c = self._calls
         if cache.device != self._device:
             mx._check_device(cache.device, self._device, "the cache")
-        mx._fill(c.matrix, x, self._device)
-        mx._fill_rows(c.rows, pages, offsets, starts, self._device)
-        if _lib.mlvc_b200_mx_cache_write(self._h, cache.ref, c.matrix_ref, c.rows_ref,
-                                         self.stream or 0 if stream is None else stream):
-            _check(-1)
+        mx.calls.cache(False, self._h.value, cache.address, x, pages, offsets, starts,
+                       self.stream or 0 if stream is None else stream, self._device)
 
     def mx_cache_read(self, cache, y, pages, offsets, starts=None, stream=None):
         """Reads packed rows back into the dense matrix y, addressed as in
         mx_cache_write; rows that have no place are zeros."""
-        c = self._calls
         if cache.device != self._device:
             mx._check_device(cache.device, self._device, "the cache")
-        mx._fill(c.matrix, y, self._device)
-        mx._fill_rows(c.rows, pages, offsets, starts, self._device)
-        if _lib.mlvc_b200_mx_cache_read(self._h, cache.ref, c.matrix_ref, c.rows_ref,
-                                        self.stream or 0 if stream is None else stream):
-            _check(-1)
+        mx.calls.cache(True, self._h.value, cache.address, y, pages, offsets, starts,
+                       self.stream or 0 if stream is None else stream, self._device)
 
     # ----------------------------------------------------------- slots
     def configure_slots(self, n):

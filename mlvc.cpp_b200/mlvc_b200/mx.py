@@ -22,12 +22,14 @@ non-finite values and cache rows without a place hold here too:
 from __future__ import annotations
 
 import ctypes
-import struct
 from typing import NamedTuple
 
 FORMATS = {"mxfp4": 0, "nvfp4": 1, "mxfp8": 2}
 _DTYPES = {"float16": 0, "bfloat16": 2, "float32": 3}
 _dtype_codes = {}  # dtype object -> code
+_int32 = set()     # dtype objects known to be int32
+
+calls = None  # the extension that describes operands and makes the calls
 
 
 class Matrix(ctypes.Structure):
@@ -82,9 +84,21 @@ def _code(dtype):
     return code
 
 
-# A Matrix at once: a call on few rows takes little longer than its description.
-_pack_matrix = struct.Struct("=Qiiqqqq").pack_into
-_pack_rows = struct.Struct("=QqQQq").pack_into
+def _is_int32(dtype):
+    if str(dtype).rsplit(".", 1)[-1] != "int32":
+        return False
+    _int32.add(dtype)
+    return True
+
+
+def connect(lib):
+    """Gives the extension the loaded library's entry points."""
+    global calls
+    from . import _calls
+    names = ("mx_quantise", "mx_dequantise", "mx_cache_write", "mx_cache_read", "mx_linear", "last_error")
+    _calls.connect(tuple(ctypes.cast(getattr(lib, "mlvc_b200_" + n), ctypes.c_void_p).value for n in names),
+                   _dtype_codes, _code, _int32, _is_int32)
+    calls = _calls
 
 
 def _device(t):
@@ -101,51 +115,10 @@ def _check_device(at, device, what):
                            f"device {device}")
 
 
-def _elsewhere(t, device):
-    """Whether `t` is known to be on another device (inlined in _fill, once a
-    dense operand: calls on few rows are as long as the host takes for them)."""
-    try:
-        return t.get_device() != device
-    except AttributeError:
-        return False
-
-
-def _fill(m, t, device):
-    """Describes the matrix `t` in the structure `m`."""
-    shape = t.shape
-    if len(shape) != 2:
-        raise RuntimeError(f"mlvc-b200: a dense matrix has two dimensions, not {len(shape)}")
-    code = _dtype_codes.get(t.dtype)
-    if code is None:
-        code = _code(t.dtype)
-    if device is not None:
-        try:
-            if t.get_device() != device:
-                _check_device(t.get_device(), device, "a dense matrix")
-        except AttributeError:
-            pass
-    _pack_matrix(m, 0, t.data_ptr(), code, 0, *shape, *t.stride())
-
-
 def _format(name):
     if name not in FORMATS:
         raise RuntimeError(f"mlvc-b200: unknown microscaled format {name!r}")
     return FORMATS[name]
-
-
-_int32 = set()  # dtype objects known to be int32
-
-
-def _ints(t, what, dims, device):
-    """Shape of a contiguous int32 device array."""
-    shape = t.shape
-    if t.dtype not in _int32 and str(t.dtype).rsplit(".", 1)[-1] == "int32":
-        _int32.add(t.dtype)
-    if t.dtype not in _int32 or len(shape) != dims or not t.is_contiguous():
-        raise RuntimeError(f"mlvc-b200: {what} must be a contiguous int32 array of {dims} dimension(s)")
-    if device is not None and _elsewhere(t, device):
-        _check_device(t.get_device(), device, what)
-    return shape
 
 
 def _room(buffer, need, what):
@@ -186,7 +159,7 @@ class MxMatrix:
         self.data, self.scales = data, scales
         self.device = _held_device(data, scales)
         self.c = MxMatrixC(_format(format), tensor_scale, rows, cols, data.data_ptr(), scales.data_ptr())
-        self.ref = ctypes.byref(self.c)
+        self.address = ctypes.addressof(self.c)
 
     @staticmethod
     def layout(format, rows, cols):
@@ -212,7 +185,7 @@ class MxCache:
         self.tensor_scale, self.data, self.scales = float(tensor_scale), data, scales
         self.device = _held_device(data, scales)
         self.c = MxCacheC(_format(format), tensor_scale, pages, page_rows, cols, data.data_ptr(), scales.data_ptr())
-        self.ref = ctypes.byref(self.c)
+        self.address = ctypes.addressof(self.c)
 
     @staticmethod
     def layout(format, pages, page_rows, cols):
@@ -223,25 +196,6 @@ class MxCache:
         """With buffers from alloc(bytes)."""
         lay = cls.layout(format, pages, page_rows, cols)
         return cls(format, pages, page_rows, cols, alloc(lay.data_bytes), alloc(lay.scale_bytes), tensor_scale, lay)
-
-
-def _fill_rows(r, pages, offsets, starts, device):
-    """Describes where packed rows lie (see mlvc_b200_mx_rows) in the structure `r`."""
-    sequences, per_sequence = _ints(pages, "the page table", 2, device)
-    if _ints(offsets, "offsets", 1, device)[0] != sequences + 1 or (
-            starts is not None and _ints(starts, "starts", 1, device)[0] != sequences):
-        raise RuntimeError("mlvc-b200: offsets has one entry more than there are sequences, starts as many")
-    _pack_rows(r, 0, pages.data_ptr(), per_sequence, offsets.data_ptr(), 0 if starts is None else starts.data_ptr(),
-               sequences)
-
-
-class Calls:
-    """A backend's descriptions of the operands of a call, filled anew by each
-    (calls on one backend come from one host thread at a time)."""
-
-    def __init__(self):
-        self.matrix, self.rows = Matrix(), MxRows()
-        self.matrix_ref, self.rows_ref = ctypes.byref(self.matrix), ctypes.byref(self.rows)
 
 
 class MxLinear:
@@ -260,14 +214,12 @@ class MxLinear:
         if bias is not None:
             _check_device(_device(bias), backend._device, "bias")
         self._keep = (weight, bias)
-        self._check, self._lib = _check, lib()
-        self._call, self._backend = self._lib.mlvc_b200_mx_linear, backend
+        self._check, self._lib, self._backend = _check, lib(), backend
         a = self._args = LinearArgs()
         a.w = weight.c
         a.bias = bias.data_ptr() if bias is not None else 0
         a.slope, a.tensor_scale = slope, tensor_scale
-        self._x, self._a, self._y, self._residual = a.x, a.a, a.y, a.residual  # views
-        self._ref = ctypes.byref(a)
+        self._address = ctypes.addressof(a)
 
     def workspace_bytes(self, rows):
         """Bytes of workspace that a call on `rows` dense rows needs."""
@@ -279,27 +231,11 @@ class MxLinear:
         """x: dense [rows, inputs], or an MxMatrix of the weight's format; y and
         residual: dense [rows, outputs] of one type.  Dense x needs a workspace
         (256-byte boundary) that nothing else uses until the call's work is done."""
-        a, device = self._args, self._backend._device
+        backend, held = self._backend, None
         if isinstance(x, MxMatrix):
-            if x.device != device:
-                _check_device(x.device, device, "x")
-            a.a = x.c
-            self._x.data = 0
-        else:
-            if self._a.data:
-                self._a.data = 0
-            _fill(self._x, x, device)
-        _fill(self._y, y, device)
-        if residual is not None:
-            _fill(self._residual, residual, device)
-        elif self._residual.data:
-            self._residual.data = 0
-        if workspace is not None:
-            if device is not None and _elsewhere(workspace, device):
-                _check_device(workspace.get_device(), device, "the workspace")
-            a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.nbytes
-        elif a.workspace:
-            a.workspace = a.workspace_bytes = 0
-        if self._call(self._backend._h, self._ref, self._backend.stream or 0 if stream is None else stream):
-            self._check(-1)
+            if x.device != backend._device:
+                _check_device(x.device, backend._device, "x")
+            held = x.address
+        calls.linear(backend._h.value, self._address, x, y, residual, workspace,
+                     backend.stream or 0 if stream is None else stream, backend._device, held)
         return y

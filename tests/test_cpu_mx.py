@@ -202,17 +202,41 @@ def test_operands_on_the_host_are_refused():
     layer = mx.MxLinear(be, held("mxfp4", 8, 64))
     ints = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
     be._device = 0
-    m_there = held("mxfp4", 4, 64)
-    m_there.device = 0
+    m_there, cache_there = held("mxfp4", 4, 64), mx.MxCache.allocate("nvfp4", 4, 8, 64, aligned)
+    m_there.device = cache_there.device = 0
+
+    class There:
+        """An operand that says that it is on device 0."""
+
+        def __init__(self, t):
+            self.t = t
+
+        def __getattr__(self, name):
+            return getattr(self.t, name)
+
+        def get_device(self):
+            return 0
+
+    x_there, y_there = There(dense(4, 64)), There(dense(4, 8))
     for call in (lambda: be.mx_quantise(dense(4, 64), m), lambda: be.mx_quantise(dense(4, 64), m_there),
                  lambda: be.mx_dequantise(m, dense(4, 64)), lambda: be.mx_dequantise(m_there, dense(4, 64)),
                  lambda: be.mx_cache_write(cache, dense(4, 64), ints(2, 3), ints(3)),
                  lambda: be.mx_cache_read(cache, dense(4, 64), ints(2, 3), ints(3)),
-                 lambda: mx._fill_rows(mx.MxRows(), ints(2, 3), ints(3), None, 0),
+                 lambda: be.mx_cache_write(cache_there, dense(4, 64), ints(2, 3), ints(3)),
+                 lambda: be.mx_cache_read(cache_there, x_there, ints(2, 3), ints(3)),
+                 lambda: be.mx_cache_read(cache_there, x_there, There(ints(2, 3)), ints(3)),
+                 lambda: be.mx_cache_read(cache_there, x_there, There(ints(2, 3)), There(ints(3)), starts=ints(2)),
+                 lambda: layer(x_there, dense(4, 8), workspace=There(aligned(4096))),
+                 lambda: layer(x_there, y_there, residual=dense(4, 8), workspace=There(aligned(4096))),
+                 lambda: layer(x_there, y_there, workspace=aligned(4096)),
                  lambda: layer(dense(4, 64), dense(4, 8), workspace=aligned(4096)), lambda: layer(m, dense(4, 8)),
                  lambda: mx.MxLinear(be, held("mxfp4", 8, 64))):
         with pytest.raises(RuntimeError, match="is on the host, the backend on device 0"):
             call()
+    with pytest.raises(RuntimeError, match="planning-only"):
+        layer(x_there, y_there, workspace=There(aligned(4096)))
+    with pytest.raises(RuntimeError, match="planning-only"):
+        be.mx_cache_read(cache_there, x_there, There(ints(2, 3)), There(ints(3)), starts=There(ints(2)))
 
 
 def test_null_arguments_are_errors():
