@@ -2,8 +2,9 @@
 // with data_ptr(), and for matrices shape, stride() and dtype) and makes it.
 //
 // A call on few rows takes a few microseconds on the device, and describing its
-// operands attribute by attribute in Python took as long: two 16-bit rows
-// written to a cache and read back 14.6 us a pass, 8.4 a linear layer's row.
+// operands attribute by attribute in Python took as long: two streams' rows
+// written to a cache and read back 14.6 us a pass (here 11.4), a linear layer on
+// one row 8.4 (7.1).
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
